@@ -1,0 +1,753 @@
+// Attention over pages of keys and values in 4 bits (fp4.h), for one head size (LS_HEAD_DIM, a multiple of 32).
+//
+// Query rows of request b are the packed rows offsets[b] .. offsets[b + 1] - 1; the last of them stands at position
+// lengths[b] - 1.  A row at position p attends to the keys 0 .. p of its request, with a window w to p - w + 1 .. p:
+//   out = sum_t e^(c q.k_t - m) v_t / sum_t e^(c q.k_t - m),   m = max_t c q.k_t.
+// The g query heads of a key/value head are rows of one product: row r of a request is head r % g of its token r / g.
+//
+// A wave holds NT tiles of 16 query rows and walks the keys in tiles of 32.  It computes S^T = K Q^T and then
+// O^T += V^T P^T, both on the matrix units (16x16x32, bfloat16 operands, sums in 32 bits): the scores of S^T lie in the
+// registers of just the lane that has to bring them to the second product, so neither the keys and values nor the
+// weights pass through LDS.  Codes become bfloat16 operands exactly, two an instruction with their scale.  The
+// softmax keeps a reference instead of the maximum: a row's reference moves only when a score passes it by more than 8
+// (powers of two: weights up to 256), so most tiles do not touch the sums; weights are held in 32 bits, added up as they
+// are and rounded to bfloat16 for the product (half a step of 2^-8 each, as the queries' own type has it).
+// The float32 path has queries and weights as three bfloat16 terms each (24 bits together): every product of a term with
+// a key or value is exact, so the sums are those of 32-bit operands.
+//
+// Requests of at most 16 rows a head (decoded tokens): a workgroup's four waves take the key tiles of one split in turn
+// and fold at the end through LDS.  Others (prompts): every wave has a block of rows of its own.  In both a request's keys
+// are cut into splits by a rule of its own length (and rows) alone; where there are several, they leave sums that a second
+// launch folds in ascending order.  So a row's result does not depend on what else is in the step.
+//
+// What bounds it: decoding reads 17/32 bytes a key element from HBM and spends about 1.2 vector instructions on each, some
+// two thirds of what the memory leaves room for; prompts are bound by the vector unit's softmax next to the matrix units.
+
+#include "fp4.h"
+#include "fp4_attention_api.h"
+
+#include <type_traits>
+
+#ifndef LS_HEAD_DIM
+#error "LS_HEAD_DIM must be defined"
+#endif
+
+namespace ls {
+
+constexpr int D = LS_HEAD_DIM;
+static_assert(D % 32 == 0 && D >= 32 && D <= 256, "head sizes are multiples of 32 up to 256");
+
+// A head is cut into sections of 128, 64 and 32 elements: section s has E(s) elements a lane column (16 columns).
+constexpr int kSections = D / 128 + (D % 128 >= 64) + (D % 64 >= 32);
+__host__ __device__ constexpr int section_elems(int s) { return s < D / 128 ? 8 : (s == D / 128 && D % 128 >= 64) ? 4 : 2; }
+__host__ __device__ constexpr int section_dim(int s) {
+  int at = 0;
+  for (int i = 0; i < s; ++i) at += 16 * section_elems(i);
+  return at;
+}
+
+constexpr int kTileKeys = 32;
+constexpr int kThreads = 256;
+constexpr float kSlack = 8.f;  // how far a score may pass the reference, in powers of two
+constexpr float kToLog2 = 1.4426950408889634f;
+
+template <typename T> constexpr int kTerms = std::is_same_v<T, float> ? 3 : 1;
+// Row tiles a wave holds where every wave has rows of its own: what its registers allow.
+template <typename T> constexpr int kPromptTiles = std::is_same_v<T, float> ? (D <= 64 ? 2 : 1) : (D <= 64 ? 4 : D <= 128 ? 2 : 1);
+
+// Keys a split of a request of few rows covers, by how many keys its rows see.
+__host__ __device__ inline int decode_split(int span) {
+  if (span <= 4096) return 256;
+  if (span <= 32768) return 512;
+  return 1024 * ((span + 131071) / 131072);
+}
+constexpr int kPromptBlocks = 32;  // row blocks times splits that a request's head is cut into, about
+__host__ __device__ inline int prompt_split(int span, int blocks) {
+  const int want = max(1, kPromptBlocks / max(1, blocks));
+  return max(512, ((span + want - 1) / want + kTileKeys - 1) / kTileKeys * kTileKeys);
+}
+
+struct Fp4Args {
+  const void* q;
+  long ldq;
+  void* out;
+  long ldo;
+  Fp4Pool pool;
+  const int* table;
+  int columns;
+  const int* offsets;
+  const int* lengths;
+  int requests, rows;      // rows: of q and out
+  int group;               // query heads a key/value head
+  float factor;            // scale * log2(e)
+  int window;
+  float* part_acc;         // [requests * kv heads][region][D]
+  float* part_ml;          // [requests * kv heads][region][2]
+  int region;
+  int few;                 // rows a head up to which a request belongs to the decoding kernel
+};
+
+// One request as all kernels see it.
+struct Request {
+  int first, rows, start, base, end;  // first packed row, rows a head, first position, keys that are seen: base .. end - 1
+  __device__ __forceinline__ Request(const Fp4Args& a, int b) {
+    const int from = a.offsets[b], to = a.offsets[b + 1];
+    const bool ok = from >= 0 && to >= from && to <= a.rows;
+    first = ok ? from : 0;
+    const int n = ok ? to - from : 0;
+    rows = n * a.group;
+    const int room = (int)min((long)a.columns << a.pool.page_shift, 0x7fffffffl);
+    end = min(max(a.lengths[b], 0), room);
+    start = end - n;
+    base = a.window > 0 ? max(0, start - a.window + 1) & ~(kTileKeys - 1) : 0;
+  }
+};
+
+struct KeyTile {  // what a lane has of 32 keys and values, as they lie in the pages
+  unsigned int k[2][D / 32];
+  unsigned int v[2][kSections][4];
+  unsigned int ks[2][kSections], vs[2][kSections];
+  bool good[2];  // the block of four tokens of this lane's values has a page
+};
+
+__device__ __forceinline__ void load_words(unsigned int* to, const unsigned char* from, int n) {
+  if (n == 4) {
+    const auto w = *reinterpret_cast<const __attribute__((ext_vector_type(4))) unsigned int*>(from);
+    to[0] = w[0]; to[1] = w[1]; to[2] = w[2]; to[3] = w[3];
+  } else if (n == 2) {
+    const auto w = *reinterpret_cast<const __attribute__((ext_vector_type(2))) unsigned int*>(from);
+    to[0] = w[0]; to[1] = w[1];
+  } else {
+    to[0] = *reinterpret_cast<const unsigned int*>(from);
+  }
+}
+
+struct PageIds {
+  int k[2], v[2];
+};
+
+__device__ __forceinline__ PageIds load_ids(const Fp4Args& a, const int* __restrict__ row, int t0, int lane) {
+  PageIds ids;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int k_at = (t0 + 16 * s + (lane & 15)) >> a.pool.page_shift, v_at = (t0 + 16 * s + 4 * (lane >> 4)) >> a.pool.page_shift;
+    ids.k[s] = row[min(k_at, a.columns - 1)];
+    ids.v[s] = row[min(v_at, a.columns - 1)];
+  }
+  return ids;
+}
+
+__device__ __forceinline__ void load_tile(KeyTile& tile, const Fp4Args& a, const PageIds& ids, int head, int t0, int lane) {
+  const int n = lane & 15, j = lane >> 4, mask = (1 << a.pool.page_shift) - 1;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const bool k_ok = ids.k[s] >= 0 && ids.k[s] < a.pool.pages, v_ok = ids.v[s] >= 0 && ids.v[s] < a.pool.pages;
+    const long k_row = (((long)(k_ok ? ids.k[s] : 0) * a.pool.kv_heads + head) << a.pool.page_shift) + ((t0 + 16 * s + n) & mask);
+    const long v_blk = ((((long)(v_ok ? ids.v[s] : 0) * a.pool.kv_heads + head) << a.pool.page_shift) + ((t0 + 16 * s + 4 * j) & mask)) >> 2;
+    tile.good[s] = v_ok;
+    const unsigned char* kc = a.pool.k_codes + k_row * (D / 2);
+    const unsigned char* ks = a.pool.k_scales + k_row * (D / 32);
+    const unsigned char* vc = a.pool.v_codes + v_blk * (2 * D);
+    const unsigned char* vs = a.pool.v_scales + v_blk * (D / 8);
+#pragma unroll
+    for (int c = 0; c < kSections; ++c) {
+      const int e = section_elems(c), dim = section_dim(c);
+      load_words(&tile.k[s][dim / 32], kc + dim / 2 + j * 2 * e, e / 2);
+      tile.ks[s][c] = ks[(dim + j * 4 * e) / 32];
+      load_words(tile.v[s][c], vc + (dim + n * e) / 8 * 16, 4);
+      load_words(&tile.vs[s][c], vs + (dim + n * e) / 32 * 4, 1);
+    }
+  }
+}
+
+template <typename T> __device__ __forceinline__ float weight_exp2(float x);
+template <> __device__ __forceinline__ float weight_exp2<float>(float x) { return exp2f(x); }
+template <> __device__ __forceinline__ float weight_exp2<bf16_t>(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ bf16x8 as_operand(unsigned int a, unsigned int b, unsigned int c, unsigned int d) {
+  typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
+  return __builtin_bit_cast(bf16x8, u32x4{a, b, c, d});
+}
+
+// The rows of a wave: NT tiles of 16, a lane has column lane % 16 of each.
+template <typename T, int NT>
+struct Rows {
+  bf16x8 q[kTerms<T>][NT][D / 32];
+  f32x4 acc[NT][D / 16];
+  float m[NT], l[NT];
+  int last[NT], low[NT];       // the keys low .. last are seen by the lane's row (last < low: none)
+  int any_last, all_last;      // uniform: the largest and the smallest `last` of the rows there are
+  int any_low, all_low;        // the smallest and the largest `low`
+
+  __device__ __forceinline__ void init(const Fp4Args& a, const Request& rq, int head, int row0, int lane) {
+    any_last = -1; all_last = 0x7fffffff; any_low = 0x7fffffff; all_low = 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int r = row0 + 16 * t + (lane & 15);
+      const bool there = r < rq.rows;
+      const int token = there ? r / a.group : 0, sub = there ? r - token * a.group : 0;
+      last[t] = there ? rq.start + token : -1;
+      low[t] = there && a.window > 0 ? max(0, last[t] - a.window + 1) : 0;
+      const T* from = static_cast<const T*>(a.q) + (long)(rq.first + token) * a.ldq + (long)(head * a.group + sub) * D;
+#pragma unroll
+      for (int c = 0; c < kSections; ++c) {
+        const int e = section_elems(c), dim = section_dim(c);
+#pragma unroll
+        for (int i = 0; i < e / 2; ++i) {
+          const T* p = from + dim + (lane >> 4) * 4 * e + 8 * i;
+          float x[8];
+          if (there) {
+            if constexpr (sizeof(T) == 2) {
+              typedef unsigned int any4 __attribute__((ext_vector_type(4), aligned(2)));
+              const any4 w = *reinterpret_cast<const any4*>(p);
+              q[0][t][dim / 32 + i] = as_operand(w[0], w[1], w[2], w[3]);
+            } else {
+              typedef float any4 __attribute__((ext_vector_type(4), aligned(4)));
+              const any4 u = *reinterpret_cast<const any4*>(p), w = *reinterpret_cast<const any4*>(reinterpret_cast<const float*>(p) + 4);
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                x[y] = u[y];
+                x[4 + y] = w[y];
+              }
+            }
+          } else {
+            q[0][t][dim / 32 + i] = as_operand(0, 0, 0, 0);
+#pragma unroll
+            for (int y = 0; y < 8; ++y) x[y] = 0.f;
+          }
+          if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+              float rest = x[y];
+#pragma unroll
+              for (int term = 0; term < 3; ++term) {
+                const bf16_t part = static_cast<bf16_t>(rest);
+                q[term][t][dim / 32 + i][y] = part;
+                rest = rest - static_cast<float>(part);
+              }
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) acc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m[t] = -INFINITY;
+      l[t] = 0.f;
+    }
+    // uniform bounds: rows are in the order of their positions
+    const int row_end = min(row0 + 16 * NT, rq.rows);
+    if (row0 < row_end) {
+      all_last = rq.start + row0 / a.group;
+      any_last = rq.start + (row_end - 1) / a.group;
+      any_low = a.window > 0 ? max(0, all_last - a.window + 1) : 0;
+      all_low = a.window > 0 ? max(0, any_last - a.window + 1) : 0;
+    }
+  }
+
+  // 32 keys from t0 on.
+  __device__ __forceinline__ void step(const Fp4Args& a, KeyTile& tile, int t0, int lane) {
+    const int n = lane & 15, j = lane >> 4;
+    const bool whole = t0 >= all_low && t0 + kTileKeys - 1 <= all_last && __ballot(!(tile.good[0] && tile.good[1])) == 0ull;
+    if (!whole) {
+      // what lies where no row looks may be anything: its values become zeros
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int key = t0 + 16 * s + 4 * j + y;
+          const bool seen = tile.good[s] && key >= any_low && key <= any_last;
+#pragma unroll
+          for (int c = 0; c < kSections; ++c) {
+            tile.v[s][c][y] = seen ? tile.v[s][c][y] : 0u;
+            tile.vs[s][c] = seen ? tile.vs[s][c] : ((tile.vs[s][c] & ~(255u << (8 * y))) | (127u << (8 * y)));
+          }
+        }
+    }
+    // groups that are not finite (rare): which keys, and which values
+    bool k_nan[2] = {false, false}, v_nan = false;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int c = 0; c < kSections; ++c) {
+        k_nan[s] = k_nan[s] || tile.ks[s][c] == kFp4Nan;
+        const unsigned int w = tile.vs[s][c];
+        v_nan = v_nan || (((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u) != 0u;
+      }
+    unsigned int nan_keys = 0u;
+    const bool bad_keys = __ballot(k_nan[0] || k_nan[1]) != 0ull;
+    const bool bad_values = __ballot(v_nan) != 0ull;
+    if (bad_keys) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const unsigned long long b = __ballot(k_nan[s]);
+        const unsigned int f = (unsigned int)(b | (b >> 32));
+        nan_keys |= ((f | (f >> 16)) & 0xffffu) << (16 * s);
+      }
+    }
+    if (bad_values) mark_values(tile, t0, lane);
+
+    // S^T = K Q^T
+    f32x4 sc[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int c = 0; c < kSections; ++c) {
+        const float scale = fp4_scale(tile.ks[s][c]);
+        const int base = section_dim(c) / 32;
+#pragma unroll
+        for (int i = 0; i < section_elems(c) / 2; ++i) {
+          const unsigned int w = tile.k[s][base + i];
+          const bf16x8 k = as_operand(fp4_pair<0>(w, scale), fp4_pair<1>(w, scale), fp4_pair<2>(w, scale), fp4_pair<3>(w, scale));
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int term = kTerms<T> - 1; term >= 0; --term)  // the small terms first
+              sc[t][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[term][t][base + i], sc[t][s], 0, 0, 0);
+        }
+      }
+    // the weights
+    bf16x8 p[kTerms<T>][NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = sc[t][i >> 2][i & 3] * a.factor;
+      if (bad_keys) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if ((nan_keys >> (16 * (i >> 2) + 4 * j + (i & 3))) & 1u) x[i] = __uint_as_float(0x7fc00000u);
+      }
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int key = t0 + 16 * (i >> 2) + 4 * j + (i & 3);
+          const bool seen = key >= low[t] && key <= last[t] && tile.good[i >> 2];
+          x[i] = seen ? x[i] : -INFINITY;
+        }
+      }
+      float top = x[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
+      if (__ballot(top > m[t] + kSlack) != 0ull) {  // (-inf + 8 is -inf: any score moves the first reference)
+        const float next = fmaxf(m[t], quad16_max(top));
+        const float f = m[t] == -INFINITY ? 0.f : weight_exp2<T>(m[t] - next);
+        m[t] = next;
+        l[t] = l[t] * f;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) acc[t][i][y] = acc[t][i][y] * f;
+      }
+      const float ref = m[t] == -INFINITY ? 0.f : m[t];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = weight_exp2<T>(x[i] - ref);
+        l[t] = l[t] + w;
+        float rest = w;
+#pragma unroll
+        for (int term = 0; term < kTerms<T>; ++term) {
+          const bf16_t part = static_cast<bf16_t>(rest);
+          p[term][t][i] = part;
+          if constexpr (kTerms<T> > 1) rest = rest - static_cast<float>(part);
+        }
+      }
+    }
+    // O^T += V^T P^T
+#pragma unroll
+    for (int c = 0; c < kSections; ++c) {
+      const int e = section_elems(c), at = section_dim(c) / 16;
+      float scale[2][4];
+      unsigned int w[2][4];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          scale[s][y] = fp4_scale((tile.vs[s][c] >> (8 * y)) & 255u);
+          w[s][y] = e == 8 ? tile.v[s][c][y] : e == 4 ? tile.v[s][c][y] >> (16 * (n & 1)) : tile.v[s][c][y] >> (8 * (n & 3));
+        }
+#pragma unroll
+      for (int pair = 0; pair < e / 2; ++pair) {
+        unsigned int both[2][4];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            both[s][y] = pair == 0 ? fp4_pair<0>(w[s][y], scale[s][y]) : pair == 1 ? fp4_pair<1>(w[s][y], scale[s][y])
+                         : pair == 2 ? fp4_pair<2>(w[s][y], scale[s][y]) : fp4_pair<3>(w[s][y], scale[s][y]);
+        const bf16x8 even = as_operand(__builtin_amdgcn_perm(both[0][1], both[0][0], 0x05040100u), __builtin_amdgcn_perm(both[0][3], both[0][2], 0x05040100u),
+                                       __builtin_amdgcn_perm(both[1][1], both[1][0], 0x05040100u), __builtin_amdgcn_perm(both[1][3], both[1][2], 0x05040100u));
+        const bf16x8 odd = as_operand(__builtin_amdgcn_perm(both[0][1], both[0][0], 0x07060302u), __builtin_amdgcn_perm(both[0][3], both[0][2], 0x07060302u),
+                                      __builtin_amdgcn_perm(both[1][1], both[1][0], 0x07060302u), __builtin_amdgcn_perm(both[1][3], both[1][2], 0x07060302u));
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int term = kTerms<T> - 1; term >= 0; --term) {
+            acc[t][at + 2 * pair] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, p[term][t], acc[t][at + 2 * pair], 0, 0, 0);
+            acc[t][at + 2 * pair + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, p[term][t], acc[t][at + 2 * pair + 1], 0, 0, 0);
+          }
+      }
+    }
+  }
+
+  // Values of groups that are not finite: zeros for the product, and NaN in the sums of the rows that see them.
+  __device__ __forceinline__ void mark_values(KeyTile& tile, int t0, int lane) {
+    const int j = lane >> 4;
+    for (int c = 0; c < kSections; ++c)
+      for (int s = 0; s < 2; ++s)
+        for (int y = 0; y < 4; ++y) {
+          unsigned int byte = 0u, word = 0u;
+          // (registers are not indexed by a loop's variable)
+#pragma unroll
+          for (int cc = 0; cc < kSections; ++cc)
+#pragma unroll
+            for (int ss = 0; ss < 2; ++ss)
+              if (cc == c && ss == s) {
+                byte = (tile.vs[ss][cc] >> (8 * y)) & 255u;
+                if (byte == kFp4Nan) {
+                  tile.vs[ss][cc] = (tile.vs[ss][cc] & ~(255u << (8 * y))) | (127u << (8 * y));
+#pragma unroll
+                  for (int yy = 0; yy < 4; ++yy)
+                    if (yy == y) tile.v[ss][cc][yy] = word;
+                }
+              }
+          const unsigned long long b = __ballot(byte == kFp4Nan);
+          if (b == 0ull) continue;
+          for (int block = 0; block < 4; ++block) {
+            // the lane's sums are of the columns 4 j .. 4 j + 3, which lie in one group; lane 4 j of the block tells
+            const bool mine = (b >> (4 * j + 16 * block)) & 1ull;
+            const int key = t0 + 16 * s + 4 * block + y;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              if (mine && key >= low[t] && key <= last[t]) {
+#pragma unroll
+                for (int cc = 0; cc < kSections; ++cc)
+#pragma unroll
+                  for (int i = 0; i < section_elems(cc); ++i)
+                    if (cc == c)
+#pragma unroll
+                      for (int z = 0; z < 4; ++z) acc[t][section_dim(cc) / 16 + i][z] = __uint_as_float(0x7fc00000u);
+              }
+          }
+        }
+  }
+};
+
+// Walk the key tiles first, first + stride, ... below end.
+template <typename T, int NT>
+__device__ __forceinline__ void walk_keys(Rows<T, NT>& rows, const Fp4Args& a, const int* __restrict__ table_row, int head,
+                                          int first, int end, int stride, int lane) {
+  if (first >= end) return;
+  PageIds ids = load_ids(a, table_row, first, lane);
+  KeyTile tile;
+  load_tile(tile, a, ids, head, first, lane);
+  ids = load_ids(a, table_row, first + stride < end ? first + stride : first, lane);
+  for (int t0 = first; t0 < end; t0 += stride) {
+    KeyTile next;
+    const int t1 = t0 + stride < end ? t0 + stride : t0;  // (behind the last tile the same one again: within bounds)
+    load_tile(next, a, ids, head, t1, lane);
+    ids = load_ids(a, table_row, t1 + stride < end ? t1 + stride : t1, lane);
+    rows.step(a, tile, t0, lane);
+    tile = next;
+  }
+}
+
+template <typename T> __device__ __forceinline__ void store_run(T* to, const float* x, int n);
+template <> __device__ __forceinline__ void store_run<float>(float* to, const float* x, int n) {
+  typedef float any2 __attribute__((ext_vector_type(2), aligned(4)));
+  typedef float any4 __attribute__((ext_vector_type(4), aligned(4)));
+  if (n == 8) {
+    *reinterpret_cast<any4*>(to) = any4{x[0], x[1], x[2], x[3]};
+    *reinterpret_cast<any4*>(to + 4) = any4{x[4], x[5], x[6], x[7]};
+  } else if (n == 4) {
+    *reinterpret_cast<any4*>(to) = any4{x[0], x[1], x[2], x[3]};
+  } else {
+    *reinterpret_cast<any2*>(to) = any2{x[0], x[1]};
+  }
+}
+template <> __device__ __forceinline__ void store_run<bf16_t>(bf16_t* to, const float* x, int n) {
+  typedef __bf16 any2 __attribute__((ext_vector_type(2), aligned(2)));
+  typedef __bf16 any4 __attribute__((ext_vector_type(4), aligned(2)));
+  typedef __bf16 any8 __attribute__((ext_vector_type(8), aligned(2)));
+  if (n == 8) {
+    *reinterpret_cast<any8*>(to) = any8{(bf16_t)x[0], (bf16_t)x[1], (bf16_t)x[2], (bf16_t)x[3], (bf16_t)x[4], (bf16_t)x[5], (bf16_t)x[6], (bf16_t)x[7]};
+  } else if (n == 4) {
+    *reinterpret_cast<any4*>(to) = any4{(bf16_t)x[0], (bf16_t)x[1], (bf16_t)x[2], (bf16_t)x[3]};
+  } else {
+    *reinterpret_cast<any2*>(to) = any2{(bf16_t)x[0], (bf16_t)x[1]};
+  }
+}
+
+// Decoded tokens: grid (splits, kv heads, requests).
+template <typename T>
+__global__ __launch_bounds__(kThreads, (std::is_same_v<T, float> && D > 160 ? 1 : 2)) void fp4_decode_kernel(Fp4Args a) {
+  constexpr int kPad = D + 4;
+  __shared__ float fold_acc[4][16][kPad];
+  __shared__ float fold_m[4][16], fold_l[4][16];
+  const int split = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const Request rq(a, b);
+  if (rq.rows == 0 || rq.rows > a.few) return;
+  const int span = rq.end - rq.base, len = decode_split(span);
+  const int splits = max(1, (span + len - 1) / len);
+  if (split >= splits) return;
+  const int begin = rq.base + split * len, end = min(rq.end, begin + len);
+  Rows<T, 1> rows;
+  rows.init(a, rq, head, 0, lane);
+  walk_keys<T, 1>(rows, a, a.table + (long)b * a.columns, head, begin + kTileKeys * w, end, 4 * kTileKeys, lane);
+  const int n = lane & 15, j = lane >> 4;
+  const float l = quad16_sum(rows.l[0]);
+  if (j == 0) {
+    fold_m[w][n] = rows.m[0];
+    fold_l[w][n] = l;
+  }
+#pragma unroll
+  for (int c = 0; c < kSections; ++c)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int e = section_elems(c);
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < e; ++i) x[i] = rows.acc[0][section_dim(c) / 16 + i][y];
+      float* to = &fold_acc[w][n][section_dim(c) + e * (4 * j + y)];
+#pragma unroll
+      for (int i = 0; i < e; ++i) to[i] = x[i];
+    }
+  __syncthreads();
+  const int there = min(rq.rows, 16);
+  for (int i = threadIdx.x; i < there * (D / 4); i += kThreads) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4));
+    float top = fold_m[0][r];
+#pragma unroll
+    for (int k = 1; k < 4; ++k) top = fmaxf(top, fold_m[k][r]);
+    float sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float f = fold_m[k][r] == -INFINITY ? fold_l[k][r] : weight_exp2<T>(fold_m[k][r] - top);  // (no score: 0, or NaN)
+      sum = fmaf(fold_l[k][r], f, sum);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) x[y] = fmaf(fold_acc[k][r][d + y], f, x[y]);
+    }
+    if (splits == 1) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) x[y] = x[y] * inv;
+      const int token = r / a.group, sub = r - token * a.group;
+      store_run<T>(static_cast<T*>(a.out) + (long)(rq.first + token) * a.ldo + (long)(head * a.group + sub) * D + d, x, 4);
+    } else {
+      const int entry = split * 16 + r;
+      if (entry < a.region) {
+        const long at = ((long)b * a.pool.kv_heads + head) * a.region + entry;
+        store_run<float>(a.part_acc + at * D + d, x, 4);
+        if (d == 0) {
+          a.part_ml[2 * at] = top;
+          a.part_ml[2 * at + 1] = sum;
+        }
+      }
+    }
+  }
+}
+
+// Prompts: grid (groups of four row blocks, kv heads * splits, requests); a wave a row block.
+template <typename T>
+__global__ __launch_bounds__(kThreads, 1) void fp4_prompt_kernel(Fp4Args a) {
+  constexpr int NT = kPromptTiles<T>, kBlock = 16 * NT;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int head = blockIdx.y % a.pool.kv_heads, split = blockIdx.y / a.pool.kv_heads, b = blockIdx.z;
+  const Request rq(a, b);
+  if (rq.rows <= a.few) return;
+  const int blocks = (rq.rows + kBlock - 1) / kBlock;
+  const int block = 4 * (gridDim.x - 1 - blockIdx.x) + w;  // the blocks that see most keys first
+  if (block >= blocks) return;
+  const int span = rq.end - rq.base, len = prompt_split(span, blocks);
+  const int splits = max(1, (span + len - 1) / len);
+  if (split >= splits) return;
+  const int row0 = block * kBlock;
+  Rows<T, NT> rows;
+  rows.init(a, rq, head, row0, lane);
+  const int begin = max(rq.base + split * len, rows.any_low & ~(kTileKeys - 1));
+  const int end = min(min(rq.end, rq.base + (split + 1) * len), rows.any_last + 1);
+  walk_keys<T, NT>(rows, a, a.table + (long)b * a.columns, head, begin, end, kTileKeys, lane);
+  const int n = lane & 15, j = lane >> 4;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int r = row0 + 16 * t + n;
+    const float l = quad16_sum(rows.l[t]);
+    const bool there = r < rq.rows;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int token = there ? r / a.group : 0, sub = there ? r - token * a.group : 0;
+    T* out = static_cast<T*>(a.out) + (long)(rq.first + token) * a.ldo + (long)(head * a.group + sub) * D;
+    const int entry = split * blocks * kBlock + r;
+    const bool keep = there && entry < a.region;
+    const long at = ((long)b * a.pool.kv_heads + head) * a.region + (keep ? entry : 0);
+    if (splits > 1 && keep && j == 0) {
+      a.part_ml[2 * at] = rows.m[t];
+      a.part_ml[2 * at + 1] = l;
+    }
+#pragma unroll
+    for (int c = 0; c < kSections; ++c)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int e = section_elems(c), dim = section_dim(c) + e * (4 * j + y);
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < e; ++i) x[i] = rows.acc[t][section_dim(c) / 16 + i][y];
+        if (splits == 1) {
+#pragma unroll
+          for (int i = 0; i < e; ++i) x[i] = x[i] * inv;
+          if (there) store_run<T>(out + dim, x, e);
+        } else if (keep) {
+          store_run<float>(a.part_acc + at * D + dim, x, e);
+        }
+      }
+  }
+}
+
+// Fold the splits of every (row, head): a wave each, four a workgroup.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void fp4_combine_kernel(Fp4Args a) {
+  constexpr int kBlock = 16 * kPromptTiles<T>;
+  const int lane = threadIdx.x & 63;
+  const int heads = a.group * a.pool.kv_heads;
+  const long i = (long)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  if (i >= (long)a.rows * heads) return;
+  const int row = (int)(i / heads), query_head = (int)(i - (long)row * heads);
+  int b = 0, e = a.requests;  // the last request that begins at or before the row
+  while (e - b > 1) {
+    const int mid = (b + e) >> 1;
+    if (a.offsets[mid] <= row) b = mid; else e = mid;
+  }
+  const Request rq(a, b);
+  if (row < rq.first || row >= rq.first + rq.rows / a.group) return;
+  const int span = rq.end - rq.base;
+  const int head = query_head / a.group, r = (row - rq.first) * a.group + query_head % a.group;
+  const bool few = rq.rows <= a.few;
+  const int blocks = (rq.rows + kBlock - 1) / kBlock;
+  const int len = few ? decode_split(span) : prompt_split(span, blocks);
+  const int splits = (span + len - 1) / len, stride = few ? 16 : blocks * kBlock;
+  if (splits <= 1) return;
+  const long base = ((long)b * a.pool.kv_heads + head) * a.region;
+  if ((long)(splits - 1) * stride + r >= a.region) return;
+  float top = -INFINITY;
+  for (int s = lane; s < splits; s += 64) top = fmaxf(top, a.part_ml[2 * (base + (long)s * stride + r)]);
+  top = wave_max(top);
+  constexpr int kEach = (D + 63) / 64;
+  float sum = 0.f, x[kEach];
+#pragma unroll
+  for (int y = 0; y < kEach; ++y) x[y] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const long at = base + (long)s * stride + r;
+    const float m = a.part_ml[2 * at], l = a.part_ml[2 * at + 1];
+    const float f = m == -INFINITY ? l : weight_exp2<T>(m - top);  // (no score: 0, or NaN)
+    sum = fmaf(l, f, sum);
+#pragma unroll
+    for (int y = 0; y < kEach; ++y) {
+      const int d = kEach * lane + y;
+      const float v = a.part_acc[at * D + min(d, D - 1)];
+      x[y] = fmaf(v, f, x[y]);
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T* out = static_cast<T*>(a.out) + (long)row * a.ldo + (long)query_head * D;
+#pragma unroll
+  for (int y = 0; y < kEach; ++y) {
+    const int d = kEach * lane + y;
+    if (d < D) out[d] = from_f32<T>(x[y] * inv);
+  }
+}
+
+struct Plan {
+  int few, decode_splits, prompt_groups, prompt_splits, region;
+};
+
+// What is launched for requests of at most `most` rows and `longest` keys.
+template <typename T>
+Plan make_plan(int group, int most, int longest, int window) {
+  constexpr int kBlock = 16 * kPromptTiles<T>;
+  Plan p{16, 0, 0, 0, 0};
+  // the keys that a request's rows see, at most: with a window those of its tokens and the window before, in whole tiles
+  const auto seen = [&](int n) { return window > 0 ? (int)min((long)longest, (long)n + window - 1 + kTileKeys) : longest; };
+  // (a request of few rows, and any number of keys up to `longest`: the splits do not shrink with the span but where
+  // the length of a split steps up)
+  const int few_tokens = max(1, 16 / group);
+  const int span = seen(min(few_tokens, most));
+  p.decode_splits = 1;
+  const int steps[4] = {span, min(span, 4096), min(span, 32768), min(span, 131072)};
+  for (int s : steps) p.decode_splits = max(p.decode_splits, (s + decode_split(s) - 1) / max(1, decode_split(s)));
+  if (p.decode_splits > 1) p.region = 16 * p.decode_splits;
+  const long rows = (long)most * group;
+  if (rows > p.few) {
+    const int blocks = (int)((rows + kBlock - 1) / kBlock);
+    p.prompt_groups = (blocks + 3) / 4;
+    const int far = seen(most);
+    p.prompt_splits = min(kPromptBlocks, max(1, (far + 511) / 512));
+    if (p.prompt_splits > 1) p.region = max(p.region, kPromptBlocks * kBlock);
+  }
+  return p;
+}
+
+template <typename T>
+int run_fp4(Fp4Args& a, int most, int longest, void* scratch, long scratch_bytes, hipStream_t stream) {
+  const Plan p = make_plan<T>(a.group, most, longest, a.window);
+  a.few = p.few;
+  a.region = p.region;
+  const long entries = (long)a.requests * a.pool.kv_heads * p.region;
+  LS_REQUIRE(scratch_bytes >= entries * (D + 2) * (long)sizeof(float), "fp4_attention: %ld bytes of scratch, %ld needed",
+             scratch_bytes, entries * (D + 2) * (long)sizeof(float));
+  a.part_acc = static_cast<float*>(scratch);
+  a.part_ml = a.part_acc + entries * D;
+  const int heads = a.pool.kv_heads;
+  if (p.prompt_groups > 0) {
+    LS_REQUIRE((long)heads * p.prompt_splits <= 65535, "fp4_attention: %d heads in %d splits", heads, p.prompt_splits);
+    fp4_prompt_kernel<T><<<dim3(p.prompt_groups, heads * p.prompt_splits, a.requests), kThreads, 0, stream>>>(a);
+  }
+  // all requests of the step bring `most` rows where the rows say so: then none is left for the other kernel
+  if (p.prompt_groups == 0 || (long)a.requests * most != a.rows)
+    fp4_decode_kernel<T><<<dim3(p.decode_splits, heads, a.requests), kThreads, 0, stream>>>(a);
+  if (p.region > 0) {
+    const long groups = ((long)a.rows * a.group * heads + 3) / 4;
+    LS_REQUIRE(groups <= 0x7fffffffl, "fp4_attention: %d rows", a.rows);
+    fp4_combine_kernel<T><<<(unsigned)groups, kThreads, 0, stream>>>(a);
+  }
+  return check_launch("fp4_attention");
+}
+
+}  // namespace ls
+
+LS_DEFINE_ERROR_API
+
+extern "C" int ls_fp4_attention_head_dim() { return ls::D; }
+
+extern "C" long ls_fp4_attention_scratch_bytes(int dtype, int requests, int kv_heads, int group, int most, int longest, int window) {
+  using namespace ls;
+  if (requests <= 0 || kv_heads <= 0 || group <= 0 || most <= 0) return 0;
+  const Plan p = dtype == kF32 ? make_plan<float>(group, most, longest, window) : make_plan<bf16_t>(group, most, longest, window);
+  return (long)requests * kv_heads * p.region * (D + 2) * (long)sizeof(float);
+}
+
+extern "C" int ls_fp4_attention(int dtype, const void* q, long ldq, void* out, long ldo, int rows, const void* k_codes,
+                                const void* k_scales, const void* v_codes, const void* v_scales, int pages, int page_size,
+                                int kv_heads, int group, const int* table, int columns, const int* offsets,
+                                const int* lengths, int requests, int most, int longest, float scale, int window,
+                                void* scratch, long scratch_bytes, void* stream) {
+  using namespace ls;
+  LS_REQUIRE(dtype == kF32 || dtype == kBF16, "fp4_attention: dtype %d", dtype);
+  LS_REQUIRE(rows >= 0 && pages >= 1 && kv_heads >= 1 && kv_heads <= 65535 && group >= 1 && columns >= 1 && requests >= 1 &&
+                 requests <= 65535 && most >= 0 && longest >= 0 && window >= 0 && ldq >= 0 && ldo >= 0,
+             "fp4_attention: %d rows of %d requests, %d heads by %d, %d pages, %d columns", rows, requests, kv_heads, group,
+             pages, columns);
+  LS_REQUIRE(page_size >= 4 && (page_size & (page_size - 1)) == 0, "fp4_attention: pages of %d tokens", page_size);
+  LS_REQUIRE(most <= rows && (long)most * group <= 0x7fffff00l && longest <= 0x7fff0000, "fp4_attention: %d rows a request, %d keys", most, longest);
+  if (rows == 0 || most == 0) return 0;
+  Fp4Args a;
+  a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo;
+  a.pool = Fp4Pool{static_cast<const unsigned char*>(k_codes), static_cast<const unsigned char*>(k_scales),
+                   static_cast<const unsigned char*>(v_codes), static_cast<const unsigned char*>(v_scales), pages,
+                   __builtin_ctz((unsigned)page_size), kv_heads};
+  a.table = table; a.columns = columns; a.offsets = offsets; a.lengths = lengths; a.requests = requests; a.rows = rows;
+  a.group = group; a.factor = scale * kToLog2; a.window = window;
+  return dtype == kF32 ? run_fp4<float>(a, most, longest, scratch, scratch_bytes, (hipStream_t)stream)
+                       : run_fp4<bf16_t>(a, most, longest, scratch, scratch_bytes, (hipStream_t)stream);
+}

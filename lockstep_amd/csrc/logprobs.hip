@@ -1,0 +1,498 @@
+// Log probabilities of given tokens, with the entropy of the distribution, the token's rank and the first alternatives.
+//
+// For a row x of `vocab` logits and a token t, with m = max x, S = sum e^(x - m), T = sum e^(x - m) (x - m):
+//   logprob = (x_t - m) - log S,   entropy = log S - T / S,
+//   rank    = how many tokens come before t in the order "larger logit first, then lower id",
+//   top     = the first k tokens of that order, each with its log probability.
+//
+// What bounds it: reading the row once.  A row is cut into pieces of 2,048 neighbouring logits, a piece is a wave's: a
+// lane takes vectors of 16 bytes, 64 vectors apart, and has its 32 logits in registers for the maximum first and the sums
+// then, so a piece costs one maximum and one rescaling a lane and the row is read once.  Everything is held a lane (m, S,
+// T) and a lane's pieces are folded in the order of a stream: piece i belongs to stream i mod 8.  Only at the end are a
+// stream's lanes folded (butterfly) and the streams after one another.  So the order of every sum depends on the row's
+// length alone: with many rows a workgroup of eight waves takes a row, a wave a stream; with few rows every piece is a
+// wave of its own that leaves its lanes' (m, S, T), and a second launch folds them -- the same bits.
+//
+// The alternatives come without a sort.  The lanes' maxima of every piece are kept; the k-th largest of 128 maxima over
+// disjoint parts of the row is a bound that the k first tokens reach (each of those parts holds one that does), and only
+// the lanes that reach it, some k of them, are read again.  Rows where more tokens reach it than there is room for (equal
+// logits, rows that are masked but for a few tokens) and rows with an infinity or a NaN go by the digits of the k-th key
+// instead, which reads the row a dozen times.  A NaN counts as larger than all numbers, -0 as 0.
+
+#include "common.h"
+#include "serving_api.h"
+
+namespace ls {
+
+constexpr int kPiece = 2048;
+constexpr int kLaneElems = kPiece / 64;
+constexpr int kStreams = 8;
+constexpr int kRowThreads = kStreams * 64;
+constexpr int kMaxPieces = 256;
+constexpr int kMaxVocab = kPiece * kMaxPieces;
+constexpr int kMaxTop = 32;
+constexpr int kParts = 128;       // disjoint parts of the row whose maxima give the bound
+constexpr int kMaxSets = 512;     // lanes of a piece that are read again
+constexpr int kMaxFound = 512;    // tokens that reach the bound
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct LaneSums {
+  float m, s, t;
+};
+
+__device__ __forceinline__ unsigned int logit_key(float f) {  // ascending; -0 counts as 0, every NaN as the largest
+  const unsigned int b = __float_as_uint(f + 0.0f);
+  if (f != f) return 0xffffffffu;
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
+__device__ __forceinline__ LaneSums fold_sums(const LaneSums& a, const LaneSums& b) {
+  const float m = fmaxf(a.m, b.m);
+  LaneSums r{m, 0.f, 0.f};
+  // a side without any weight (nothing yet, or only logits of -inf) adds nothing; NaN weights do.  (Behind a distance of
+  // 1e4 nothing is left of a side, and a greater one would make 0 times an infinity of it.)
+  if (a.s != 0.f) {
+    const float d = fmaxf(a.m - m, -1e4f), f = __builtin_amdgcn_exp2f(d * kLog2e);
+    r.s = a.s * f;
+    r.t = f * fmaf(a.s, d, a.t);
+  }
+  if (b.s != 0.f) {
+    const float d = fmaxf(b.m - m, -1e4f), f = __builtin_amdgcn_exp2f(d * kLog2e);
+    r.s = fmaf(b.s, f, r.s);
+    r.t = fmaf(f, fmaf(b.s, d, b.t), r.t);
+  }
+  return r;
+}
+
+template <typename T> struct Row;
+template <> struct Row<float> {
+  static constexpr int VEC = 4;
+  typedef float vec_t __attribute__((ext_vector_type(4), aligned(4)));
+};
+template <> struct Row<bf16_t> {
+  static constexpr int VEC = 8;
+  typedef unsigned int vec_t __attribute__((ext_vector_type(4), aligned(2)));
+};
+
+// The lane's 32 logits of a piece as floats; -inf behind the row's end.
+template <typename T>
+__device__ __forceinline__ void load_piece(float (&x)[kLaneElems], const T* __restrict__ row, int piece, int vocab, int lane) {
+  constexpr int VEC = Row<T>::VEC;
+  const int base = piece * kPiece;
+  if (base + kPiece <= vocab) {  // uniform
+    typename Row<T>::vec_t raw[kLaneElems / VEC];
+#pragma unroll
+    for (int i = 0; i < kLaneElems / VEC; ++i)
+      raw[i] = *reinterpret_cast<const typename Row<T>::vec_t*>(row + base + (i * 64 + lane) * VEC);
+#pragma unroll
+    for (int i = 0; i < kLaneElems / VEC; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(T) == 4) {
+          x[i * 4 + e] = raw[i][e];
+        } else {
+          x[i * 8 + 2 * e] = __uint_as_float(raw[i][e] << 16);
+          x[i * 8 + 2 * e + 1] = __uint_as_float(raw[i][e] & 0xffff0000u);
+        }
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kLaneElems; ++i) {
+      const int at = base + ((i / VEC) * 64 + lane) * VEC + i % VEC;
+      x[i] = at < vocab ? to_f32(row[min(at, vocab - 1)]) : -INFINITY;
+    }
+  }
+}
+
+// The piece's sums of a lane, and (uniform) how many of the piece's tokens come before the token `given` of logit `mine`.
+template <typename T>
+__device__ __forceinline__ LaneSums piece_sums(const float (&x)[kLaneElems], int piece, int given, float mine, int& before, int lane) {
+  constexpr int VEC = Row<T>::VEC;
+  LaneSums r;
+  r.m = x[0];
+#pragma unroll
+  for (int i = 1; i < kLaneElems; ++i) r.m = fmaxf(r.m, x[i]);
+  const float ref = r.m == -INFINITY ? 0.f : r.m;
+  r.s = 0.f;
+  r.t = 0.f;
+#pragma unroll
+  for (int i = 0; i < kLaneElems; ++i) {
+    const float d = x[i] - ref;
+    const float e = __builtin_amdgcn_exp2f(d * kLog2e);
+    r.s = r.s + e;
+    r.t = fmaf(e, fmaxf(d, -1e4f), r.t);  // (a logit of -inf: 0 times a number)
+  }
+  // A NaN compares false with everything, so "not smaller" counts it as larger.
+  const int base = piece * kPiece;
+  if (base > given) {  // uniform: equal logits of this piece come later
+#pragma unroll
+    for (int i = 0; i < kLaneElems; ++i) before += __popcll(__ballot(!(x[i] <= mine)));
+  } else if (base + kPiece <= given) {  // or before
+#pragma unroll
+    for (int i = 0; i < kLaneElems; ++i) before += __popcll(__ballot(!(x[i] < mine)));
+  } else {
+#pragma unroll
+    for (int i = 0; i < kLaneElems; ++i) {
+      const int at = base + ((i / VEC) * 64 + lane) * VEC + i % VEC;
+      before += __popcll(__ballot(at < given ? !(x[i] < mine) : !(x[i] <= mine)));
+    }
+  }
+  return r;
+}
+
+struct FinishShared {
+  float m[kStreams], s[kStreams], t[kStreams];
+  int before[kStreams];
+  unsigned int part[kParts];
+  unsigned int bound;
+  int set_list[kMaxSets];
+  unsigned int key[kMaxFound];
+  int id[kMaxFound];
+  int digits[kStreams][16];
+  int wave_count[kStreams];
+};
+
+// Exclusive sum over the workgroup's threads; `total` gets the whole sum.
+__device__ __forceinline__ int row_scan(int v, int* __restrict__ wave_sums, int& total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int inclusive = v;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int other = __shfl_up(inclusive, off);
+    if (lane >= off) inclusive += other;
+  }
+  __syncthreads();  // wave_sums may still be read from the call before
+  if (lane == 63) wave_sums[w] = inclusive;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int k = 0; k < kStreams; ++k) {
+    if (k < w) before += wave_sums[k];
+    total += wave_sums[k];
+  }
+  return before + inclusive - v;
+}
+
+// The first k tokens of the row in sh.key / sh.id by the digits of the k-th key: a workgroup of kRowThreads.
+template <typename T>
+__device__ __forceinline__ int find_by_digits(FinishShared& sh, const T* __restrict__ row, int vocab, int top) {
+  const int t = threadIdx.x;
+  unsigned int prefix = 0;
+  int want = top;  // the place of the key looked for among the keys with this prefix
+  for (int shift = 28; shift >= 0; shift -= 4) {
+    int count[16];
+#pragma unroll
+    for (int d = 0; d < 16; ++d) count[d] = 0;
+    for (int i = t; i < vocab; i += kRowThreads) {
+      const unsigned int key = logit_key(to_f32(row[i]));
+      const unsigned int digit = shift == 28 || (key >> (shift + 4)) == prefix ? (key >> shift) & 15u : 16u;
+#pragma unroll
+      for (int d = 0; d < 16; ++d) count[d] += digit == (unsigned int)d ? 1 : 0;
+    }
+#pragma unroll
+    for (int d = 0; d < 16; ++d) {
+      const int n = wave_sum(count[d]);
+      if ((t & 63) == 0) sh.digits[t >> 6][d] = n;
+    }
+    __syncthreads();
+    int digit = 15, above = 0;
+    for (; digit >= 0; --digit) {  // (every thread comes to the same digit)
+      int n = 0;
+#pragma unroll
+      for (int w = 0; w < kStreams; ++w) n += sh.digits[w][digit];
+      if (digit == 0 || above + n >= want) break;
+      above += n;
+    }
+    prefix = (prefix << 4) | (unsigned int)digit;
+    want -= above;
+    __syncthreads();
+  }
+  // the keys above it, fewer than `top`, and the first `want` equal ones in the order of their ids
+  int mine = 0, all;
+  for (int i = t; i < vocab; i += kRowThreads) mine += logit_key(to_f32(row[i])) > prefix ? 1 : 0;
+  int at = row_scan(mine, sh.wave_count, all);
+  if (mine > 0)
+    for (int i = t; i < vocab; i += kRowThreads) {
+      const unsigned int key = logit_key(to_f32(row[i]));
+      if (key > prefix && at < kMaxFound) {
+        sh.key[at] = key;
+        sh.id[at++] = i;
+      }
+    }
+  int ties = 0;
+  for (int base = 0; base < vocab && ties < want; base += kRowThreads) {
+    const int i = base + t;
+    const bool tie = i < vocab && logit_key(to_f32(row[i])) == prefix;
+    const int place = ties + row_scan(tie ? 1 : 0, sh.wave_count, all);
+    if (tie && place < want) {
+      sh.key[top - want + place] = prefix;
+      sh.id[top - want + place] = i;
+    }
+    ties += all;
+  }
+  __syncthreads();
+  return top;
+}
+
+// What is left when every stream's lanes have their sums: a workgroup of kRowThreads, wave w with stream w.
+template <typename T>
+__device__ __forceinline__ void finish_row(FinishShared& sh, const float* __restrict__ set_max, LaneSums mine, int before,
+                                           const T* __restrict__ row, int vocab, int pieces, int given, float given_logit,
+                                           int top, int r, float* __restrict__ logprob, float* __restrict__ entropy,
+                                           int* __restrict__ rank, int* __restrict__ top_ids,
+                                           float* __restrict__ top_logprobs) {
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  // fold the lanes (butterfly: every lane the same bits)
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    LaneSums other{__shfl_xor(mine.m, off), __shfl_xor(mine.s, off), __shfl_xor(mine.t, off)};
+    mine = (lane & off) ? fold_sums(other, mine) : fold_sums(mine, other);
+  }
+  if (lane == 0) {
+    sh.m[w] = mine.m; sh.s[w] = mine.s; sh.t[w] = mine.t;
+    sh.before[w] = before;
+  }
+  __syncthreads();
+  LaneSums all{sh.m[0], sh.s[0], sh.t[0]};
+  int ahead = sh.before[0];
+#pragma unroll
+  for (int s = 1; s < kStreams; ++s) {
+    all = fold_sums(all, LaneSums{sh.m[s], sh.s[s], sh.t[s]});
+    ahead += sh.before[s];
+  }
+  const float log_sum = logf(all.s);
+  const bool valid = given >= 0 && given < vocab;
+  if (valid && given_logit != given_logit) {  // (uniform) before a NaN come only the NaN of lower ids
+    int nan = 0;
+    for (int i = t; i < given; i += kRowThreads) {
+      const float x = to_f32(row[i]);
+      nan += x != x ? 1 : 0;
+    }
+    nan = wave_sum(nan);
+    __syncthreads();
+    if (lane == 0) sh.before[w] = nan;
+    __syncthreads();
+    ahead = 0;
+#pragma unroll
+    for (int s = 0; s < kStreams; ++s) ahead += sh.before[s];
+  }
+  if (t == 0) {
+    logprob[r] = valid ? (given_logit - all.m) - log_sum : __uint_as_float(0x7fc00000u);
+    entropy[r] = log_sum - all.t / all.s;
+    rank[r] = valid ? ahead : -1;
+  }
+  if (top == 0) return;
+
+  int found = -1;
+  if (all.s == all.s && all.s != 0.f) {  // finite logits but for -inf
+    const int sets = pieces * 64;
+    float part = -INFINITY;
+    for (int i = t; i < sets; i += kRowThreads) part = fmaxf(part, set_max[i]);
+    with_lane_xor16(part, part, mine.m);
+    part = fmaxf(part, mine.m);
+    with_lane_xor32(part, part, mine.m);
+    part = fmaxf(part, mine.m);
+    if (lane < 16) sh.part[w * 16 + lane] = logit_key(part);
+    __syncthreads();
+    if (t < kParts) {
+      const unsigned int key = sh.part[t];
+      int larger = 0;
+#pragma unroll 8
+      for (int i = 0; i < kParts; ++i) {
+        const unsigned int other = sh.part[i];
+        larger += other > key || (other == key && i < t) ? 1 : 0;
+      }
+      if (larger == top - 1) sh.bound = key;
+    }
+    __syncthreads();
+    const unsigned int bound = sh.bound;
+    // count, add up, write: the lists come out the same every time
+    int hits = 0, listed, reached;
+    for (int i = t; i < sets; i += kRowThreads) hits += logit_key(set_max[i]) >= bound ? 1 : 0;
+    int at = row_scan(hits, sh.wave_count, listed);
+    if (listed <= kMaxSets) {  // uniform
+      if (hits > 0)
+        for (int i = t; i < sets; i += kRowThreads)
+          if (logit_key(set_max[i]) >= bound) sh.set_list[at++] = i;
+      __syncthreads();
+      constexpr int VEC = Row<T>::VEC;
+      const auto entry = [&](int i, int& id, unsigned int& key) LS_INLINED -> bool {
+        const int set = sh.set_list[i / kLaneElems], e = i % kLaneElems;
+        id = (set >> 6) * kPiece + ((e / VEC) * 64 + (set & 63)) * VEC + e % VEC;
+        key = id < vocab ? logit_key(to_f32(row[id])) : 0u;
+        return id < vocab && key >= bound;
+      };
+      int id;
+      unsigned int key;
+      hits = 0;
+      for (int i = t; i < listed * kLaneElems; i += kRowThreads) hits += entry(i, id, key) ? 1 : 0;
+      at = row_scan(hits, sh.wave_count, reached);
+      if (reached <= kMaxFound) {
+        found = reached;
+        if (hits > 0)
+          for (int i = t; i < listed * kLaneElems; i += kRowThreads)
+            if (entry(i, id, key)) {
+              sh.key[at] = key;
+              sh.id[at++] = id;
+            }
+        __syncthreads();
+      }
+    }
+  }
+  if (found < 0) found = find_by_digits<T>(sh, row, vocab, top);
+  // their order: a token's place is how many of the others come before it
+  for (int c = t; c < found; c += kRowThreads) {
+    const unsigned int key = sh.key[c];
+    const int id = sh.id[c];
+    int place = 0;
+    for (int i = 0; i < found; ++i) {
+      const unsigned int other = sh.key[i];
+      place += other > key || (other == key && sh.id[i] < id) ? 1 : 0;
+    }
+    if (place < top) {
+      top_ids[(long)r * top + place] = id;
+      top_logprobs[(long)r * top + place] = (to_f32(row[id]) - all.m) - log_sum;
+    }
+  }
+}
+
+// A workgroup a row (many rows).
+template <typename T>
+__global__ __launch_bounds__(kRowThreads) void logprobs_rows_kernel(const T* __restrict__ logits, long ld,
+                                                                    const int* __restrict__ tokens, int vocab, int top,
+                                                                    float* __restrict__ logprob, float* __restrict__ entropy,
+                                                                    int* __restrict__ rank, int* __restrict__ top_ids,
+                                                                    float* __restrict__ top_logprobs) {
+  extern __shared__ float set_max[];  // [pieces * 64] where alternatives are asked for
+  __shared__ FinishShared sh;
+  const int r = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const T* row = logits + (long)r * ld;
+  const int pieces = (vocab + kPiece - 1) / kPiece;
+  const int given = tokens[r];
+  const float mine = given >= 0 && given < vocab ? to_f32(row[given]) : 0.f;
+  LaneSums sums{-INFINITY, 0.f, 0.f};
+  int before = 0;
+  for (int p = w; p < pieces; p += kStreams) {
+    float x[kLaneElems];
+    load_piece<T>(x, row, p, vocab, lane);
+    const LaneSums here = piece_sums<T>(x, p, given, mine, before, lane);
+    if (top > 0) set_max[p * 64 + lane] = here.m;
+    sums = fold_sums(sums, here);
+  }
+  finish_row<T>(sh, set_max, sums, before, row, vocab, pieces, given, mine, top, r, logprob, entropy, rank, top_ids,
+                top_logprobs);
+}
+
+// A wave a piece (few rows): the lanes' sums to part[row][piece][3][64], the count to count[row][piece].
+constexpr int kPieceThreads = 256;
+template <typename T>
+__global__ __launch_bounds__(kPieceThreads) void logprobs_pieces_kernel(const T* __restrict__ logits, long ld,
+                                                                        const int* __restrict__ tokens, int vocab,
+                                                                        int pieces, float* __restrict__ part,
+                                                                        int* __restrict__ count) {
+  const int r = blockIdx.y, lane = threadIdx.x & 63;
+  const int p = blockIdx.x * (kPieceThreads / 64) + (threadIdx.x >> 6);
+  if (p >= pieces) return;  // (no wave waits for another)
+  const T* row = logits + (long)r * ld;
+  float x[kLaneElems];
+  load_piece<T>(x, row, p, vocab, lane);
+  const int given = tokens[r];
+  const float mine = given >= 0 && given < vocab ? to_f32(row[given]) : 0.f;
+  int before = 0;
+  const LaneSums here = piece_sums<T>(x, p, given, mine, before, lane);
+  const long at = (long)r * pieces + p;
+  part[at * 192 + lane] = here.m;
+  part[at * 192 + 64 + lane] = here.s;
+  part[at * 192 + 128 + lane] = here.t;
+  if (lane == 0) count[at] = before;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kRowThreads) void logprobs_fold_kernel(const T* __restrict__ logits, long ld,
+                                                                    const int* __restrict__ tokens, int vocab, int pieces,
+                                                                    const float* __restrict__ part, const int* __restrict__ count,
+                                                                    int top, float* __restrict__ logprob,
+                                                                    float* __restrict__ entropy, int* __restrict__ rank,
+                                                                    int* __restrict__ top_ids, float* __restrict__ top_logprobs) {
+  extern __shared__ float set_max[];
+  __shared__ FinishShared sh;
+  const int r = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const T* row = logits + (long)r * ld;
+  const int given = tokens[r];
+  const float mine = given >= 0 && given < vocab ? to_f32(row[given]) : 0.f;
+  LaneSums sums{-INFINITY, 0.f, 0.f};
+  int before = 0;
+#pragma unroll 4
+  for (int p = w; p < pieces; p += kStreams) {
+    const long at = (long)r * pieces + p;
+    const LaneSums here{part[at * 192 + lane], part[at * 192 + 64 + lane], part[at * 192 + 128 + lane]};
+    before += count[at];
+    if (top > 0) set_max[p * 64 + lane] = here.m;
+    sums = fold_sums(sums, here);
+  }
+  finish_row<T>(sh, set_max, sums, before, row, vocab, pieces, given, mine, top, r, logprob, entropy, rank, top_ids,
+                top_logprobs);
+}
+
+inline int logprob_pieces(int vocab) { return (vocab + kPiece - 1) / kPiece; }
+// With fewer rows than compute units a workgroup a row leaves units idle.
+inline bool logprobs_by_pieces(int rows, int vocab) { return rows < compute_units() && vocab > kRowThreads; }
+
+template <typename T>
+int run_logprobs(const void* logits, long ld, const int* tokens, int rows, int vocab, int top, float* logprob, float* entropy,
+                 int* rank, int* top_ids, float* top_logprobs, void* scratch, hipStream_t stream) {
+  const int pieces = logprob_pieces(vocab);
+  const size_t lds = top > 0 ? sizeof(float) * 64 * (size_t)pieces : 0;
+  const T* x = static_cast<const T*>(logits);
+  if (logprobs_by_pieces(rows, vocab)) {
+    LS_REQUIRE(rows <= 65535, "token_logprobs: %d rows", rows);
+    if (lds > 48 * 1024) {
+      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(logprobs_fold_kernel<T>),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024 + 1024);
+      LS_REQUIRE(e == hipSuccess, "token_logprobs: %s", hipGetErrorString(e));
+    }
+    float* part = static_cast<float*>(scratch);
+    int* count = reinterpret_cast<int*>(part + (size_t)rows * pieces * 192);
+    const int waves = kPieceThreads / 64;
+    logprobs_pieces_kernel<T><<<dim3((pieces + waves - 1) / waves, rows), kPieceThreads, 0, stream>>>(x, ld, tokens, vocab,
+                                                                                                 pieces, part, count);
+    logprobs_fold_kernel<T><<<rows, kRowThreads, lds, stream>>>(x, ld, tokens, vocab, pieces, part, count, top, logprob,
+                                                               entropy, rank, top_ids, top_logprobs);
+  } else {
+    if (lds > 48 * 1024) {
+      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(logprobs_rows_kernel<T>),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024 + 1024);
+      LS_REQUIRE(e == hipSuccess, "token_logprobs: %s", hipGetErrorString(e));
+    }
+    logprobs_rows_kernel<T><<<rows, kRowThreads, lds, stream>>>(x, ld, tokens, vocab, top, logprob, entropy, rank, top_ids,
+                                                               top_logprobs);
+  }
+  return check_launch("token_logprobs");
+}
+
+}  // namespace ls
+
+extern "C" int ls_logprobs_max_vocab() { return ls::kMaxVocab; }
+extern "C" int ls_logprobs_max_top() { return ls::kMaxTop; }
+
+extern "C" long ls_logprobs_scratch_bytes(int rows, int vocab) {
+  if (rows <= 0 || vocab <= 0 || !ls::logprobs_by_pieces(rows, vocab)) return 0;
+  return (long)rows * ls::logprob_pieces(vocab) * (192 + 1) * (long)sizeof(float);
+}
+
+extern "C" int ls_token_logprobs(int dtype, const void* logits, long ld, const int* tokens, int rows, int vocab, int top,
+                                 float* logprob, float* entropy, int* rank, int* top_ids, float* top_logprobs,
+                                 void* scratch, long scratch_bytes, void* stream) {
+  using namespace ls;
+  LS_REQUIRE(dtype == kF32 || dtype == kBF16, "token_logprobs: dtype %d", dtype);
+  LS_REQUIRE(rows >= 1 && vocab >= 1 && vocab <= kMaxVocab && top >= 0 && top <= kMaxTop && top <= vocab && ld >= 0,
+             "token_logprobs: %d rows of %d logits, %d alternatives", rows, vocab, top);
+  LS_REQUIRE(scratch_bytes >= ls_logprobs_scratch_bytes(rows, vocab), "token_logprobs: %ld bytes of scratch", scratch_bytes);
+  if (dtype == kF32)
+    return run_logprobs<float>(logits, ld, tokens, rows, vocab, top, logprob, entropy, rank, top_ids, top_logprobs, scratch,
+                               (hipStream_t)stream);
+  return run_logprobs<bf16_t>(logits, ld, tokens, rows, vocab, top, logprob, entropy, rank, top_ids, top_logprobs, scratch,
+                              (hipStream_t)stream);
+}

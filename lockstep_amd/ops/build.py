@@ -19,6 +19,11 @@ Two kinds of library exist:
 ``sink<D>x<DV>``    grouped-query attention with a sink in the softmax, windows or
                     chunks of keys, a bias by distance and an output gate, for one
                     key size and one value size;
+``serving``         what stands around a step: block tables and slot maps built on
+                    the GPU, keys and values into pages of 4 bits and back, log
+                    probabilities of given tokens;
+``fp4attention<D>`` attention over pages of keys and values in 4 bits for one head
+                    size ``D``;
 ``experts``         routing of tokens to a few of many small feed-forward experts
                     and the grouped products of those experts.
 
@@ -57,6 +62,8 @@ MIXERS_SOURCES = ("mixers.hip", "latent_delta.hip", "sublayers.hip", "memory.hip
 TALKING_SOURCES = ("talking_attention.hip",)
 SINK_SOURCES = ("sink_attention.hip",)
 EXPERTS_SOURCES = ("experts.hip",)
+SERVING_SOURCES = ("tables.hip", "logprobs.hip", "fp4_pages.hip")
+FP4_ATTENTION_SOURCES = ("fp4_attention.hip",)
 
 
 class BuildError(RuntimeError):
@@ -240,6 +247,18 @@ def build_experts(force: bool = False) -> Path:
     return build("experts", EXPERTS_SOURCES, (), force)
 
 
+def build_serving(force: bool = False) -> Path:
+    return build("serving", SERVING_SOURCES, (), force)
+
+
+def build_fp4_attention(head_dim: int, force: bool = False) -> Path:
+    """The library of attention over pages in 4 bits for one head size."""
+    if head_dim % 32 or not 32 <= head_dim <= 256:
+        raise BuildError(
+            f"head size {head_dim} is not supported: attention over pages in 4 bits takes multiples of 32 from 32 to 256")
+    return build(f"fp4attention{head_dim}", FP4_ATTENTION_SOURCES, (f"-DLS_HEAD_DIM={head_dim}",), force)
+
+
 MUTANT_DEFINE = "-DLS_MUTANTS"
 
 
@@ -254,6 +273,8 @@ def build_attention_mutants(head_dim: int, force: bool = False) -> Path:
 
 
 DEFAULT_HEAD_DIMS = (16, 32, 48, 64, 80, 112, 128, 144, 160, 192, 256)
+#: head sizes of attention over pages in 4 bits that the tests and measurements use
+DEFAULT_FP4_HEAD_DIMS = (32, 64, 96, 128, 160, 224, 256)
 MUTANT_HEAD_DIMS = (16, 32, 128)     # the head sizes of the tests that use the controls
 #: (query heads, kv heads, key size, value size) of the talking-heads attention the tests and measurements use
 DEFAULT_TALKING_SHAPES = ((4, 2, 32, 16), (6, 3, 48, 24), (3, 1, 24, 40), (2, 2, 16, 16), (16, 8, 128, 128),
@@ -265,12 +286,15 @@ DEFAULT_SINK_SHAPES = ((16, 16), (32, 16), (24, 24), (40, 40), (32, 32), (24, 6)
 
 
 def build_all(head_dims=DEFAULT_HEAD_DIMS, force: bool = True, mutants: bool = True,
-              talking_shapes=DEFAULT_TALKING_SHAPES, sink_shapes=DEFAULT_SINK_SHAPES) -> list[Path]:
+              talking_shapes=DEFAULT_TALKING_SHAPES, sink_shapes=DEFAULT_SINK_SHAPES,
+              fp4_head_dims=DEFAULT_FP4_HEAD_DIMS) -> list[Path]:
     """Compile the core library, the mixers library, the attention library of each head size and the
     talking-heads attention library of each shape, the sink attention
-    library of each key and value size and the experts library, a few at a time; with ``mutants`` also the control
+    library of each key and value size, the experts and the serving library and attention over pages in 4 bits for each of
+    its head sizes, a few at a time; with ``mutants`` also the control
     libraries of the tests."""
     jobs = [lambda: build_core(force), lambda: build_mixers(force), lambda: build_experts(force)]
+    jobs += [lambda: build_serving(force)] + [lambda d=d: build_fp4_attention(d, force) for d in fp4_head_dims]
     jobs += [lambda shape=shape: build_sink(*shape, force) for shape in sink_shapes]
     jobs += [lambda d=d: build_attention(d, force) for d in head_dims]
     jobs += [lambda shape=shape: build_talking(*shape, force) for shape in talking_shapes]

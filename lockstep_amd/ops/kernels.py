@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 from ctypes import c_float, c_int, c_long, c_void_p
+from typing import NamedTuple
 
 import torch
 
@@ -65,6 +66,49 @@ def _rows_ok(t: torch.Tensor, name: str) -> None:
                           f"strides {t.stride()} on {t.device}")
 
 
+class Fp4Pages(NamedTuple):
+    """A pool of pages of keys and values in 4 bits (csrc/fp4.h has the layout and the number format): uint8 tensors
+
+    ``k_codes`` [pages, kv heads, page size, d/2], ``k_scales`` [pages, kv heads, page size, d/32],
+    ``v_codes`` [pages, kv heads, page size/4, d/8, 4, 4], ``v_scales`` [pages, kv heads, page size/4, d/32, 4].
+
+    17/32 bytes an element of a key or value; ``d`` is a multiple of 32 up to 256, the page size a power of two from 4 on."""
+
+    k_codes: torch.Tensor
+    k_scales: torch.Tensor
+    v_codes: torch.Tensor
+    v_scales: torch.Tensor
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, page_size: int, d: int, device="cuda") -> "Fp4Pages":
+        """A pool of zeros."""
+        pool = cls(*(torch.zeros(shape, dtype=torch.uint8, device=device)
+                     for shape in cls.shapes(pages, kv_heads, page_size, d)))
+        return pool
+
+    @staticmethod
+    def shapes(pages: int, kv_heads: int, page_size: int, d: int) -> tuple:
+        if not (pages >= 1 and kv_heads >= 1 and page_size >= 4 and page_size & (page_size - 1) == 0):
+            raise KernelError(f"pages in 4 bits: {pages} pages of {page_size} tokens and {kv_heads} heads (the page size is a "
+                              "power of two from 4 on)")
+        if not (d % 32 == 0 and 32 <= d <= MAX_HEAD_DIM):
+            raise KernelError(f"pages in 4 bits: heads of {d} elements, multiples of 32 up to {MAX_HEAD_DIM} are supported")
+        return ((pages, kv_heads, page_size, d // 2), (pages, kv_heads, page_size, d // 32),
+                (pages, kv_heads, page_size // 4, d // 8, 4, 4), (pages, kv_heads, page_size // 4, d // 32, 4))
+
+    def geometry(self) -> tuple[int, int, int, int]:
+        """(pages, kv heads, page size, d), checked."""
+        if not (self.k_codes.dim() == 4):
+            raise KernelError(f"pages in 4 bits: key codes must be 4-D, got {tuple(self.k_codes.shape)}")
+        pages, kv_heads, page_size, half = self.k_codes.shape
+        for name, t, shape in zip(self._fields, self, self.shapes(pages, kv_heads, page_size, 2 * half)):
+            if not (t.is_cuda and t.dtype == torch.uint8 and t.is_contiguous() and t.shape == shape
+                    and t.device == self.k_codes.device and t.data_ptr() % 16 == 0):
+                raise KernelError(f"pages in 4 bits: {name} must be contiguous, 16-byte aligned uint8 {list(shape)} on one GPU, got "
+                                  f"{t.dtype} {list(t.shape)} on {t.device}")
+        return pages, kv_heads, page_size, 2 * half
+
+
 class Kernels:
     """The loaded libraries.  One instance per process (see ``kernels()``)."""
 
@@ -87,6 +131,10 @@ class Kernels:
         self.sink_paths: dict[tuple, str] = {}
         self._experts = None
         self.experts_path = None
+        self._serving = None
+        self.serving_path = None
+        self._fp4_attention: dict[int, ctypes.CDLL] = {}
+        self.fp4_attention_paths: dict[int, str] = {}
         self._argmax_scratch: dict = {}
         self._sample_scratch: dict = {}
         self._sample_scratch_kept: list = []
@@ -1940,6 +1988,227 @@ class Kernels:
         self._launch(lib, lib.ls_gated_parts_norm, (
             c_int(DTYPE_CODE[out.dtype]), _ptr(y), c_long(y.stride(0)), _ptr(z), c_long(z.stride(0)), c_int(t), c_int(inner),
             c_int(parts), _ptr(weight), c_float(eps), _ptr(out), c_long(out.stride(0)), _stream()))
+
+    # -- around a step: tables, pages in 4 bits, log probabilities -------------------------
+    @property
+    def serving(self):
+        if self._serving is None:
+            path = _build.build_serving()
+            lib = ctypes.CDLL(str(path))
+            lib.ls_last_error.restype = ctypes.c_char_p
+            lib.ls_logprobs_scratch_bytes.restype = c_long
+            self._serving = lib
+            self.serving_path = str(path)
+        return self._serving
+
+    def fp4_attention_lib(self, head_dim: int):
+        lib = self._fp4_attention.get(head_dim)
+        if lib is None:
+            path = _build.build_fp4_attention(head_dim)
+            lib = ctypes.CDLL(str(path))
+            lib.ls_last_error.restype = ctypes.c_char_p
+            lib.ls_fp4_attention_scratch_bytes.restype = c_long
+            if not (lib.ls_fp4_attention_head_dim() == head_dim):
+                raise KernelError(f"{path} was built for another head size")
+            self._fp4_attention[head_dim] = lib
+            self.fp4_attention_paths[head_dim] = str(path)
+        return lib
+
+    @staticmethod
+    def _here(device, what: str) -> None:
+        """Launches go to the current device's stream: operands on another device are refused."""
+        if device.index != (_raw_device() if _raw_device is not None else torch.cuda.current_device()):
+            raise KernelError(f"{what} works on {device}, which is not the current device")
+
+    @staticmethod
+    def _ints(t, n, what: str, device) -> None:
+        if not (t.is_cuda and t.device == device and t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous()
+                and (n is None or t.shape[0] == n)):
+            raise KernelError(f"{what} must be a contiguous int32 vector{'' if n is None else f' of {n}'} on {device}, got "
+                              f"{t.dtype} {list(t.shape)} on {t.device}")
+
+    def step_tables(self, lengths: torch.Tensor, news: torch.Tensor, table: torch.Tensor, page_size: int,
+                    free_pages: torch.Tensor, cursor: torch.Tensor, slots: torch.Tensor, tok_seq: torch.Tensor,
+                    tok_pos: torch.Tensor, offsets: torch.Tensor, new_lengths: torch.Tensor,
+                    progress: torch.Tensor) -> None:
+        """Block tables and slot maps of one step, built on the GPU (all tensors int32 there).
+
+        Request i holds ``lengths[i]`` tokens, in the pages of row i of ``table [requests, columns]``, and brings
+        ``news[i]`` more.  Pages that it lacks are taken from ``free_pages`` from entry ``cursor[0]`` on, in the order of
+        the requests, and written into its row; no other entry of the table changes.  For the packed tokens of the step
+        (request 0's first): ``slots`` (page * page size + place in the page; -1 where the table has no page),
+        ``tok_seq`` (the request) and ``tok_pos`` (the position); entries behind the last token become -1.
+        ``offsets [requests + 1]``: first packed token of every request, and their number; ``new_lengths``: lengths
+        after the step; ``progress [2]``: the cursor after the step, and how many requests were refused.
+
+        A request is refused (it brings no tokens and gets no pages) if its numbers are negative or exceed its row of the
+        table; and from the first request on for which the free list, or the room of ``slots``, does not suffice, every
+        later one that needs a page (brings a token).  Inputs and outputs must not overlap."""
+        requests = lengths.shape[0] if lengths.dim() == 1 else -1
+        device = lengths.device
+        self._ints(lengths, None, "step_tables lengths", device)
+        self._here(device, "step_tables")
+        for name, t, n in (("news", news, requests), ("cursor", cursor, 1), ("free_pages", free_pages, None),
+                           ("slots", slots, None), ("tok_seq", tok_seq, slots.shape[0]), ("tok_pos", tok_pos, slots.shape[0]),
+                           ("offsets", offsets, requests + 1), ("new_lengths", new_lengths, requests),
+                           ("progress", progress, 2)):
+            self._ints(t, n, f"step_tables {name}", device)
+        if not (table.is_cuda and table.device == device and table.dtype == torch.int32 and table.dim() == 2
+                and table.is_contiguous() and table.shape[0] == requests and table.shape[1] >= 1):
+            raise KernelError(f"step_tables table must be a contiguous int32 matrix of {requests} rows, got {list(table.shape)}")
+        if not (page_size >= 4 and page_size & (page_size - 1) == 0):
+            raise KernelError(f"step_tables: a page size is a power of two from 4 on, got {page_size}")
+        if table.shape[1] * page_size > 0x7FFFFFFF:
+            raise KernelError("step_tables: positions beyond 31 bits")
+        limit = self._memo(("tables_requests",), lambda: int(self.serving.ls_step_tables_max_requests()))
+        if requests > limit:
+            raise KernelError(f"step_tables takes at most {limit} requests, got {requests}")
+        ins = [(t.data_ptr(), t.data_ptr() + 4 * t.numel()) for t in (lengths, news, free_pages, cursor)]
+        outs = [(t.data_ptr(), t.data_ptr() + 4 * t.numel())
+                for t in (table, slots, tok_seq, tok_pos, offsets, new_lengths, progress)]
+        for i, (lo, hi) in enumerate(outs):
+            if any(lo < other_hi and other_lo < hi for other_lo, other_hi in ins + outs[:i]):
+                raise KernelError("step_tables: outputs overlap one another or an input")
+        lib = self.serving
+        self._launch(lib, lib.ls_step_tables, (
+            _ptr(lengths), _ptr(news), c_int(requests), _ptr(table), c_int(table.shape[1]), c_int(page_size),
+            _ptr(free_pages), c_int(free_pages.shape[0]), _ptr(cursor), _ptr(slots), _ptr(tok_seq), _ptr(tok_pos),
+            c_int(slots.shape[0]), _ptr(offsets), _ptr(new_lengths), _ptr(progress), _stream()))
+
+    def _fp4_rows(self, what: str, k, v, slots, pages: Fp4Pages):
+        count, kv_heads, page_size, d = pages.geometry()
+        device = pages.k_codes.device
+        self._here(device, what)
+        if count * page_size > 0x7FFFFFFF:
+            raise KernelError(f"{what}: slots beyond 31 bits")
+        for name, t in (("keys", k), ("values", v)):
+            _rows_ok(t, f"{what} {name}")
+            if not (t.dtype in DTYPE_CODE and t.dtype == k.dtype and t.device == device
+                    and t.shape == (k.shape[0], kv_heads * d) and t.stride(0) >= 0):
+                raise KernelError(f"{what} {name} must be float32 or bfloat16 [{k.shape[0]},{kv_heads * d}] on {device}, got "
+                                  f"{t.dtype} {list(t.shape)} on {t.device}")
+        self._ints(slots, k.shape[0], f"{what} slots", device)
+        return count, kv_heads, page_size, d
+
+    def fp4_write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pages: Fp4Pages) -> None:
+        """Keys and values ``[tokens, kv heads * d]`` (float32 or bfloat16, rows may be parts of wider ones) rounded to 4
+        bits into the slots (page * page size + place in the page) of ``pages``; a token whose slot is negative or
+        beyond the pool is left out.  Every group of 32 elements gets a power of two as its scale; a group with an
+        infinity or a NaN is held as NaN.  The slots of a call are distinct: of two tokens with one slot a mix remains."""
+        count, kv_heads, page_size, d = self._fp4_rows("fp4_write", k, v, slots, pages)
+        if k.shape[0] == 0:
+            return
+        lib = self.serving
+        self._launch(lib, lib.ls_fp4_write, (
+            c_int(DTYPE_CODE[k.dtype]), _ptr(k), c_long(k.stride(0)), _ptr(v), c_long(v.stride(0)), _ptr(slots),
+            c_int(k.shape[0]), c_int(kv_heads), c_int(d), _ptr(pages.k_codes), _ptr(pages.k_scales), _ptr(pages.v_codes),
+            _ptr(pages.v_scales), c_int(count), c_int(page_size), _stream()))
+
+    def fp4_read(self, pages: Fp4Pages, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+        """The keys and values that the slots hold, as float32 or bfloat16 (both exact) rows ``[tokens, kv heads * d]``;
+        rows whose slot is negative or beyond the pool stay as they are."""
+        count, kv_heads, page_size, d = self._fp4_rows("fp4_read", k, v, slots, pages)
+        for name, t in (("keys", k), ("values", v)):
+            if not (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]):
+                raise KernelError(f"fp4_read {name}: rows overlap")
+        if k.shape[0] == 0:
+            return
+        lib = self.serving
+        self._launch(lib, lib.ls_fp4_read, (
+            c_int(DTYPE_CODE[k.dtype]), _ptr(k), c_long(k.stride(0)), _ptr(v), c_long(v.stride(0)), _ptr(slots),
+            c_int(k.shape[0]), c_int(kv_heads), c_int(d), _ptr(pages.k_codes), _ptr(pages.k_scales), _ptr(pages.v_codes),
+            _ptr(pages.v_scales), c_int(count), c_int(page_size), _stream()))
+
+    def fp4_attention(self, q: torch.Tensor, nq: int, nkv: int, d: int, pages: Fp4Pages, table: torch.Tensor,
+                      offsets: torch.Tensor, lengths: torch.Tensor, max_tokens: int, max_length: int,
+                      out: torch.Tensor, scale: float, window: int = 0) -> None:
+        """Causal attention of packed query rows over pages in 4 bits.
+
+        ``q [tokens, >= nq * d]`` (float32 or bfloat16; ``out`` likewise): request i has the rows ``offsets[i]`` to
+        ``offsets[i + 1] - 1``, the last of them at position ``lengths[i] - 1`` (its key and value are in the pages
+        already); ``table [requests, columns]`` are the block tables (int32, as are offsets and lengths).  With a
+        ``window`` a row sees that many keys, its own among them.  ``max_tokens`` and ``max_length``: the most rows and
+        the greatest length of any request; they size the launches, so rows or keys beyond them are not computed.  Rows
+        that belong to no request stay as they are; a row that sees no key (a length of 0, pages that the table does not
+        have) becomes zeros.  Keys whose page is negative or beyond the pool are not seen.  A row's result depends on its
+        own request only, not on what else is in the step, but for the rounding between requests of at most 16 rows a
+        key/value head and longer ones, which go through different kernels."""
+        count, kv_heads, page_size, dim = pages.geometry()
+        device = q.device
+        _rows_ok(q, "fp4_attention q"); _rows_ok(out, "fp4_attention out")
+        self._here(device, "fp4_attention")
+        if not (q.dtype in DTYPE_CODE and out.dtype == q.dtype and out.device == device and pages.k_codes.device == device):
+            raise KernelError(f"fp4_attention: q {q.dtype} on {q.device}, out {out.dtype} on {out.device}, pages on "
+                              f"{pages.k_codes.device}")
+        if not (dim == d and kv_heads == nkv and nkv >= 1 and nq >= nkv and nq % nkv == 0):
+            raise KernelError(f"fp4_attention: {nq} query heads over {nkv} of {d}, pages of {kv_heads} heads of {dim}")
+        if not (q.shape[1] >= nq * d and out.shape[1] >= nq * d and out.shape[0] == q.shape[0] and q.stride(0) >= 0
+                and (out.shape[0] <= 1 or out.stride(0) >= nq * d)):
+            raise KernelError(f"fp4_attention: rows q {list(q.shape)}, out {list(out.shape)} for {nq} heads of {d}")
+        if not (table.is_cuda and table.device == device and table.dtype == torch.int32 and table.dim() == 2
+                and table.is_contiguous() and table.shape[1] >= 1):
+            raise KernelError("fp4_attention block tables must be a contiguous int32 matrix on the GPU")
+        requests = table.shape[0]
+        self._ints(offsets, requests + 1, "fp4_attention offsets", device)
+        self._ints(lengths, requests, "fp4_attention lengths", device)
+        if not (0 <= max_tokens and 0 <= max_length <= table.shape[1] * page_size and window >= 0 and requests <= 65535
+                and nkv <= 1024):
+            raise KernelError(f"fp4_attention: at most {max_tokens} rows and {max_length} keys a request, window {window}, "
+                              f"{requests} requests with {table.shape[1]} pages of {page_size}, {nkv} kv heads")
+        max_tokens = min(max_tokens, q.shape[0])
+        if max_tokens == 0 or requests == 0:
+            return
+        lib = self.fp4_attention_lib(d)
+        code, group = DTYPE_CODE[q.dtype], nq // nkv
+        need = lib.ls_fp4_attention_scratch_bytes(c_int(code), c_int(requests), c_int(nkv), c_int(group), c_int(max_tokens),
+                                                  c_int(max_length), c_int(window))
+        # (of the call's stream, and of the graph's own memory while one is captured: no two calls share it)
+        scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        self._launch(lib, lib.ls_fp4_attention, (
+            c_int(code), _ptr(q), c_long(q.stride(0)), _ptr(out), c_long(out.stride(0)), c_int(q.shape[0]),
+            _ptr(pages.k_codes), _ptr(pages.k_scales), _ptr(pages.v_codes), _ptr(pages.v_scales), c_int(count),
+            c_int(page_size), c_int(nkv), c_int(group), _ptr(table), c_int(table.shape[1]), _ptr(offsets), _ptr(lengths),
+            c_int(requests), c_int(max_tokens), c_int(max_length), c_float(scale), c_int(window), _ptr(scratch),
+            c_long(need), _stream()))
+
+    def token_logprobs(self, logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tensor, entropy: torch.Tensor,
+                       rank: torch.Tensor, top_ids: torch.Tensor, top_logprobs: torch.Tensor) -> None:
+        """Log probabilities of the given ``tokens [rows]`` (int32) under the softmax of ``logits [rows, vocabulary]``
+        (float32 or bfloat16): ``logprob`` and ``entropy`` (natural logarithms, float32 ``[rows]``), ``rank`` (int32: how many
+        tokens come before it, larger logits first, then lower ids) and the first ``k`` tokens of that order, ``top_ids``
+        (int32) and ``top_logprobs`` (float32) ``[rows, k]``, k from 0 to 32 and at most the vocabulary.
+
+        A token outside the vocabulary (-1: none) gets NaN and the rank -1.  A NaN counts as larger than every number; rows
+        with a NaN, with an infinity of +, or with nothing but -inf have NaN for what the formula leaves undefined."""
+        _rows_ok(logits, "token_logprobs logits")
+        device = logits.device
+        self._here(device, "token_logprobs")
+        rows, vocab = logits.shape
+        if not (logits.dtype in DTYPE_CODE and logits.stride(0) >= 0):
+            raise KernelError(f"token_logprobs logits must be float32 or bfloat16, got {logits.dtype}")
+        self._ints(tokens, rows, "token_logprobs tokens", device)
+        self._ints(rank, rows, "token_logprobs rank", device)
+        for name, t, shape in (("logprob", logprob, (rows,)), ("entropy", entropy, (rows,)),
+                               ("top_logprobs", top_logprobs, tuple(top_ids.shape))):
+            if not (t.is_cuda and t.device == device and t.dtype == torch.float32 and t.is_contiguous() and t.shape == shape):
+                raise KernelError(f"token_logprobs {name} must be contiguous float32 {list(shape)} on {device}, got "
+                                  f"{t.dtype} {list(t.shape)} on {t.device}")
+        lib = self.serving
+        most, widest = self._memo(("logprobs",), lambda: (int(lib.ls_logprobs_max_top()), int(lib.ls_logprobs_max_vocab())))
+        if not (top_ids.is_cuda and top_ids.device == device and top_ids.dtype == torch.int32 and top_ids.is_contiguous()
+                and top_ids.dim() == 2 and top_ids.shape[0] == rows and top_ids.shape[1] <= min(most, vocab)):
+            raise KernelError(f"token_logprobs top_ids must be contiguous int32 [{rows}, at most {min(most, vocab)}], got "
+                              f"{top_ids.dtype} {list(top_ids.shape)}")
+        if rows == 0:
+            return
+        if not (1 <= vocab <= widest):
+            raise KernelError(f"token_logprobs takes 1 to {widest} logits a row, got {vocab}")
+        need = lib.ls_logprobs_scratch_bytes(c_int(rows), c_int(vocab))
+        scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        self._launch(lib, lib.ls_token_logprobs, (
+            c_int(DTYPE_CODE[logits.dtype]), _ptr(logits), c_long(logits.stride(0)), _ptr(tokens), c_int(rows), c_int(vocab),
+            c_int(top_ids.shape[1]), _ptr(logprob), _ptr(entropy), _ptr(rank), _ptr(top_ids), _ptr(top_logprobs),
+            _ptr(scratch), c_long(need), _stream()))
 
 
 ATTENTION_ITEM_INTS = 32

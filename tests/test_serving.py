@@ -1,0 +1,88 @@
+"""Block tables on the GPU, pages in 4 bits and log probabilities: what is refused before anything is launched, and the
+plain implementations against one another (no GPU needed)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+from plain import serving_plain as plain
+
+from lockstep_amd.ops import Fp4Pages, KernelError, kernels
+from lockstep_amd.ops import build as kernel_build
+
+
+def test_nearest_levels():
+    x = torch.zeros(64)
+    x[:9] = torch.tensor([6.0, 0.25, 0.75, 1.25, -1.75, 2.5, 3.5, -5.0, 5.1])
+    want = torch.zeros(64, dtype=torch.float64)
+    want[:9] = torch.tensor([6.0, 0.0, 1.0, 1.0, -2.0, 2.0, 4.0, -4.0, 6.0])
+    assert torch.equal(plain.held(x), want)
+    big = torch.zeros(32)
+    big[0], big[1] = 7.9, 0.2           # the scale is 1: beyond 6 is 6, and 0.2 is nothing
+    assert plain.held(big)[0] == 6 and plain.held(big)[1] == 0
+    big[3] = float("inf")
+    assert torch.isnan(plain.held(big)).all()
+
+
+def test_plain_tables_refuse_from_the_first_request_that_does_not_fit():
+    table = [[7, -1], [-1, -1], [-1, -1], [9, 8], [-1, -1]]
+    found = plain.step_tables([4, 0, 0, 16, 0], [3, 9, 17, 0, 2], table, 8, [5, 6, 3], 0, 20)
+    # request 1 takes two pages, request 2 exceeds its row, request 3 is full and brings nothing
+    assert found["progress"] == [3, 1]
+    assert found["offsets"] == [0, 3, 12, 12, 12, 14]
+    assert found["slots"][:3] == [60, 61, 62] and found["slots"][3] == 40 and found["slots"][11] == 48
+    assert found["slots"][12:14] == [24, 25] and found["slots"][14:] == [-1] * 6
+    assert table == [[7, -1], [5, 6], [-1, -1], [9, 8], [3, -1]]
+    table = [[-1], [-1], [-1]]
+    found = plain.step_tables([0, 0, 0], [2, 2, 2], table, 8, [1], 0, 20)
+    assert found["progress"] == [1, 2] and found["offsets"] == [0, 2, 2, 2] and table == [[1], [-1], [-1]]
+
+
+def test_page_shapes():
+    assert Fp4Pages.shapes(3, 2, 16, 96) == ((3, 2, 16, 48), (3, 2, 16, 3), (3, 2, 4, 12, 4, 4), (3, 2, 4, 3, 4))
+    for bad in ((0, 2, 16, 96), (3, 0, 16, 96), (3, 2, 12, 96), (3, 2, 2, 96), (3, 2, 16, 80), (3, 2, 16, 288), (3, 2, 16, 0)):
+        with pytest.raises(KernelError):
+            Fp4Pages.shapes(*bad)
+    with pytest.raises(kernel_build.BuildError):
+        kernel_build.build_fp4_attention(48)
+
+
+def test_tensors_on_the_host_are_refused():
+    k = kernels()
+    i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    pages = Fp4Pages.empty(2, 1, 16, 32, device="cpu")
+    with pytest.raises(KernelError, match="step_tables"):
+        k.step_tables(i(2), i(2), i(2, 2), 16, i(4), i(1), i(8), i(8), i(8), i(3), i(2), i(2))
+    with pytest.raises(KernelError, match="pages in 4 bits"):
+        k.fp4_write(torch.zeros(2, 32), torch.zeros(2, 32), i(2), pages)
+    with pytest.raises(KernelError, match="pages in 4 bits"):
+        k.fp4_read(pages, i(2), torch.zeros(2, 32), torch.zeros(2, 32))
+    with pytest.raises(KernelError, match="pages in 4 bits"):
+        k.fp4_attention(torch.zeros(2, 32), 1, 1, 32, pages, i(1, 2), i(2), i(1), 2, 8, torch.zeros(2, 32), 1.0)
+    with pytest.raises(KernelError, match="logits"):
+        k.token_logprobs(torch.zeros(2, 9), i(2), torch.zeros(2), torch.zeros(2), i(2), i(2, 0), torch.zeros(2, 0))
+
+
+def test_the_plan_of_the_splits_covers_every_request():
+    """The launch's bounds (how many splits there are room and workgroups for) hold for every shorter request: the rule
+    of csrc/fp4_attention.hip in whole numbers."""
+    def decode_split(span):
+        return 256 if span <= 4096 else 512 if span <= 32768 else 1024 * ((span + 131071) // 131072)
+
+    def prompt_split(span, blocks):
+        want = max(1, 32 // max(1, blocks))
+        return max(512, ((span + want - 1) // want + 31) // 32 * 32)
+
+    def planned(span):
+        return max([1] + [-(-s // decode_split(s)) for s in (span, min(span, 4096), min(span, 32768), min(span, 131072)) if s])
+
+    spans = list(range(0, 5000, 7)) + list(range(32000, 34000, 13)) + list(range(130000, 1100000, 1709)) + [131072, 131073, 262144, 262145]
+    worst = 0
+    for span in sorted(spans):
+        splits = -(-span // decode_split(span))
+        worst = max(worst, splits)
+        assert worst <= planned(span), span
+        for blocks in (1, 2, 3, 5, 11, 16, 31, 32, 33, 500):
+            many = -(-span // prompt_split(span, blocks))
+            assert many <= min(32, max(1, -(-span // 512)))
+            assert blocks * many <= 32 or many <= 1

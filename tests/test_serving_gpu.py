@@ -1,0 +1,599 @@
+"""Block tables on the GPU, pages in 4 bits with their attention, and log probabilities, against plain implementations in
+64 bits; their refusals; a run of them together, captured and replayed."""
+
+from __future__ import annotations
+
+import random
+
+import pytest
+import torch
+from plain import serving_plain as plain
+
+from lockstep_amd.ops import Fp4Pages, KernelError, kernels
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}        # half a step, relative
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+# -- tables ---------------------------------------------------------------------------------------------------------
+def run_tables(lengths, news, table, page, free, cursor, room):
+    n = len(lengths)
+    out = {"slots": i32([7] * room), "tok_seq": i32([7] * room), "tok_pos": i32([7] * room), "offsets": i32([7] * (n + 1)),
+           "new_lengths": i32([7] * n), "progress": i32([7, 7])}
+    t = torch.tensor(table, dtype=torch.int32, device=DEV).reshape(n, -1 if n else 1)
+    kernels().step_tables(i32(lengths), i32(news), t, page, i32(free), i32([cursor]), out["slots"], out["tok_seq"],
+                          out["tok_pos"], out["offsets"], out["new_lengths"], out["progress"])
+    found = {k: v.tolist() for k, v in out.items()}
+    found["table"] = t.tolist()
+    return found
+
+
+def check_tables(lengths, news, table, page, free, cursor, room):
+    found = run_tables(lengths, news, table, page, free, cursor, room)
+    want = plain.step_tables(lengths, news, [list(r) for r in table], page, free, cursor, room)
+    for key in want:
+        assert found[key] == want[key], key
+
+
+@pytest.mark.parametrize("requests,longest,new,page,spare,short_rows", [
+    (1, 0, 1, 16, 0, 0), (1, 16, 1, 16, 0, 0), (1, 15, 1, 16, 0, 0), (64, 300, 1, 16, 5, 0), (7, 100, 65, 8, 0, 0),
+    (255, 40, 9, 32, 3, 0), (257, 40, 9, 4, 0, 0), (1100, 20, 7, 8, 0, 0), (3, 1000, 5000, 128, 0, 0), (40, 90, 30, 8, -9, 0),
+    (40, 90, 30, 8, 0, 55), (40, 90, 30, 8, -30, 100), (513, 10, 3, 4, -100, 400)])
+def test_tables(requests, longest, new, page, spare, short_rows):
+    rng = random.Random(requests * 31 + new)
+    lengths = [rng.randint(0, longest) for _ in range(requests)]
+    news = [rng.choice((0, 1, new, rng.randint(0, new))) for _ in range(requests)]
+    columns = -(-(longest + new) // page)
+    ids = list(range(requests * columns))
+    rng.shuffle(ids)
+    table = [[-1] * columns for _ in range(requests)]
+    for row, length in zip(table, lengths):
+        for c in range(-(-length // page)):
+            row[c] = ids.pop()
+    need = sum(-(-(h + n) // page) - -(-h // page) for h, n in zip(lengths, news))
+    cursor = rng.choice((0, 3))
+    free = [rng.randrange(1 << 20) for _ in range(max(0, cursor + need + spare))]
+    room = max(0, sum(news) + (5 if not short_rows else -short_rows))
+    check_tables(lengths, news, table, page, free, cursor, room)
+
+
+def test_tables_of_odd_requests():
+    # negative numbers, more than the row holds, a released page in the row, a negative page in the list, no free list
+    check_tables([-1, 3, 60, 8, 2, 2147483647], [2, -4, 10, 2, 0, 5], [[1] * 8, [2] * 8, [3] * 8, [4, 5] + [-1] * 6, [-1] * 8, [6] * 8], 8,
+                 [-3, 11], 0, 30)
+    check_tables([8, 20], [1, 3], [[5, -1, -1, -1], [6, 7, -1, -1]], 8, [], 0, 9)
+    check_tables([8, 20], [1, 3], [[5, -1, -1, -1], [6, 7, -1, -1]], 8, [1, 2], -1, 9)
+    check_tables([8, 20], [0, 0], [[5, -1, -1, -1], [6, 7, 1, -1]], 8, [1, 2], 5, 0)
+
+
+def test_tables_refusals():
+    k = kernels()
+    base = dict(lengths=i32([1, 2]), news=i32([1, 1]), table=torch.zeros((2, 3), dtype=torch.int32, device=DEV), page_size=8,
+                free_pages=i32([1, 2]), cursor=i32([0]), slots=i32([0] * 4), tok_seq=i32([0] * 4), tok_pos=i32([0] * 4),
+                offsets=i32([0] * 3), new_lengths=i32([0] * 2), progress=i32([0] * 2))
+    k.step_tables(**base)
+    both = i32([0] * 8)
+    for change in (dict(news=i32([1])), dict(page_size=12), dict(page_size=2), dict(cursor=i32([0, 1])), dict(tok_pos=i32([0] * 3)),
+                   dict(offsets=i32([0, 0])), dict(progress=i32([0])), dict(lengths=i32([1, 2]).long()),
+                   dict(table=torch.zeros((3, 3), dtype=torch.int32, device=DEV)), dict(table=torch.zeros((2, 6), dtype=torch.int32, device=DEV)[:, ::2]),
+                   dict(new_lengths=base["lengths"]), dict(slots=both[:4], tok_seq=both[2:6])):
+        with pytest.raises(KernelError):
+            k.step_tables(**{**base, **change})
+    many = 8193
+    with pytest.raises(KernelError, match="at most"):
+        k.step_tables(**{**base, "lengths": i32([0] * many), "news": i32([0] * many), "table": torch.zeros((many, 1), dtype=torch.int32, device=DEV),
+                         "offsets": i32([0] * (many + 1)), "new_lengths": i32([0] * many)})
+    torch.cuda.synchronize()
+
+
+def test_tables_of_the_most_requests():
+    n = 8192
+    check_tables([i % 9 for i in range(n)], [1 + i % 2 for i in range(n)], [[i, -1, -1] for i in range(n)], 8, list(range(n, 2 * n)), 0, 2 * n)
+
+
+# -- pages in 4 bits --------------------------------------------------------------------------------------------------
+def random_rows(g, tokens, heads, d, dtype):
+    x = torch.randn((tokens, heads * d), generator=g) * torch.exp(torch.randn((tokens, heads * d), generator=g))
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens,heads,d,page", [(1, 1, 32, 4), (3, 2, 64, 8), (37, 3, 96, 16), (70, 1, 128, 64), (9, 2, 256, 128), (130, 5, 160, 8)])
+def test_write_and_read(tokens, heads, d, page, dtype):
+    g = torch.Generator().manual_seed(tokens * d)
+    k, v = (random_rows(g, tokens, heads, d, dtype) for _ in range(2))
+    # values on the borders between two levels, small and large magnitudes, zeros
+    borders = torch.tensor([6.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -0.25, -0.75, -2.5, -5.0, 7.9, 0.0, -0.0, 0.2499])
+    k[0, :16] = borders.to(dtype)
+    k[0, 16:32] = 0
+    v[0, :32] = 0
+    v[tokens - 1, d - 32:d] = (v[tokens - 1, d - 32:d].float() * 2.0 ** 100).to(dtype)
+    v[tokens // 2, :32] = (v[tokens // 2, :32].float() * 2.0 ** -118).to(dtype)
+    pages = tokens // page + 3
+    pool = Fp4Pages.empty(pages, heads, page, d, device=DEV)
+    for t in pool:
+        t.random_(0, 255)           # (no 255: groups of zeros and ones in between)
+    before = [t.clone() for t in pool]
+    order = torch.randperm(pages * page, generator=g)[:tokens]
+    slots = order.to(torch.int32).to(DEV)
+    wide = torch.full((tokens, heads * d + 8), 3.0, dtype=dtype)      # rows that are parts of wider ones, not aligned to 16 bytes
+    wide[:, 1:heads * d + 1] = k
+    kernels().fp4_write(wide.to(DEV)[:, 1:heads * d + 1], v.to(DEV), slots, pool)
+    keys, values = plain.values_of_pages(pool)
+    flat = [x.transpose(1, 2).reshape(pages * page, heads * d) for x in (keys, values)]
+    assert torch.equal(flat[0][order], plain.held(k))
+    assert torch.equal(flat[1][order], plain.held(v))
+    # nothing else has changed
+    old = [x.transpose(1, 2).reshape(pages * page, heads * d) for x in plain.values_of_pages(before)]
+    rest = torch.ones(pages * page, dtype=torch.bool)
+    rest[order] = False
+    assert all(torch.equal(a[rest], b[rest]) for a, b in zip(flat, old))
+    # and back, exact in both types
+    for out_dtype in (torch.float32, torch.bfloat16):
+        rows = torch.full((tokens, heads * d + 24), 5.0, dtype=out_dtype, device=DEV)
+        other = torch.full((tokens, heads * d), 5.0, dtype=out_dtype, device=DEV)
+        kernels().fp4_read(pool, slots, rows[:, 3:heads * d + 3], other)
+        assert torch.equal(rows[:, 3:heads * d + 3].cpu().double(), plain.held(k))
+        assert torch.equal(other.cpu().double(), plain.held(v))
+        assert bool((rows[:, :3] == 5).all()) and bool((rows[:, heads * d + 3:] == 5).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_slots_that_are_none_and_groups_that_are_not_finite(dtype):
+    heads, d, page, pages = 2, 64, 8, 3
+    g = torch.Generator().manual_seed(5)
+    k, v = (random_rows(g, 6, heads, d, dtype) for _ in range(2))
+    k[1, 70], v[1, 3], v[2, 40] = float("nan"), float("inf"), float("-inf")
+    pool = Fp4Pages.empty(pages, heads, page, d, device=DEV)
+    slots = i32([0, 23, 9, -1, 24, 2147483647])
+    kernels().fp4_write(k.to(DEV), v.to(DEV), slots, pool)
+    keys, values = plain.values_of_pages(pool)
+    flat = [x.transpose(1, 2).reshape(pages * page, heads * d) for x in (keys, values)]
+    for row, slot in ((0, 0), (1, 23), (2, 9)):
+        for x, got in ((k, flat[0]), (v, flat[1])):
+            assert torch.equal(torch.nan_to_num(got[slot], nan=77.0), torch.nan_to_num(plain.held(x[row]), nan=77.0))
+    untouched = [s for s in range(24) if s not in (0, 23, 9)]
+    assert not flat[0][untouched].any() and not flat[1][untouched].any()
+    back = torch.full((6, heads * d), 5.0, dtype=dtype, device=DEV)
+    other = back.clone()
+    kernels().fp4_read(pool, slots, back, other)
+    assert torch.isnan(back[1, 64:96]).all() and torch.isnan(other[2, 32:64]).all()
+    assert bool((back[3:] == 5).all()) and bool((other[3:] == 5).all())
+
+
+def test_numbers_below_the_smallest_scale():
+    x = torch.zeros((1, 32))
+    x[0, :6] = torch.tensor([2.0 ** -126, 1.5 * 2.0 ** -127, 2.0 ** -127, 2.0 ** -128, -(2.0 ** -126), 3 * 2.0 ** -149])
+    pool = Fp4Pages.empty(1, 1, 4, 32, device=DEV)
+    kernels().fp4_write(x.to(DEV), x.to(DEV), i32([1]), pool)
+    assert torch.equal(plain.values_of_pages(pool)[0][0, 0, 1], plain.held(x[0]))
+
+
+def test_page_refusals():
+    k = kernels()
+    pool = Fp4Pages.empty(2, 2, 16, 64, device=DEV)
+    x = torch.zeros((3, 128), device=DEV)
+    s = i32([0, 1, 2])
+    k.fp4_write(x, x, s, pool)
+    for args in ((x[:, :64], x, s, pool), (x, x.bfloat16(), s, pool), (x, x[:2], s, pool), (x, x, s[:2], pool), (x, x, s.long(), pool),
+                 (x.half(), x.half(), s, pool), (x.t(), x, s, pool), (x, x, s, pool._replace(k_scales=pool.k_scales[:1])),
+                 (x, x, s, pool._replace(v_codes=pool.v_codes.float())), (x, x, s, pool._replace(v_codes=pool.v_codes.transpose(2, 3)))):
+        with pytest.raises(KernelError):
+            k.fp4_write(*args)
+    one = torch.zeros((1, 128), device=DEV)
+    with pytest.raises(KernelError, match="overlap"):
+        k.fp4_read(pool, s, one.expand(3, 128), x)
+    torch.cuda.synchronize()
+
+
+# -- attention ----------------------------------------------------------------------------------------------------------
+def make_cache(g, lengths, heads, d, page, extra_columns=0, spare_pages=3):
+    """Pages of random keys and values; what no request holds reads as NaN."""
+    need = [-(-max(n, 0) // page) for n in lengths]
+    pages = sum(need) + spare_pages
+    pool = Fp4Pages.empty(pages, heads, page, d, device=DEV)
+    for t in pool:
+        t.fill_(255)
+    ids = torch.randperm(pages, generator=g).tolist()
+    columns = max(max(need, default=0), 1) + extra_columns
+    table, slots = [], []
+    for n, c in zip(lengths, need):
+        row = [ids.pop() for _ in range(c)]
+        slots += [row[p // page] * page + p % page for p in range(max(n, 0))]
+        table.append(row + [-1] * (columns - c))
+    if slots:
+        spread = torch.exp(0.3 * torch.randn(heads * d, generator=g))
+        k, v = ((torch.randn((len(slots), heads * d), generator=g) * spread).to(DEV) for _ in range(2))
+        kernels().fp4_write(k, v, i32(slots), pool)
+    return pool, table
+
+
+def run_attention(q, heads, kv_heads, d, pool, table, offsets, lengths, window, scale=None, most=None, longest=None):
+    n = [b - a for a, b in zip(offsets, offsets[1:])]
+    out = torch.full_like(q, 9.0)
+    kernels().fp4_attention(q, heads, kv_heads, d, pool, torch.tensor(table, dtype=torch.int32, device=DEV), i32(offsets), i32(lengths),
+                            max(n) if most is None else most, max(max(lengths), 0) if longest is None else longest, out,
+                            d ** -0.5 if scale is None else scale, window=window)
+    return out
+
+
+def check_attention(out, q, heads, kv_heads, d, pool, table, offsets, lengths, page, window, scale=None):
+    keys, values = plain.values_of_pages(pool)
+    want, spread, reach = plain.attention(q, heads, kv_heads, d, keys, values, table, offsets, lengths, page,
+                                          d ** -0.5 if scale is None else scale, window)
+    rows = offsets[-1]
+    got = out[:rows, :heads * d].double().cpu()
+    want, spread, reach = want[:rows], spread[:rows], reach[:rows]
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    # A score is a sum of d products, in 32 bits: off by (d + 4) 2^-24 of the sum of their magnitudes at most, which moves a
+    # weight by that factor, and twice the output's spread (weights and their sum); a hardware exponential is within 2^-21.
+    # Weights and outputs are rounded to the type (weights in float32: three terms, exact); sums of n terms in 32 bits are
+    # off by n 2^-24 of their magnitudes, n at most the length, the folds included.
+    u = U[q.dtype]
+    weights = u if q.dtype == torch.bfloat16 else 0.0
+    sums = (max(lengths) + 64) * 2.0 ** -24
+    bound = 2 * spread * ((d + 4) * 2.0 ** -24 * reach + 2.0 ** -21) + spread * (weights + 2 * sums) + u * want.abs() + 1e-30
+    wrong = (got - want).abs() > bound
+    assert not bool(wrong.any()), ((got - want).abs() / bound).nan_to_num().max()
+    return got, want
+
+
+SHAPES = [
+    # lengths, new tokens of each, query heads, kv heads, d, page, window
+    ([1], [1], 1, 1, 32, 4, 0),
+    ([5, 1, 33], [1, 1, 1], 4, 2, 64, 8, 0),
+    ([532, 17, 256, 257], [1, 1, 1, 1], 8, 4, 128, 16, 0),
+    ([700, 0, 31, 32], [1, 1, 1, 1], 6, 2, 96, 8, 0),
+    ([300, 1000], [2, 3], 4, 1, 128, 64, 0),
+    ([90, 40], [1, 1], 16, 1, 256, 32, 0),
+    ([513], [1], 3, 3, 160, 128, 0),
+    ([400, 90], [1, 1], 2, 1, 224, 16, 77),
+    ([40], [40], 2, 2, 32, 4, 0),
+    ([100, 70], [61, 70], 4, 2, 64, 16, 0),
+    ([130, 260], [129, 131], 3, 1, 128, 16, 0),
+    ([200, 30], [100, 30], 2, 2, 256, 32, 0),
+    ([150], [77], 4, 4, 96, 8, 0),
+    ([260, 64], [70, 64], 4, 2, 128, 16, 33),
+    ([333], [50], 2, 1, 64, 8, 1),
+    # prompts beside decoded tokens, requests that bring nothing, splits of a short portion of a long context
+    ([150, 500, 20, 90, 0], [60, 1, 0, 2, 0], 8, 2, 128, 16, 0),
+    ([2100], [20], 4, 4, 64, 32, 0),
+    ([1500, 700], [40, 1], 2, 2, 128, 16, 400),
+    ([70], [70], 40, 1, 32, 16, 0),
+    ([30, 9], [1, 1], 40, 2, 64, 16, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_attention(shape, dtype):
+    lengths, news, heads, kv_heads, d, page, window = SHAPES[shape]
+    g = torch.Generator().manual_seed(shape)
+    pool, table = make_cache(g, lengths, kv_heads, d, page, extra_columns=shape % 3)
+    offsets = [0]
+    for n in news:
+        offsets.append(offsets[-1] + n)
+    wide = (2.0 * torch.randn((offsets[-1] + 2, heads * d + 24), generator=g)).to(dtype).to(DEV)
+    q = wide[:, 8:]
+    out = run_attention(q, heads, kv_heads, d, pool, table, offsets, lengths, window)
+    check_attention(out, q[:, :heads * d], heads, kv_heads, d, pool, table, offsets, lengths, page, window)
+    assert bool((out[offsets[-1]:] == 9).all()) and bool((out[:, heads * d:] == 9).all())
+
+
+def test_attention_of_one_key_is_its_value():
+    g = torch.Generator().manual_seed(3)
+    pool, table = make_cache(g, [1], 1, 64, 8)
+    q = torch.randn((1, 64), generator=g).to(DEV)
+    out = run_attention(q, 1, 1, 64, pool, table, [0, 1], [1], 0)
+    assert torch.equal(out.cpu().double(), plain.values_of_pages(pool)[1][table[0][0], 0, 0][None])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("news", [[1, 2], [40, 33]])
+def test_pages_that_are_not_there(news, dtype):
+    heads, kv_heads, d, page, lengths = 4, 2, 64, 8, [200, 90]
+    g = torch.Generator().manual_seed(11)
+    pool, table = make_cache(g, lengths, kv_heads, d, page)
+    table[0][0], table[0][7], table[0][11] = -1, pool.k_codes.shape[0], 2 ** 31 - 1
+    table[1] = [-5] * len(table[1])                    # nothing left
+    offsets = [0, news[0], sum(news)]
+    q = torch.randn((sum(news), heads * d), generator=g).to(dtype).to(DEV)
+    out = run_attention(q, heads, kv_heads, d, pool, table, offsets, lengths, 0)
+    check_attention(out, q, heads, kv_heads, d, pool, table, offsets, lengths, page, 0)
+    assert not out[news[0]:].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [32, 64, 128, 96])
+def test_groups_that_are_not_finite_reach_the_rows_that_see_them(d, dtype):
+    heads, kv_heads, page, lengths, news = 4, 2, 16, [70, 300], [30, 1]
+    g = torch.Generator().manual_seed(d)
+    pool, table = make_cache(g, lengths, kv_heads, d, page)
+    # a key at position 50 and a value at position 60 of request 0 (seen by some of its rows), a value at position 290 of request 1
+    pool.k_scales[table[0][3], 0, 2, 0] = 255
+    pool.v_scales[table[0][3], 1, 3, d // 32 - 1, 0] = 255
+    pool.v_scales[table[1][18], 0, 0, 0, 2] = 255
+    offsets = [0, 30, 31]
+    q = torch.randn((31, heads * d), generator=g).to(dtype).to(DEV)
+    for window in (0, 10):
+        out = run_attention(q, heads, kv_heads, d, pool, table, offsets, lengths, window)
+        got, _ = check_attention(out, q, heads, kv_heads, d, pool, table, offsets, lengths, page, window)
+        assert bool(torch.isnan(got).any()) and bool(torch.isfinite(got[:10]).all())
+
+
+@pytest.mark.parametrize("news", [1, 40])
+def test_queries_that_are_not_finite_stay_in_their_rows(news):
+    g = torch.Generator().manual_seed(2)
+    pool, table = make_cache(g, [90, 90], 2, 64, 16)
+    q = torch.randn((2 * news, 4 * 64), generator=g)
+    q[0, 70] = float("nan")
+    out = run_attention(q.to(DEV), 4, 2, 64, pool, table, [0, news, 2 * news], [90, 90], 0).cpu()
+    assert torch.isnan(out[0, 64:128]).all()
+    out[0, 64:128] = 0
+    assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_request_has_the_same_bits_beside_others(dtype):
+    heads, kv_heads, d, page = 8, 2, 128, 16
+    lengths, news = [700, 3000, 90, 5000], [1, 1, 40, 1]
+    g = torch.Generator().manual_seed(4)
+    pool, table = make_cache(g, lengths, kv_heads, d, page)
+    offsets = [0, 1, 2, 42, 43]
+    q = torch.randn((43, heads * d), generator=g).to(dtype).to(DEV)
+    together = run_attention(q, heads, kv_heads, d, pool, table, offsets, lengths, 0)
+    for i in range(4):
+        part = q[offsets[i]:offsets[i + 1]]
+        alone = run_attention(part, heads, kv_heads, d, pool, [table[i]], [0, news[i]], [lengths[i]], 0)
+        assert torch.equal(alone, together[offsets[i]:offsets[i + 1]]), i
+        again = run_attention(part, heads, kv_heads, d, pool, [table[i]], [0, news[i]], [lengths[i]], 0, most=news[i], longest=len(table[i]) * page)
+        assert torch.equal(again, alone), i
+
+
+def test_offsets_and_lengths_that_do_not_fit():
+    g = torch.Generator().manual_seed(6)
+    pool, table = make_cache(g, [40, 40, 40], 1, 32, 8)
+    q = torch.randn((6, 32), generator=g).to(DEV)
+    # requests 0 and 2 end beyond the rows or before they begin: their rows stay; request 1 says more keys than its table has
+    out = run_attention(q, 1, 1, 32, pool, table, [4, 1, 3, 90], [40, 1000, 40], 0, most=6, longest=40)
+    assert bool((out[0] == 9).all()) and bool((out[3:] == 9).all())
+    check_attention(out[1:3], q[1:3], 1, 1, 32, pool, [table[1]], [0, 2], [40], 8, 0)
+    # a length below the rows: those before the first key see nothing
+    out = run_attention(q[:5], 1, 1, 32, pool, table[:1], [0, 5], [2], 0)
+    assert not out[:3].any() and bool(out[3:].any())
+
+
+def test_pages_beyond_32_bits():
+    heads, d, page = 8, 128, 16
+    pages = 2 ** 32 // (heads * page * d // 2) + 40             # codes of more than 4 GiB
+    pool = Fp4Pages(*(torch.empty(s, dtype=torch.uint8, device=DEV) for s in Fp4Pages.shapes(pages, heads, page, d)))
+    ids = [pages - 1, 3, pages - 7, 0, pages // 2]
+    g = torch.Generator().manual_seed(8)
+    n = 5 * page - 3
+    k, v = (torch.randn((n, heads * d), generator=g).to(DEV) for _ in range(2))
+    slots = [ids[p // page] * page + p % page for p in range(n)]
+    kernels().fp4_write(k, v, i32(slots), pool)
+    q = torch.randn((1, heads * d), generator=g).to(DEV)
+    out = run_attention(q, heads, heads, d, pool, [ids], [0, 1], [n], 0)
+    few = Fp4Pages(*(t[torch.tensor(ids, device=DEV)].contiguous() for t in pool))
+    check_attention(out, q, heads, heads, d, few, [[0, 1, 2, 3, 4]], [0, 1], [n], page, 0)
+
+
+def test_attention_refusals():
+    k = kernels()
+    pool = Fp4Pages.empty(4, 2, 16, 64, device=DEV)
+    base = dict(q=torch.zeros((3, 256), device=DEV), nq=4, nkv=2, d=64, pages=pool, table=torch.zeros((2, 2), dtype=torch.int32, device=DEV),
+                offsets=i32([0, 1, 3]), lengths=i32([5, 7]), max_tokens=2, max_length=7, out=torch.zeros((3, 256), device=DEV), scale=0.1)
+    k.fp4_attention(**base)
+    for change in (dict(nq=5), dict(nkv=1), dict(d=32), dict(q=base["q"].half()), dict(out=base["out"].bfloat16()), dict(q=base["q"][:, :128]),
+                   dict(out=base["out"][:2]), dict(offsets=i32([0, 3])), dict(lengths=i32([5])), dict(max_length=33), dict(window=-1),
+                   dict(table=base["table"].long()), dict(table=base["table"][0]), dict(out=base["out"][:1].expand(3, 256)), dict(max_tokens=-1)):
+        with pytest.raises(KernelError):
+            k.fp4_attention(**{**base, **change})
+    torch.cuda.synchronize()
+
+
+# -- log probabilities ----------------------------------------------------------------------------------------------------
+def run_logprobs(logits, tokens, top):
+    n = logits.shape[0]
+    f = lambda *s: torch.full(s, 9.0, device=DEV)  # noqa: E731
+    i = lambda *s: torch.full(s, 9, dtype=torch.int32, device=DEV)  # noqa: E731
+    out = {"logprob": f(n), "entropy": f(n), "rank": i(n), "top_ids": i(n, top), "top_logprobs": f(n, top)}
+    kernels().token_logprobs(logits, i32(tokens), out["logprob"], out["entropy"], out["rank"], out["top_ids"], out["top_logprobs"])
+    return out
+
+
+def check_logprobs(logits, tokens, top):
+    got = {k: v.cpu() for k, v in run_logprobs(logits, tokens, top).items()}
+    want = plain.token_logprobs(logits, tokens, top)
+    assert got["rank"].tolist() == want["rank"]
+    assert got["top_ids"].tolist() == want["top_ids"]
+    # The sum of the weights: at most 160 additions one after the other for these rows (32 of a lane's piece, a stream's
+    # pieces, the lanes, the streams), each off by 2^-24, and weights within 2^-21; a logarithm's ulp; two subtractions.
+    # The entropy has the same sums over terms of up to log S + H.
+    sums = 160 * 2.0 ** -24 + 2.0 ** -21
+    scale = want["log_sum"].abs()
+    for name, bound in (("logprob", sums + 4 * 2.0 ** -24 * (want["logprob"].abs() + scale)),
+                        ("top_logprobs", sums + 4 * 2.0 ** -24 * (want["top_logprobs"].abs() + scale[:, None])),
+                        ("entropy", 2 * sums * (1 + scale + want["entropy"].abs()) + 4 * 2.0 ** -24 * scale)):
+        a, b = got[name].double(), want[name]
+        assert torch.equal(torch.isnan(a), torch.isnan(b)), name
+        same = (a == b) | torch.isnan(b)                    # infinities
+        assert bool((same | ((a - b).abs() <= bound)).all()), (name, (a - b).abs().nan_to_num().max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,top", [(1, 1, 0), (1, 1, 1), (3, 2, 2), (2, 63, 5), (5, 100, 32), (2, 513, 32), (4, 2047, 20),
+                                            (3, 2048, 1), (2, 2049, 32), (3, 4099, 7), (2, 50001, 20), (300, 700, 5), (260, 5003, 32),
+                                            (1, 151936, 20), (2, 300007, 32)])
+def test_logprobs(rows, vocab, top, dtype):
+    g = torch.Generator().manual_seed(rows * vocab)
+    wide = (2.5 * torch.randn((rows, vocab + 3), generator=g)).to(dtype).to(DEV)
+    logits = wide[:, 1:vocab + 1]
+    tokens = torch.randint(0, vocab, (rows,), generator=g).tolist()
+    check_logprobs(logits, tokens, top)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [11, 280])
+def test_logprobs_of_odd_rows(rows, dtype):
+    vocab, top = 3001, 20
+    g = torch.Generator().manual_seed(rows)
+    x = (2.5 * torch.randn((rows, vocab), generator=g)).to(dtype)
+    inf = float("inf")
+    tokens = torch.randint(0, vocab, (rows,), generator=g).tolist()
+    x[0] = 1.5                                     # all equal
+    x[1] = -inf; x[1, [5, 2500, 700]] = torch.tensor([1.0, 3.0, 1.0]).to(dtype); tokens[1] = 700       # masked but for three
+    x[2] = -inf                                    # nothing left
+    x[3, 40] = float("nan"); tokens[3] = 41        # a NaN
+    x[4, 2999] = inf; tokens[4] = 2999             # an infinity
+    x[5] = torch.arange(vocab).to(dtype); tokens[5] = 0               # ascending (with ties in bfloat16)
+    x[6] = -torch.arange(vocab).to(dtype); tokens[6] = 2500
+    x[7, ::2] = -inf; tokens[7] = 2                # half masked, the token too
+    x[8] = 0.0; x[8, 1::2] = -0.0; tokens[8] = 3   # zeros of both signs are equal
+    x[9, 30] = float("nan"); x[9, 35] = float("nan"); x[9, 2000] = float("nan"); tokens[9] = 35
+    x[10, 17] = 3e38; tokens[10] = 18              # one large logit
+    check_logprobs(x.to(DEV), tokens, top)
+    check_logprobs(x.to(DEV)[:, :40], [t % 40 for t in tokens], 32)
+
+
+def test_tokens_outside_the_vocabulary():
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn((4, 50), generator=g).to(DEV)
+    check_logprobs(x, [-1, 50, 49, 2 ** 31 - 1], 3)
+
+
+def test_a_row_has_the_same_bits_beside_others():
+    g = torch.Generator().manual_seed(12)
+    for dtype in (torch.float32, torch.bfloat16):
+        x = (2.5 * torch.randn((600, 20011), generator=g)).to(dtype).to(DEV)
+        tokens = torch.randint(0, 20011, (600,), generator=g).tolist()
+        many = run_logprobs(x, tokens, 5)
+        for lo, hi in ((0, 1), (5, 22), (599, 600)):
+            few = run_logprobs(x[lo:hi], tokens[lo:hi], 5)
+            for name in few:
+                assert torch.equal(few[name], many[name][lo:hi]), name
+
+
+def test_logprobs_refusals():
+    k = kernels()
+    f, i = (lambda *s: torch.zeros(s, device=DEV)), (lambda *s: torch.zeros(s, dtype=torch.int32, device=DEV))
+    base = dict(logits=f(3, 40), tokens=i(3), logprob=f(3), entropy=f(3), rank=i(3), top_ids=i(3, 2), top_logprobs=f(3, 2))
+    k.token_logprobs(**base)
+    for change in (dict(logits=f(3, 40).half()), dict(logits=f(40, 3).t()), dict(tokens=i(2)), dict(tokens=i(3).long()), dict(logprob=f(4)),
+                   dict(entropy=i(3)), dict(rank=f(3)), dict(top_ids=i(3, 3)), dict(top_ids=i(3, 33), top_logprobs=f(3, 33)),
+                   dict(logits=f(3, 1)), dict(logits=torch.empty((3, 0), device=DEV), top_ids=i(3, 0), top_logprobs=f(3, 0)),
+                   dict(logits=torch.empty((3, 524289), device=DEV))):
+        with pytest.raises(KernelError):
+            k.token_logprobs(**{**base, **change})
+    k.token_logprobs(f(0, 40), i(0), f(0), f(0), i(0), i(0, 2), f(0, 2))
+    torch.cuda.synchronize()
+
+
+# -- together ---------------------------------------------------------------------------------------------------------------
+class Serving:
+    """A small decoder's serving state: a linear model of keys, values, queries and logits from token ids."""
+
+    def __init__(self, requests, dtype, seed):
+        g = torch.Generator().manual_seed(seed)
+        self.dtype, self.page, self.columns = dtype, 8, 12
+        self.heads, self.kv_heads, self.d, self.vocab = 4, 2, 64, 500
+        make = lambda *s: torch.randn(s, generator=g).to(dtype).to(DEV)  # noqa: E731
+        self.keys, self.values = make(self.vocab, 128), make(self.vocab, 128)
+        self.queries, self.head = make(self.vocab, 256), make(self.vocab, 256) * 0.2
+        self.pool = Fp4Pages.empty(requests * self.columns, self.kv_heads, self.page, self.d, device=DEV)
+        self.table = torch.full((requests, self.columns), -1, dtype=torch.int32, device=DEV)
+        self.free = torch.randperm(requests * self.columns, generator=g).to(torch.int32).to(DEV)
+        self.lengths = torch.zeros(requests, dtype=torch.int32, device=DEV)
+        self.cursor = i32([0])
+        self.requests = requests
+
+    def buffers(self, rows):
+        i = lambda *s: torch.zeros(s, dtype=torch.int32, device=DEV)  # noqa: E731
+        f = lambda *s: torch.zeros(s, device=DEV)  # noqa: E731
+        return dict(slots=i(rows), tok_seq=i(rows), tok_pos=i(rows), offsets=i(self.requests + 1), new_lengths=i(self.requests),
+                    progress=i(2), out=torch.zeros((rows, 256), dtype=self.dtype, device=DEV), logprob=f(rows), entropy=f(rows),
+                    rank=i(rows), top_ids=i(rows, 3), top_logprobs=f(rows, 3))
+
+    def step(self, tokens, news, most, b):
+        k = kernels()
+        k.step_tables(self.lengths, news, self.table, self.page, self.free, self.cursor, b["slots"], b["tok_seq"], b["tok_pos"],
+                      b["offsets"], b["new_lengths"], b["progress"])
+        ids = tokens.long()
+        k.fp4_write(self.keys[ids], self.values[ids], b["slots"], self.pool)
+        k.fp4_attention(self.queries[ids], self.heads, self.kv_heads, self.d, self.pool, self.table, b["offsets"], b["new_lengths"],
+                        most, self.columns * self.page, b["out"], self.d ** -0.5)
+        logits = torch.mm(b["out"].float(), self.head.float().t())
+        k.token_logprobs(logits, tokens, b["logprob"], b["entropy"], b["rank"], b["top_ids"], b["top_logprobs"])
+        self.lengths.copy_(b["new_lengths"])
+        self.cursor.copy_(b["progress"][:1])
+        return b["top_ids"][:, 0]
+
+
+def serve(dtype, graph, stream=None):
+    s = Serving(3, dtype, 7)
+    g = torch.Generator().manual_seed(1)
+    news = i32([5, 1, 30])
+    tokens = torch.randint(0, s.vocab, (36,), generator=g).to(torch.int32).to(DEV)
+    history = []
+    prompt = s.buffers(36)
+    picked = s.step(tokens, news, 30, prompt)
+    history.append({k: v.clone() for k, v in prompt.items()})
+    ends = prompt["offsets"][1:].long() - 1
+    feed = picked[ends].clone()
+    ones = i32([1, 1, 1])
+    b = s.buffers(3)
+    if graph:
+        saved = [t.clone() for t in (s.lengths, s.cursor, s.table, *s.pool, feed)]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            feed.copy_(s.step(feed, ones, 1, b))
+        torch.cuda.current_stream().wait_stream(side)
+        for t, old in zip((s.lengths, s.cursor, s.table, *s.pool, feed), saved):
+            t.copy_(old)
+        captured = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(captured):
+            feed.copy_(s.step(feed, ones, 1, b))
+    for _ in range(9):
+        if graph:
+            captured.replay()
+            (torch.ones(1000, device=DEV) * 2).sum().item()     # the program's own work in between
+        else:
+            feed.copy_(s.step(feed, ones, 1, b))
+        history.append({k: v.clone() for k, v in b.items()})
+    history.append({"table": s.table.clone(), "lengths": s.lengths.clone(), **{f"pool{i}": t.clone() for i, t in enumerate(s.pool)}})
+    return history
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_run_of_them_together_eager_captured_and_on_two_streams(dtype):
+    eager = serve(dtype, False)
+    assert eager[-1]["lengths"].tolist() == [14, 10, 39] and eager[-2]["progress"].tolist() == [9, 0]
+    replayed = serve(dtype, True)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    others = []
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            others.append(serve(dtype, False))
+    torch.cuda.synchronize()
+    for other in (replayed, *others):
+        for a, b in zip(eager, other):
+            for name in a:
+                assert torch.equal(a[name], b[name]), name
+    # and the last step against the plain implementations
+    s = Serving(3, dtype, 7)
+    pool = [eager[-1][f"pool{i}"] for i in range(4)]
+    keys, values = plain.values_of_pages(pool)
+    feed = eager[-3]["top_ids"][:, 0].long()
+    last = eager[-2]
+    want, spread, reach = plain.attention(s.queries[feed], 4, 2, 64, keys, values, eager[-1]["table"].tolist(), [0, 1, 2, 3],
+                                          last["new_lengths"].tolist(), 8, 0.125, 0)
+    bound = 2 * spread * (68 * 2.0 ** -24 * reach + 2.0 ** -21) + spread * (U[torch.bfloat16] + 2.0 ** -16) + U[dtype] * want.abs() + 1e-30
+    assert bool(((last["out"].double().cpu() - want).abs() <= bound).all())
