@@ -52,8 +52,17 @@ constexpr float kSlack = 8.f;  // how far a score may pass the reference, in pow
 constexpr float kToLog2 = 1.4426950408889634f;
 
 template <typename T> constexpr int kTerms = std::is_same_v<T, float> ? 3 : 1;
+#ifndef LS_FP4_PROMPT_TILES
+#define LS_FP4_PROMPT_TILES 2
+#endif
 // Row tiles a wave holds where every wave has rows of its own: what its registers allow.
-template <typename T> constexpr int kPromptTiles = std::is_same_v<T, float> ? (D <= 64 ? 2 : 1) : (D <= 64 ? 4 : D <= 128 ? 2 : 1);
+template <typename T> constexpr int kPromptTiles = std::is_same_v<T, float> ? 1 : (D <= 128 ? LS_FP4_PROMPT_TILES : 1);
+
+// Waves a SIMD of the prompt kernel.
+#ifndef LS_FP4_PROMPT_WAVES
+#define LS_FP4_PROMPT_WAVES 2
+#endif
+template <typename T> constexpr int kPromptWaves = D <= 128 ? LS_FP4_PROMPT_WAVES : 1;
 
 // Keys a split of a request of few rows covers, by how many keys its rows see.
 __host__ __device__ inline int decode_split(int span) {
@@ -64,7 +73,7 @@ __host__ __device__ inline int decode_split(int span) {
 constexpr int kPromptBlocks = 32;  // row blocks times splits that a request's head is cut into, about
 __host__ __device__ inline int prompt_split(int span, int blocks) {
   const int want = max(1, kPromptBlocks / max(1, blocks));
-  return max(512, ((span + want - 1) / want + kTileKeys - 1) / kTileKeys * kTileKeys);
+  return max(512, ((span + want - 1) / want + 63) / 64 * 64);  // whole tiles of 64
 }
 
 struct Fp4Args {
@@ -79,7 +88,8 @@ struct Fp4Args {
   const int* lengths;
   int requests, rows;      // rows: of q and out
   int group;               // query heads a key/value head
-  float factor;            // scale * log2(e)
+  float factor;            // |scale| * log2(e)
+  bool negative;           // the scale is: queries change their sign
   int window;
   float* part_acc;         // [requests * kv heads][region][D]
   float* part_ml;          // [requests * kv heads][region][2]
@@ -199,15 +209,16 @@ struct Rows {
           if (there) {
             if constexpr (sizeof(T) == 2) {
               typedef unsigned int any4 __attribute__((ext_vector_type(4), aligned(2)));
-              const any4 w = *reinterpret_cast<const any4*>(p);
+              any4 w = *reinterpret_cast<const any4*>(p);
+              if (a.negative) w ^= any4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
               q[0][t][dim / 32 + i] = as_operand(w[0], w[1], w[2], w[3]);
             } else {
               typedef float any4 __attribute__((ext_vector_type(4), aligned(4)));
               const any4 u = *reinterpret_cast<const any4*>(p), w = *reinterpret_cast<const any4*>(reinterpret_cast<const float*>(p) + 4);
 #pragma unroll
               for (int y = 0; y < 4; ++y) {
-                x[y] = u[y];
-                x[4 + y] = w[y];
+                x[y] = a.negative ? -u[y] : u[y];
+                x[4 + y] = a.negative ? -w[y] : w[y];
               }
             }
           } else {
@@ -241,6 +252,37 @@ struct Rows {
       any_last = rq.start + (row_end - 1) / a.group;
       any_low = a.window > 0 ? max(0, all_last - a.window + 1) : 0;
       all_low = a.window > 0 ? max(0, any_last - a.window + 1) : 0;
+    }
+  }
+
+  // The weights of 8 scores of row tile t (before their factor), and what they add to the sums.
+  __device__ __forceinline__ void weigh(const Fp4Args& a, int t, const float (&x)[8], bf16x8 (&p)[kTerms<T>][NT]) {
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
+    top = top * a.factor;
+    if (__ballot(top > m[t] + kSlack) != 0ull) {  // (-inf + 8 is -inf: any score moves the first reference)
+      const float next = fmaxf(m[t], quad16_max(top));
+      const float f = m[t] == -INFINITY ? 0.f : weight_exp2<T>(m[t] - next);
+      m[t] = next;
+      l[t] = l[t] * f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) acc[t][i][y] = acc[t][i][y] * f;
+    }
+    const float ref = m[t] == -INFINITY ? 0.f : m[t];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float w = weight_exp2<T>(fmaf(x[i], a.factor, -ref));
+      l[t] = l[t] + w;
+      float rest = w;
+#pragma unroll
+      for (int term = 0; term < kTerms<T>; ++term) {
+        const bf16_t part = static_cast<bf16_t>(rest);
+        p[term][t][i] = part;
+        if constexpr (kTerms<T> > 1) rest = rest - static_cast<float>(part);
+      }
     }
   }
 
@@ -307,13 +349,12 @@ struct Rows {
               sc[t][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[term][t][base + i], sc[t][s], 0, 0, 0);
         }
       }
-    // the weights
     bf16x8 p[kTerms<T>][NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = sc[t][i >> 2][i & 3] * a.factor;
+      for (int i = 0; i < 8; ++i) x[i] = sc[t][i >> 2][i & 3];
       if (bad_keys) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -327,32 +368,7 @@ struct Rows {
           x[i] = seen ? x[i] : -INFINITY;
         }
       }
-      float top = x[0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
-      if (__ballot(top > m[t] + kSlack) != 0ull) {  // (-inf + 8 is -inf: any score moves the first reference)
-        const float next = fmaxf(m[t], quad16_max(top));
-        const float f = m[t] == -INFINITY ? 0.f : weight_exp2<T>(m[t] - next);
-        m[t] = next;
-        l[t] = l[t] * f;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-          for (int y = 0; y < 4; ++y) acc[t][i][y] = acc[t][i][y] * f;
-      }
-      const float ref = m[t] == -INFINITY ? 0.f : m[t];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float w = weight_exp2<T>(x[i] - ref);
-        l[t] = l[t] + w;
-        float rest = w;
-#pragma unroll
-        for (int term = 0; term < kTerms<T>; ++term) {
-          const bf16_t part = static_cast<bf16_t>(rest);
-          p[term][t][i] = part;
-          if constexpr (kTerms<T> > 1) rest = rest - static_cast<float>(part);
-        }
-      }
+      weigh(a, t, x, p);
     }
     // O^T += V^T P^T
 #pragma unroll
@@ -549,26 +565,284 @@ __global__ __launch_bounds__(kThreads, (std::is_same_v<T, float> && D > 160 ? 1 
   }
 }
 
-// Prompts: grid (groups of four row blocks, kv heads * splits, requests); a wave a row block.
+// Prompts: a workgroup's four waves share the tiles of 64 keys, as operands in LDS.  Wave w makes the operands of the
+// keys 16 w .. 16 w + 15, and of half of the values of the 32 keys from 32 (w / 2) on; an operand is 1 KiB, 16 bytes a lane,
+// written and read in one piece.  Two buffers: while one is read, the codes of the next tile are on their way to registers.
+constexpr int kSharedKeys = 64;
+constexpr int kOperands = 4 * (D / 32) + 2 * (D / 16);  // operands of a tile: keys, then values
+struct SharedFlags {  // what is out of the ordinary in a tile (rare); `any` says whether there is something
+  unsigned int any[4], k_nan[4], k_bad[4];
+  unsigned long long v_nan[2][kSections][2][4];  // by half of the tile, section, 16 keys, place in a block: a bit a lane
+};
+
+struct Staged {  // the codes a wave turns into operands
+  unsigned int k[D / 32], ks[kSections];
+  unsigned int v[2][kSections][4], vs[2][kSections];
+  bool k_ok, v_ok[2];
+};
+struct StagedIds {
+  int k, v[2];
+};
+
+__device__ __forceinline__ StagedIds staged_ids(const Fp4Args& a, const int* __restrict__ row, int t0, int lane, int w) {
+  StagedIds ids;
+  ids.k = row[min((t0 + 16 * w + (lane & 15)) >> a.pool.page_shift, a.columns - 1)];
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+    ids.v[s] = row[min((t0 + 32 * (w >> 1) + 16 * s + 4 * (lane >> 4)) >> a.pool.page_shift, a.columns - 1)];
+  return ids;
+}
+
+__device__ __forceinline__ void stage_tile(Staged& st, const Fp4Args& a, const StagedIds& ids, int head, int t0, int lane, int w) {
+  const int n = lane & 15, j = lane >> 4, mask = (1 << a.pool.page_shift) - 1;
+  st.k_ok = ids.k >= 0 && ids.k < a.pool.pages;
+  const long k_row = (((long)(st.k_ok ? ids.k : 0) * a.pool.kv_heads + head) << a.pool.page_shift) + ((t0 + 16 * w + n) & mask);
+  const unsigned char* kc = a.pool.k_codes + k_row * (D / 2);
+  const unsigned char* ks = a.pool.k_scales + k_row * (D / 32);
+#pragma unroll
+  for (int c = 0; c < kSections; ++c) {
+    const int e = section_elems(c), dim = section_dim(c);
+    load_words(&st.k[dim / 32], kc + dim / 2 + j * 2 * e, e / 2);
+    st.ks[c] = ks[(dim + j * 4 * e) / 32];
+  }
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    st.v_ok[s] = ids.v[s] >= 0 && ids.v[s] < a.pool.pages;
+    const long v_blk = ((((long)(st.v_ok[s] ? ids.v[s] : 0) * a.pool.kv_heads + head) << a.pool.page_shift) +
+                        ((t0 + 32 * (w >> 1) + 16 * s + 4 * j) & mask)) >> 2;
+    const unsigned char* vc = a.pool.v_codes + v_blk * (2 * D);
+    const unsigned char* vs = a.pool.v_scales + v_blk * (D / 8);
+#pragma unroll
+    for (int c = 0; c < kSections; ++c) {
+      const int e = section_elems(c), dim = section_dim(c);
+      load_words(st.v[s][c], vc + (dim + n * e) / 8 * 16, 4);
+      load_words(&st.vs[s][c], vs + (dim + n * e) / 32 * 4, 1);
+    }
+  }
+}
+
+// Codes to operands.  Keys that no row of the workgroup sees (outside low .. last) are zeros.
+__device__ __forceinline__ void share_tile(Staged& st, bf16x8* __restrict__ operands, SharedFlags& flags, int t0, int low, int last,
+                                           int lane, int w) {
+  const int n = lane & 15, j = lane >> 4;
+  bool k_nan = false, v_nan = false;
+#pragma unroll
+  for (int c = 0; c < kSections; ++c) k_nan = k_nan || st.ks[c] == kFp4Nan;
+  const int v0 = t0 + 32 * (w >> 1);
+  if (v0 < low || v0 + 31 > last || __ballot(!(st.v_ok[0] && st.v_ok[1])) != 0ull) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int key = v0 + 16 * s + 4 * j + y;
+        const bool seen = st.v_ok[s] && key >= low && key <= last;
+#pragma unroll
+        for (int c = 0; c < kSections; ++c) {
+          st.v[s][c][y] = seen ? st.v[s][c][y] : 0u;
+          st.vs[s][c] = seen ? st.vs[s][c] : ((st.vs[s][c] & ~(255u << (8 * y))) | (127u << (8 * y)));
+        }
+      }
+  }
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int c = 0; c < kSections; ++c) {
+      const unsigned int b = st.vs[s][c];
+      v_nan = v_nan || (((b & 0x7f7f7f7fu) + 0x01010101u) & b & 0x80808080u) != 0u;
+    }
+  const bool odd = __ballot(k_nan || v_nan || !st.k_ok) != 0ull;
+  if (lane == 0) flags.any[w] = odd ? 1u : 0u;
+  if (odd) {
+    const unsigned long long nan = __ballot(k_nan), bad = __ballot(!st.k_ok);
+    const unsigned int f = (unsigned int)(nan | (nan >> 32)), g = (unsigned int)(bad | (bad >> 32));
+    if (lane == 0) {
+      flags.k_nan[w] = (f | (f >> 16)) & 0xffffu;
+      flags.k_bad[w] = (g | (g >> 16)) & 0xffffu;
+    }
+#pragma unroll
+    for (int c = 0; c < kSections; ++c)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const bool here = ((st.vs[s][c] >> (8 * y)) & 255u) == kFp4Nan;
+          const unsigned long long b = __ballot(here);
+          if (lane == 0 && (w & 1) == 0) flags.v_nan[w >> 1][c][s][y] = b;
+          if (here) {
+            st.v[s][c][y] = 0u;
+            st.vs[s][c] = (st.vs[s][c] & ~(255u << (8 * y))) | (127u << (8 * y));
+          }
+        }
+  }
+#pragma unroll
+  for (int c = 0; c < kSections; ++c) {
+    const float scale = fp4_scale(st.ks[c]);
+    const int base = section_dim(c) / 32;
+#pragma unroll
+    for (int i = 0; i < section_elems(c) / 2; ++i) {
+      const unsigned int x = st.k[base + i];
+      operands[(w * (D / 32) + base + i) * 64 + lane] =
+          as_operand(fp4_pair<0>(x, scale), fp4_pair<1>(x, scale), fp4_pair<2>(x, scale), fp4_pair<3>(x, scale));
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kSections; ++c) {
+    const int e = section_elems(c), at = section_dim(c) / 16;
+    const int mine = max(1, e / 4);              // pairs a wave makes of the section's e / 2
+    if (e == 2 && (w & 1)) continue;             // (uniform) a section of one pair: one of the two waves makes it
+    const int from = e == 2 ? 0 : mine * (w & 1);  // (uniform)
+    float scale[2][4];
+    unsigned int x[2][4];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        scale[s][y] = fp4_scale((st.vs[s][c] >> (8 * y)) & 255u);
+        const int place = e == 8 ? 0 : e == 4 ? 16 * (n & 1) : 8 * (n & 3);
+        x[s][y] = st.v[s][c][y] >> (place + 8 * from);
+      }
+#pragma unroll
+    for (int pair = 0; pair < mine; ++pair) {
+      unsigned int both[2][4];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) both[s][y] = pair == 0 ? fp4_pair<0>(x[s][y], scale[s][y]) : fp4_pair<1>(x[s][y], scale[s][y]);
+      bf16x8* to = operands + (4 * (D / 32) + (w >> 1) * (D / 16) + at + 2 * (from + pair)) * 64 + lane;
+      to[0] = as_operand(__builtin_amdgcn_perm(both[0][1], both[0][0], 0x05040100u), __builtin_amdgcn_perm(both[0][3], both[0][2], 0x05040100u),
+                         __builtin_amdgcn_perm(both[1][1], both[1][0], 0x05040100u), __builtin_amdgcn_perm(both[1][3], both[1][2], 0x05040100u));
+      to[64] = as_operand(__builtin_amdgcn_perm(both[0][1], both[0][0], 0x07060302u), __builtin_amdgcn_perm(both[0][3], both[0][2], 0x07060302u),
+                          __builtin_amdgcn_perm(both[1][1], both[1][0], 0x07060302u), __builtin_amdgcn_perm(both[1][3], both[1][2], 0x07060302u));
+    }
+  }
+}
+
+// 32 keys from t0 on (half u of a shared tile).
+template <typename T, int NT>
+__device__ __forceinline__ void step_shared(Rows<T, NT>& rows, const Fp4Args& a, const bf16x8* __restrict__ operands, const SharedFlags& flags,
+                                            bool odd, int u, int t0, int lane) {
+  const int j = lane >> 4;
+  const bool whole = t0 >= rows.all_low && t0 + kTileKeys - 1 <= rows.all_last;
+  f32x4 sc[NT][2];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const bf16x8 k = operands[((2 * u + s) * (D / 32) + i) * 64 + lane];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int term = kTerms<T> - 1; term >= 0; --term)
+          sc[t][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, rows.q[term][t][i], sc[t][s], 0, 0, 0);
+    }
+  bf16x8 p[kTerms<T>][NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = sc[t][i >> 2][i & 3];
+    if (odd) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int w = 2 * u + (i >> 2), bit = 4 * j + (i & 3);
+        if (flags.any[w] && ((flags.k_nan[w] >> bit) & 1u)) x[i] = __uint_as_float(0x7fc00000u);
+        if (flags.any[w] && ((flags.k_bad[w] >> bit) & 1u)) x[i] = -INFINITY;
+      }
+    }
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int key = t0 + 16 * (i >> 2) + 4 * j + (i & 3);
+        x[i] = key >= rows.low[t] && key <= rows.last[t] ? x[i] : -INFINITY;
+      }
+    }
+    rows.weigh(a, t, x, p);
+  }
+  if (odd && flags.any[2 * u]) {  // values that are not finite (the keys' bad pages are no matter: those values are zeros)
+    for (int s = 0; s < 2; ++s)
+      for (int y = 0; y < 4; ++y)
+        for (int block = 0; block < 4; ++block) {
+          const int key = t0 + 16 * s + 4 * block + y;
+#pragma unroll
+          for (int c = 0; c < kSections; ++c)
+            if ((flags.v_nan[u][c][s][y] >> (4 * j + 16 * block)) & 1ull) {
+#pragma unroll
+              for (int t = 0; t < NT; ++t)
+                if (key >= rows.low[t] && key <= rows.last[t]) {
+#pragma unroll
+                  for (int i = 0; i < section_elems(c); ++i)
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) rows.acc[t][section_dim(c) / 16 + i][z] = __uint_as_float(0x7fc00000u);
+                }
+            }
+        }
+  }
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    const bf16x8 v = operands[(4 * (D / 32) + u * (D / 16) + i) * 64 + lane];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int term = kTerms<T> - 1; term >= 0; --term)
+        rows.acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[term][t], rows.acc[t][i], 0, 0, 0);
+  }
+}
+
+// Grid (row blocks of a workgroup, kv heads * splits, requests).
 template <typename T>
-__global__ __launch_bounds__(kThreads, 1) void fp4_prompt_kernel(Fp4Args a) {
+__global__ __launch_bounds__(kThreads, kPromptWaves<T>) void fp4_prompt_kernel(Fp4Args a) {
   constexpr int NT = kPromptTiles<T>, kBlock = 16 * NT;
+  __shared__ bf16x8 operands[2][kOperands * 64];
+  __shared__ SharedFlags flags[2];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int head = blockIdx.y % a.pool.kv_heads, split = blockIdx.y / a.pool.kv_heads, b = blockIdx.z;
   const Request rq(a, b);
   if (rq.rows <= a.few) return;
   const int blocks = (rq.rows + kBlock - 1) / kBlock;
-  const int block = 4 * (gridDim.x - 1 - blockIdx.x) + w;  // the blocks that see most keys first
-  if (block >= blocks) return;
+  const int group = gridDim.x - 1 - blockIdx.x;  // the blocks that see most keys first
+  if (4 * group >= blocks) return;
   const int span = rq.end - rq.base, len = prompt_split(span, blocks);
   const int splits = max(1, (span + len - 1) / len);
   if (split >= splits) return;
-  const int row0 = block * kBlock;
+  const int row0 = (4 * group + w) * kBlock;
   Rows<T, NT> rows;
   rows.init(a, rq, head, row0, lane);
-  const int begin = max(rq.base + split * len, rows.any_low & ~(kTileKeys - 1));
-  const int end = min(min(rq.end, rq.base + (split + 1) * len), rows.any_last + 1);
-  walk_keys<T, NT>(rows, a, a.table + (long)b * a.columns, head, begin, end, kTileKeys, lane);
+  // the keys that the workgroup's rows see
+  const int first_token = 4 * group * kBlock / a.group, last_token = (min((4 * group + 4) * kBlock, rq.rows) - 1) / a.group;
+  const int low = a.window > 0 ? max(0, rq.start + first_token - a.window + 1) : 0, last = rq.start + last_token;
+  const int split_begin = rq.base + split * len;
+  const int begin = low > split_begin ? split_begin + (low - split_begin) / kSharedKeys * kSharedKeys : split_begin;
+  const int end = min(min(rq.end, split_begin + len), last + 1);
+  const int* row = a.table + (long)b * a.columns;
+  if (begin < end) {  // (uniform)
+    Staged st;
+    StagedIds ids = staged_ids(a, row, begin, lane, w);
+    stage_tile(st, a, ids, head, begin, lane, w);
+    ids = staged_ids(a, row, begin + kSharedKeys < end ? begin + kSharedKeys : begin, lane, w);
+    share_tile(st, operands[0], flags[0], begin, low, last, lane, w);
+    __syncthreads();
+    int buffer = 0;
+    for (int t0 = begin; t0 < end; t0 += kSharedKeys, buffer ^= 1) {
+      const int t1 = t0 + kSharedKeys;
+      const bool more = t1 < end;  // (uniform)
+      if (more) {
+        stage_tile(st, a, ids, head, t1, lane, w);
+        ids = staged_ids(a, row, t1 + kSharedKeys < end ? t1 + kSharedKeys : t1, lane, w);
+      }
+      const SharedFlags& f = flags[buffer];
+      const bool odd = __builtin_amdgcn_readfirstlane(f.any[0] | f.any[1] | f.any[2] | f.any[3]) != 0;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int key = t0 + kTileKeys * u;
+        if (key <= rows.any_last && key + kTileKeys > rows.any_low)  // (uniform in the wave)
+          step_shared<T, NT>(rows, a, operands[buffer], f, odd, u, key, lane);
+      }
+      if (more) share_tile(st, operands[buffer ^ 1], flags[buffer ^ 1], t1, low, last, lane, w);
+      __syncthreads();
+    }
+  }
   const int n = lane & 15, j = lane >> 4;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -747,7 +1021,9 @@ extern "C" int ls_fp4_attention(int dtype, const void* q, long ldq, void* out, l
                    static_cast<const unsigned char*>(v_codes), static_cast<const unsigned char*>(v_scales), pages,
                    __builtin_ctz((unsigned)page_size), kv_heads};
   a.table = table; a.columns = columns; a.offsets = offsets; a.lengths = lengths; a.requests = requests; a.rows = rows;
-  a.group = group; a.factor = scale * kToLog2; a.window = window;
+  a.group = group; a.window = window;
+  a.factor = fmaxf(fabsf(scale) * kToLog2, 1.1754944e-38f);  // (never 0: a masked score stays -inf times it)
+  a.negative = scale < 0.f;
   return dtype == kF32 ? run_fp4<float>(a, most, longest, scratch, scratch_bytes, (hipStream_t)stream)
                        : run_fp4<bf16_t>(a, most, longest, scratch, scratch_bytes, (hipStream_t)stream);
 }

@@ -71,7 +71,7 @@ def test_the_plan_of_the_splits_covers_every_request():
 
     def prompt_split(span, blocks):
         want = max(1, 32 // max(1, blocks))
-        return max(512, ((span + want - 1) // want + 31) // 32 * 32)
+        return max(512, ((span + want - 1) // want + 63) // 64 * 64)
 
     def planned(span):
         return max([1] + [-(-s // decode_split(s)) for s in (span, min(span, 4096), min(span, 32768), min(span, 131072)) if s])
