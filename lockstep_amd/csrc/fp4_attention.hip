@@ -47,6 +47,7 @@ __host__ __device__ constexpr int section_dim(int s) {
 }
 
 constexpr int kTileKeys = 32;
+constexpr int kSharedKeys = 64;  // where a workgroup shares the tiles
 constexpr int kThreads = 256;
 constexpr float kSlack = 8.f;  // how far a score may pass the reference, in powers of two
 constexpr float kToLog2 = 1.4426950408889634f;
@@ -109,7 +110,7 @@ struct Request {
     const int room = (int)min((long)a.columns << a.pool.page_shift, 0x7fffffffl);
     end = min(max(a.lengths[b], 0), room);
     start = end - n;
-    base = a.window > 0 ? max(0, start - a.window + 1) & ~(kTileKeys - 1) : 0;
+    base = a.window > 0 ? max(0, start - a.window + 1) & ~(kSharedKeys - 1) : 0;
   }
 };
 
@@ -255,33 +256,46 @@ struct Rows {
     }
   }
 
-  // The weights of 8 scores of row tile t (before their factor), and what they add to the sums.
-  __device__ __forceinline__ void weigh(const Fp4Args& a, int t, const float (&x)[8], bf16x8 (&p)[kTerms<T>][NT]) {
-    float top = x[0];
+  // The weights of the lane's scores (before their factor) of every row tile, and what they add to the sums.
+  template <int H>
+  __device__ __forceinline__ void weigh(const Fp4Args& a, const float (&x)[NT][8 * H], bf16x8 (&p)[kTerms<T>][NT][H]) {
+    float top[NT];
+    bool far = false;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
-    top = top * a.factor;
-    if (__ballot(top > m[t] + kSlack) != 0ull) {  // (-inf + 8 is -inf: any score moves the first reference)
-      const float next = fmaxf(m[t], quad16_max(top));
-      const float f = m[t] == -INFINITY ? 0.f : weight_exp2<T>(m[t] - next);
-      m[t] = next;
-      l[t] = l[t] * f;
+    for (int t = 0; t < NT; ++t) {
+      top[t] = x[t][0];
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-        for (int y = 0; y < 4; ++y) acc[t][i][y] = acc[t][i][y] * f;
+      for (int i = 1; i < 8 * H; ++i) top[t] = fmaxf(top[t], x[t][i]);
+      top[t] = top[t] * a.factor;
+      far = far || top[t] > m[t] + kSlack;  // (-inf + 8 is -inf: any score moves the first reference)
     }
-    const float ref = m[t] == -INFINITY ? 0.f : m[t];
+    if (__ballot(far) != 0ull) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float w = weight_exp2<T>(fmaf(x[i], a.factor, -ref));
-      l[t] = l[t] + w;
-      float rest = w;
+      for (int t = 0; t < NT; ++t) {
+        const float next = fmaxf(m[t], quad16_max(top[t]));
+        const float f = m[t] == -INFINITY ? 0.f : weight_exp2<T>(m[t] - next);
+        m[t] = next;
+        l[t] = l[t] * f;
 #pragma unroll
-      for (int term = 0; term < kTerms<T>; ++term) {
-        const bf16_t part = static_cast<bf16_t>(rest);
-        p[term][t][i] = part;
-        if constexpr (kTerms<T> > 1) rest = rest - static_cast<float>(part);
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) acc[t][i][y] = acc[t][i][y] * f;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const float ref = m[t] == -INFINITY ? 0.f : m[t];
+#pragma unroll
+      for (int i = 0; i < 8 * H; ++i) {
+        const float w = weight_exp2<T>(fmaf(x[t][i], a.factor, -ref));
+        l[t] = l[t] + w;
+        float rest = w;
+#pragma unroll
+        for (int term = 0; term < kTerms<T>; ++term) {
+          const bf16_t part = static_cast<bf16_t>(rest);
+          p[term][t][i / 8][i % 8] = part;
+          if constexpr (kTerms<T> > 1) rest = rest - static_cast<float>(part);
+        }
       }
     }
   }
@@ -349,27 +363,27 @@ struct Rows {
               sc[t][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[term][t][base + i], sc[t][s], 0, 0, 0);
         }
       }
-    bf16x8 p[kTerms<T>][NT];
+    bf16x8 p[kTerms<T>][NT][1];
+    float x[NT][8];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = sc[t][i >> 2][i & 3];
+      for (int i = 0; i < 8; ++i) x[t][i] = sc[t][i >> 2][i & 3];
       if (bad_keys) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if ((nan_keys >> (16 * (i >> 2) + 4 * j + (i & 3))) & 1u) x[i] = __uint_as_float(0x7fc00000u);
+          x[t][i] = ((nan_keys >> (16 * (i >> 2) + 4 * j + (i & 3))) & 1u) ? __uint_as_float(0x7fc00000u) : x[t][i];
       }
       if (!whole) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int key = t0 + 16 * (i >> 2) + 4 * j + (i & 3);
           const bool seen = key >= low[t] && key <= last[t] && tile.good[i >> 2];
-          x[i] = seen ? x[i] : -INFINITY;
+          x[t][i] = seen ? x[t][i] : -INFINITY;
         }
       }
-      weigh(a, t, x, p);
     }
+    weigh<1>(a, x, p);
     // O^T += V^T P^T
 #pragma unroll
     for (int c = 0; c < kSections; ++c) {
@@ -400,8 +414,8 @@ struct Rows {
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int term = kTerms<T> - 1; term >= 0; --term) {
-            acc[t][at + 2 * pair] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, p[term][t], acc[t][at + 2 * pair], 0, 0, 0);
-            acc[t][at + 2 * pair + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, p[term][t], acc[t][at + 2 * pair + 1], 0, 0, 0);
+            acc[t][at + 2 * pair] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, p[term][t][0], acc[t][at + 2 * pair], 0, 0, 0);
+            acc[t][at + 2 * pair + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, p[term][t][0], acc[t][at + 2 * pair + 1], 0, 0, 0);
           }
       }
     }
@@ -436,14 +450,14 @@ struct Rows {
             const int key = t0 + 16 * s + 4 * block + y;
 #pragma unroll
             for (int t = 0; t < NT; ++t)
-              if (mine && key >= low[t] && key <= last[t]) {
+              {
+                const float add = mine && key >= low[t] && key <= last[t] ? __uint_as_float(0x7fc00000u) : 0.f;
 #pragma unroll
                 for (int cc = 0; cc < kSections; ++cc)
 #pragma unroll
                   for (int i = 0; i < section_elems(cc); ++i)
-                    if (cc == c)
 #pragma unroll
-                      for (int z = 0; z < 4; ++z) acc[t][section_dim(cc) / 16 + i][z] = __uint_as_float(0x7fc00000u);
+                    for (int z = 0; z < 4; ++z) acc[t][section_dim(cc) / 16 + i][z] += cc == c ? add : 0.f;
               }
           }
         }
@@ -502,7 +516,7 @@ __global__ __launch_bounds__(kThreads, (std::is_same_v<T, float> && D > 160 ? 1 
   __shared__ float fold_acc[4][16][kPad];
   __shared__ float fold_m[4][16], fold_l[4][16];
   const int split = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Request rq(a, b);
   if (rq.rows == 0 || rq.rows > a.few) return;
   const int span = rq.end - rq.base, len = decode_split(span);
@@ -568,7 +582,6 @@ __global__ __launch_bounds__(kThreads, (std::is_same_v<T, float> && D > 160 ? 1 
 // Prompts: a workgroup's four waves share the tiles of 64 keys, as operands in LDS.  Wave w makes the operands of the
 // keys 16 w .. 16 w + 15, and of half of the values of the 32 keys from 32 (w / 2) on; an operand is 1 KiB, 16 bytes a lane,
 // written and read in one piece.  Two buffers: while one is read, the codes of the next tile are on their way to registers.
-constexpr int kSharedKeys = 64;
 constexpr int kOperands = 4 * (D / 32) + 2 * (D / 16);  // operands of a tile: keys, then values
 struct SharedFlags {  // what is out of the ordinary in a tile (rare); `any` says whether there is something
   unsigned int any[4], k_nan[4], k_bad[4];
@@ -593,25 +606,50 @@ __device__ __forceinline__ StagedIds staged_ids(const Fp4Args& a, const int* __r
   return ids;
 }
 
-__device__ __forceinline__ void stage_tile(Staged& st, const Fp4Args& a, const StagedIds& ids, int head, int t0, int lane, int w) {
-  const int n = lane & 15, j = lane >> 4, mask = (1 << a.pool.page_shift) - 1;
-  st.k_ok = ids.k >= 0 && ids.k < a.pool.pages;
-  const long k_row = (((long)(st.k_ok ? ids.k : 0) * a.pool.kv_heads + head) << a.pool.page_shift) + ((t0 + 16 * w + n) & mask);
-  const unsigned char* kc = a.pool.k_codes + k_row * (D / 2);
-  const unsigned char* ks = a.pool.k_scales + k_row * (D / 32);
+// Where a lane's codes lie in a page that begins at a tile (or holds a part of one): page 0's addresses.  A row of a pool is a
+// token of a head of a page; value blocks are of four rows, so rows times the bytes of one row are their addresses too.
+struct StagedFrom {
+  const unsigned char *kc, *ks, *vc[2], *vs[2];
+  unsigned int code_page, scale_page;  // bytes of a page
+  int mask;
+  __device__ __forceinline__ void init(const Fp4Args& a, int head, int lane, int w) {
+    const int n = lane & 15, j = lane >> 4;
+    mask = (1 << a.pool.page_shift) - 1;
+    const long head_row = (long)head << a.pool.page_shift;
+    const long k_row = head_row + ((16 * w + n) & mask);
+    kc = a.pool.k_codes + k_row * (D / 2);
+    ks = a.pool.k_scales + k_row * (D / 32);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const long v_row = head_row + ((32 * (w >> 1) + 16 * s + 4 * j) & mask);
+      vc[s] = a.pool.v_codes + v_row * (D / 2);
+      vs[s] = a.pool.v_scales + v_row * (D / 32);
+    }
+    code_page = (unsigned int)(a.pool.kv_heads << a.pool.page_shift) * (D / 2);
+    scale_page = code_page / 16;
+  }
+};
+
+// The codes of the tile at t0, a multiple of 64.
+__device__ __forceinline__ void stage_tile(Staged& st, const Fp4Args& a, const StagedFrom& from, const StagedIds& ids, int t0, int lane) {
+  const int n = lane & 15, j = lane >> 4;
+  const long row = t0 & from.mask & ~(kSharedKeys - 1);  // (uniform) in pages of more than a tile
+  st.k_ok = (unsigned int)ids.k < (unsigned int)a.pool.pages;
+  const unsigned int k_page = st.k_ok ? ids.k : 0;
+  const unsigned char* kc = from.kc + row * (D / 2) + (unsigned long)k_page * from.code_page;
+  const unsigned char* ks = from.ks + row * (D / 32) + (unsigned long)k_page * from.scale_page;
 #pragma unroll
   for (int c = 0; c < kSections; ++c) {
     const int e = section_elems(c), dim = section_dim(c);
-    load_words(&st.k[dim / 32], kc + dim / 2 + j * 2 * e, e / 2);
+    load_words(&st.k[dim / 32], kc + (dim / 2 + j * 2 * e), e / 2);
     st.ks[c] = ks[(dim + j * 4 * e) / 32];
   }
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
-    st.v_ok[s] = ids.v[s] >= 0 && ids.v[s] < a.pool.pages;
-    const long v_blk = ((((long)(st.v_ok[s] ? ids.v[s] : 0) * a.pool.kv_heads + head) << a.pool.page_shift) +
-                        ((t0 + 32 * (w >> 1) + 16 * s + 4 * j) & mask)) >> 2;
-    const unsigned char* vc = a.pool.v_codes + v_blk * (2 * D);
-    const unsigned char* vs = a.pool.v_scales + v_blk * (D / 8);
+    st.v_ok[s] = (unsigned int)ids.v[s] < (unsigned int)a.pool.pages;
+    const unsigned int v_page = st.v_ok[s] ? ids.v[s] : 0;
+    const unsigned char* vc = from.vc[s] + row * (D / 2) + (unsigned long)v_page * from.code_page;
+    const unsigned char* vs = from.vs[s] + row * (D / 32) + (unsigned long)v_page * from.scale_page;
 #pragma unroll
     for (int c = 0; c < kSections; ++c) {
       const int e = section_elems(c), dim = section_dim(c);
@@ -621,59 +659,61 @@ __device__ __forceinline__ void stage_tile(Staged& st, const Fp4Args& a, const S
   }
 }
 
-// Codes to operands.  Keys that no row of the workgroup sees (outside low .. last) are zeros.
-__device__ __forceinline__ void share_tile(Staged& st, bf16x8* __restrict__ operands, SharedFlags& flags, int t0, int low, int last,
-                                           int lane, int w) {
-  const int n = lane & 15, j = lane >> 4;
-  bool k_nan = false, v_nan = false;
+// What is out of the ordinary in the codes of a tile: keys that no row of the workgroup sees (outside low .. last) and pages
+// that are not there become zeros, groups that are not finite zeros and flags.
+__device__ __forceinline__ void check_tile(Staged& st, SharedFlags& flags, int t0, int low, int last, int lane, int w) {
+  const int j = lane >> 4, v0 = t0 + 32 * (w >> 1);
+  bool odd = !(st.k_ok && st.v_ok[0] && st.v_ok[1]);
 #pragma unroll
-  for (int c = 0; c < kSections; ++c) k_nan = k_nan || st.ks[c] == kFp4Nan;
-  const int v0 = t0 + 32 * (w >> 1);
-  if (v0 < low || v0 + 31 > last || __ballot(!(st.v_ok[0] && st.v_ok[1])) != 0ull) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const int key = v0 + 16 * s + 4 * j + y;
-        const bool seen = st.v_ok[s] && key >= low && key <= last;
-#pragma unroll
-        for (int c = 0; c < kSections; ++c) {
-          st.v[s][c][y] = seen ? st.v[s][c][y] : 0u;
-          st.vs[s][c] = seen ? st.vs[s][c] : ((st.vs[s][c] & ~(255u << (8 * y))) | (127u << (8 * y)));
-        }
-      }
-  }
+  for (int c = 0; c < kSections; ++c) odd = odd || st.ks[c] == kFp4Nan;
 #pragma unroll
   for (int s = 0; s < 2; ++s)
 #pragma unroll
     for (int c = 0; c < kSections; ++c) {
       const unsigned int b = st.vs[s][c];
-      v_nan = v_nan || (((b & 0x7f7f7f7fu) + 0x01010101u) & b & 0x80808080u) != 0u;
+      odd = odd || (((b & 0x7f7f7f7fu) + 0x01010101u) & b & 0x80808080u) != 0u;
     }
-  const bool odd = __ballot(k_nan || v_nan || !st.k_ok) != 0ull;
-  if (lane == 0) flags.any[w] = odd ? 1u : 0u;
-  if (odd) {
-    const unsigned long long nan = __ballot(k_nan), bad = __ballot(!st.k_ok);
-    const unsigned int f = (unsigned int)(nan | (nan >> 32)), g = (unsigned int)(bad | (bad >> 32));
-    if (lane == 0) {
-      flags.k_nan[w] = (f | (f >> 16)) & 0xffffu;
-      flags.k_bad[w] = (g | (g >> 16)) & 0xffffu;
+  const bool any = __ballot(odd) != 0ull;
+  if (lane == 0) flags.any[w] = any ? 1u : 0u;
+  if (!any && v0 >= low && v0 + 31 <= last) return;  // (uniform)
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int key = v0 + 16 * s + 4 * j + y;
+      const bool seen = st.v_ok[s] && key >= low && key <= last;
+#pragma unroll
+      for (int c = 0; c < kSections; ++c) {
+        st.v[s][c][y] = seen ? st.v[s][c][y] : 0u;
+        st.vs[s][c] = seen ? st.vs[s][c] : ((st.vs[s][c] & ~(255u << (8 * y))) | (127u << (8 * y)));
+      }
     }
+  if (!any) return;
+  bool k_nan = false;
 #pragma unroll
-    for (int c = 0; c < kSections; ++c)
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const bool here = ((st.vs[s][c] >> (8 * y)) & 255u) == kFp4Nan;
-          const unsigned long long b = __ballot(here);
-          if (lane == 0 && (w & 1) == 0) flags.v_nan[w >> 1][c][s][y] = b;
-          if (here) {
-            st.v[s][c][y] = 0u;
-            st.vs[s][c] = (st.vs[s][c] & ~(255u << (8 * y))) | (127u << (8 * y));
-          }
-        }
+  for (int c = 0; c < kSections; ++c) k_nan = k_nan || st.ks[c] == kFp4Nan;
+  const unsigned long long nan = __ballot(k_nan), bad = __ballot(!st.k_ok);
+  const unsigned int f = (unsigned int)(nan | (nan >> 32)), g = (unsigned int)(bad | (bad >> 32));
+  if (lane == 0) {
+    flags.k_nan[w] = (f | (f >> 16)) & 0xffffu;
+    flags.k_bad[w] = (g | (g >> 16)) & 0xffffu;
   }
+#pragma unroll
+  for (int c = 0; c < kSections; ++c)
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const bool here = ((st.vs[s][c] >> (8 * y)) & 255u) == kFp4Nan;
+        const unsigned long long b = __ballot(here);
+        if (lane == 0 && (w & 1) == 0) flags.v_nan[w >> 1][c][s][y] = b;
+        st.v[s][c][y] = here ? 0u : st.v[s][c][y];
+        st.vs[s][c] = here ? ((st.vs[s][c] & ~(255u << (8 * y))) | (127u << (8 * y))) : st.vs[s][c];
+      }
+}
+
+// Codes to operands: the keys'.
+__device__ __forceinline__ void share_keys(const Staged& st, bf16x8* __restrict__ operands, int lane, int w) {
 #pragma unroll
   for (int c = 0; c < kSections; ++c) {
     const float scale = fp4_scale(st.ks[c]);
@@ -685,21 +725,25 @@ __device__ __forceinline__ void share_tile(Staged& st, bf16x8* __restrict__ oper
           as_operand(fp4_pair<0>(x, scale), fp4_pair<1>(x, scale), fp4_pair<2>(x, scale), fp4_pair<3>(x, scale));
     }
   }
+}
+
+// The values': of the pairs of elements that a lane column has, the wave's half (of a section of one pair, the even wave's).
+__device__ __forceinline__ void share_values(const Staged& st, bf16x8* __restrict__ operands, int lane, int w) {
+  const int n = lane & 15;
 #pragma unroll
   for (int c = 0; c < kSections; ++c) {
     const int e = section_elems(c), at = section_dim(c) / 16;
-    const int mine = max(1, e / 4);              // pairs a wave makes of the section's e / 2
-    if (e == 2 && (w & 1)) continue;             // (uniform) a section of one pair: one of the two waves makes it
-    const int from = e == 2 ? 0 : mine * (w & 1);  // (uniform)
-    float scale[2][4];
+    const int mine = e == 8 ? 2 : 1;
+    if (e == 2 && (w & 1)) continue;  // (uniform)
+    const int from = e == 2 ? 0 : mine * (w & 1);
     unsigned int x[2][4];
+    float scale[2][4];
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         scale[s][y] = fp4_scale((st.vs[s][c] >> (8 * y)) & 255u);
-        const int place = e == 8 ? 0 : e == 4 ? 16 * (n & 1) : 8 * (n & 3);
-        x[s][y] = st.v[s][c][y] >> (place + 8 * from);
+        x[s][y] = st.v[s][c][y] >> ((e == 8 ? 0 : e == 4 ? 16 * (n & 1) : 8 * (n & 3)) + 8 * from);
       }
 #pragma unroll
     for (int pair = 0; pair < mine; ++pair) {
@@ -717,77 +761,88 @@ __device__ __forceinline__ void share_tile(Staged& st, bf16x8* __restrict__ oper
   }
 }
 
-// 32 keys from t0 on (half u of a shared tile).
+// Scores of a shared tile's 64 keys.
 template <typename T, int NT>
-__device__ __forceinline__ void step_shared(Rows<T, NT>& rows, const Fp4Args& a, const bf16x8* __restrict__ operands, const SharedFlags& flags,
-                                            bool odd, int u, int t0, int lane) {
-  const int j = lane >> 4;
-  const bool whole = t0 >= rows.all_low && t0 + kTileKeys - 1 <= rows.all_last;
-  f32x4 sc[NT][2];
+__device__ __forceinline__ void score_shared(const Rows<T, NT>& rows, f32x4 (&sc)[NT][4], const bf16x8* __restrict__ operands, int lane) {
 #pragma unroll
-  for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < 4; ++s)
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i)
+    for (int t = 0; t < NT; ++t) sc[t][s] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const bf16x8 k = operands[((2 * u + s) * (D / 32) + i) * 64 + lane];
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      const bf16x8 k = operands[(s * (D / 32) + i) * 64 + lane];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int term = kTerms<T> - 1; term >= 0; --term)
           sc[t][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, rows.q[term][t][i], sc[t][s], 0, 0, 0);
     }
-  bf16x8 p[kTerms<T>][NT];
+}
+
+// Weights of the scores of the keys t0 .. t0 + 63, and the sums of the values.
+template <typename T, int NT>
+__device__ __forceinline__ void sum_shared(Rows<T, NT>& rows, const Fp4Args& a, const f32x4 (&sc)[NT][4], const bf16x8* __restrict__ operands,
+                                           const SharedFlags& flags, bool odd, int t0, int lane) {
+  const int j = lane >> 4;
+  const bool whole = t0 >= rows.all_low && t0 + kSharedKeys - 1 <= rows.all_last;
+  bf16x8 p[kTerms<T>][NT][2];
+  float x[NT][16];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    float x[8];
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = sc[t][i >> 2][i & 3];
-    if (odd) {
+    for (int i = 0; i < 16; ++i) x[t][i] = sc[t][i >> 2][i & 3];
+  if (odd) {  // (uniform, rare)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int w = 2 * u + (i >> 2), bit = 4 * j + (i & 3);
-        if (flags.any[w] && ((flags.k_nan[w] >> bit) & 1u)) x[i] = __uint_as_float(0x7fc00000u);
-        if (flags.any[w] && ((flags.k_bad[w] >> bit) & 1u)) x[i] = -INFINITY;
-      }
+    for (int i = 0; i < 16; ++i) {
+      const int w = i >> 2, bit = 4 * j + (i & 3);
+      const bool nan = flags.any[w] != 0u && ((flags.k_nan[w] >> bit) & 1u), bad = flags.any[w] != 0u && ((flags.k_bad[w] >> bit) & 1u);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) x[t][i] = bad ? -INFINITY : nan ? __uint_as_float(0x7fc00000u) : x[t][i];
     }
-    if (!whole) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int key = t0 + 16 * (i >> 2) + 4 * j + (i & 3);
-        x[i] = key >= rows.low[t] && key <= rows.last[t] ? x[i] : -INFINITY;
-      }
-    }
-    rows.weigh(a, t, x, p);
   }
-  if (odd && flags.any[2 * u]) {  // values that are not finite (the keys' bad pages are no matter: those values are zeros)
-    for (int s = 0; s < 2; ++s)
-      for (int y = 0; y < 4; ++y)
-        for (int block = 0; block < 4; ++block) {
-          const int key = t0 + 16 * s + 4 * block + y;
+  if (!whole) {
 #pragma unroll
-          for (int c = 0; c < kSections; ++c)
-            if ((flags.v_nan[u][c][s][y] >> (4 * j + 16 * block)) & 1ull) {
+    for (int i = 0; i < 16; ++i) {
+      const int key = t0 + 16 * (i >> 2) + 4 * j + (i & 3);
 #pragma unroll
-              for (int t = 0; t < NT; ++t)
-                if (key >= rows.low[t] && key <= rows.last[t]) {
+      for (int t = 0; t < NT; ++t) x[t][i] = key >= rows.low[t] && key <= rows.last[t] ? x[t][i] : -INFINITY;
+    }
+  }
+  rows.template weigh<2>(a, x, p);
+  if (odd) {  // values that are not finite (those of pages that are not there are zeros)
+    for (int u = 0; u < 2; ++u)
+      if (flags.any[2 * u] != 0u)
+        for (int s = 0; s < 2; ++s)
+          for (int y = 0; y < 4; ++y)
+            for (int block = 0; block < 4; ++block) {
+              const int key = t0 + 32 * u + 16 * s + 4 * block + y;
+#pragma unroll
+              for (int c = 0; c < kSections; ++c) {
+                const bool here = (flags.v_nan[u][c][s][y] >> (4 * j + 16 * block)) & 1ull;
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                  const float add = here && key >= rows.low[t] && key <= rows.last[t] ? __uint_as_float(0x7fc00000u) : 0.f;
 #pragma unroll
                   for (int i = 0; i < section_elems(c); ++i)
 #pragma unroll
-                    for (int z = 0; z < 4; ++z) rows.acc[t][section_dim(c) / 16 + i][z] = __uint_as_float(0x7fc00000u);
+                    for (int z = 0; z < 4; ++z) rows.acc[t][section_dim(c) / 16 + i][z] += add;
                 }
+              }
             }
-        }
   }
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    const bf16x8 v = operands[(4 * (D / 32) + u * (D / 16) + i) * 64 + lane];
+  for (int u = 0; u < 2; ++u)
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int i = 0; i < D / 16; ++i) {
+      const bf16x8 v = operands[(4 * (D / 32) + u * (D / 16) + i) * 64 + lane];
 #pragma unroll
-      for (int term = kTerms<T> - 1; term >= 0; --term)
-        rows.acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[term][t], rows.acc[t][i], 0, 0, 0);
-  }
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int term = kTerms<T> - 1; term >= 0; --term)
+          rows.acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[term][t][u], rows.acc[t][i], 0, 0, 0);
+    }
 }
 
 // Grid (row blocks of a workgroup, kv heads * splits, requests).
@@ -796,8 +851,9 @@ __global__ __launch_bounds__(kThreads, kPromptWaves<T>) void fp4_prompt_kernel(F
   constexpr int NT = kPromptTiles<T>, kBlock = 16 * NT;
   __shared__ bf16x8 operands[2][kOperands * 64];
   __shared__ SharedFlags flags[2];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int head = blockIdx.y % a.pool.kv_heads, split = blockIdx.y / a.pool.kv_heads, b = blockIdx.z;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int head = blockIdx.y % a.pool.kv_heads, split = blockIdx.y / a.pool.kv_heads;
+  const int b = blockIdx.z;
   const Request rq(a, b);
   if (rq.rows <= a.few) return;
   const int blocks = (rq.rows + kBlock - 1) / kBlock;
@@ -817,29 +873,33 @@ __global__ __launch_bounds__(kThreads, kPromptWaves<T>) void fp4_prompt_kernel(F
   const int end = min(min(rq.end, split_begin + len), last + 1);
   const int* row = a.table + (long)b * a.columns;
   if (begin < end) {  // (uniform)
+    StagedFrom from;
+    from.init(a, head, lane, w);
     Staged st;
+    // tiles behind the last are asked for as the last one again: within bounds, and not used
+    const int final = begin + (end - 1 - begin) / kSharedKeys * kSharedKeys;
     StagedIds ids = staged_ids(a, row, begin, lane, w);
-    stage_tile(st, a, ids, head, begin, lane, w);
-    ids = staged_ids(a, row, begin + kSharedKeys < end ? begin + kSharedKeys : begin, lane, w);
-    share_tile(st, operands[0], flags[0], begin, low, last, lane, w);
+    stage_tile(st, a, from, ids, begin, lane);
+    ids = staged_ids(a, row, min(begin + kSharedKeys, final), lane, w);
+    check_tile(st, flags[0], begin, low, last, lane, w);
+    share_keys(st, operands[0], lane, w);
+    share_values(st, operands[0], lane, w);
+    stage_tile(st, a, from, ids, min(begin + kSharedKeys, final), lane);
+    ids = staged_ids(a, row, min(begin + 2 * kSharedKeys, final), lane, w);
     __syncthreads();
     int buffer = 0;
-    for (int t0 = begin; t0 < end; t0 += kSharedKeys, buffer ^= 1) {
-      const int t1 = t0 + kSharedKeys;
-      const bool more = t1 < end;  // (uniform)
-      if (more) {
-        stage_tile(st, a, ids, head, t1, lane, w);
-        ids = staged_ids(a, row, t1 + kSharedKeys < end ? t1 + kSharedKeys : t1, lane, w);
-      }
+    for (int t0 = begin; t0 <= final; t0 += kSharedKeys, buffer ^= 1) {
       const SharedFlags& f = flags[buffer];
       const bool odd = __builtin_amdgcn_readfirstlane(f.any[0] | f.any[1] | f.any[2] | f.any[3]) != 0;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int key = t0 + kTileKeys * u;
-        if (key <= rows.any_last && key + kTileKeys > rows.any_low)  // (uniform in the wave)
-          step_shared<T, NT>(rows, a, operands[buffer], f, odd, u, key, lane);
-      }
-      if (more) share_tile(st, operands[buffer ^ 1], flags[buffer ^ 1], t1, low, last, lane, w);
+      check_tile(st, flags[buffer ^ 1], min(t0 + kSharedKeys, final), low, last, lane, w);
+      // the products of the keys, and beside them the next tile's operands
+      f32x4 sc[NT][4];
+      share_keys(st, operands[buffer ^ 1], lane, w);
+      score_shared<T, NT>(rows, sc, operands[buffer], lane);
+      share_values(st, operands[buffer ^ 1], lane, w);
+      stage_tile(st, a, from, ids, min(t0 + 2 * kSharedKeys, final), lane);
+      ids = staged_ids(a, row, min(t0 + 3 * kSharedKeys, final), lane, w);
+      sum_shared<T, NT>(rows, a, sc, operands[buffer], f, odd, t0, lane);
       __syncthreads();
     }
   }
@@ -942,7 +1002,7 @@ Plan make_plan(int group, int most, int longest, int window) {
   constexpr int kBlock = 16 * kPromptTiles<T>;
   Plan p{16, 0, 0, 0, 0};
   // the keys that a request's rows see, at most: with a window those of its tokens and the window before, in whole tiles
-  const auto seen = [&](int n) { return window > 0 ? (int)min((long)longest, (long)n + window - 1 + kTileKeys) : longest; };
+  const auto seen = [&](int n) { return window > 0 ? (int)min((long)longest, (long)n + window - 1 + kSharedKeys) : longest; };
   // (a request of few rows, and any number of keys up to `longest`: the splits do not shrink with the span but where
   // the length of a split steps up)
   const int few_tokens = max(1, 16 / group);
@@ -1013,6 +1073,7 @@ extern "C" int ls_fp4_attention(int dtype, const void* q, long ldq, void* out, l
              "fp4_attention: %d rows of %d requests, %d heads by %d, %d pages, %d columns", rows, requests, kv_heads, group,
              pages, columns);
   LS_REQUIRE(page_size >= 4 && (page_size & (page_size - 1)) == 0, "fp4_attention: pages of %d tokens", page_size);
+  LS_REQUIRE((long)kv_heads * page_size * (D / 2) <= 0x7fffffffl, "fp4_attention: pages of %d heads of %d tokens", kv_heads, page_size);
   LS_REQUIRE(most <= rows && (long)most * group <= 0x7fffff00l && longest <= 0x7fff0000, "fp4_attention: %d rows a request, %d keys", most, longest);
   if (rows == 0 || most == 0) return 0;
   Fp4Args a;
