@@ -65,16 +65,22 @@ template <typename T> constexpr int kPromptTiles = std::is_same_v<T, float> ? 1 
 #endif
 template <typename T> constexpr int kPromptWaves = D <= 128 ? LS_FP4_PROMPT_WAVES : 1;
 
-// Keys a split of a request of few rows covers, by how many keys its rows see.
-__host__ __device__ inline int decode_split(int span) {
-  if (span <= 4096) return 256;
-  if (span <= 32768) return 512;
-  return 1024 * ((span + 131071) / 131072);
+// Keys a split of a request of few rows covers, by how many keys its rows see and how many heads do so: some 512 workgroups
+// a request at most, and no split too short to be worth its launch.  One split leaves out the second launch.  (8 requests of
+// 532 keys, 8 heads: one split 8.1 us, two 9.4; 64 of up to 8,192: splits of 512 keys 113 us, of 512 and 1,024 96, of 2,048
+// 94; 4 of 131,071: 1,024 keys 134 us, 2,048 122.)
+constexpr int kOneSplit = 768, kDecodeGroups = 512;
+__host__ __device__ inline int shortest_split(int span, int kv_heads) { return kv_heads < 4 ? 256 : span <= 4096 ? 512 : 1024; }
+__host__ __device__ inline int decode_split(int span, int kv_heads) {
+  if (span <= kOneSplit) return kOneSplit;
+  const int even = (int)(((long)span * kv_heads + kDecodeGroups - 1) / kDecodeGroups);
+  return max(shortest_split(span, kv_heads), (even + 127) / 128 * 128);
 }
-constexpr int kPromptBlocks = 32;  // row blocks times splits that a request's head is cut into, about
-__host__ __device__ inline int prompt_split(int span, int blocks) {
-  const int want = max(1, kPromptBlocks / max(1, blocks));
-  return max(512, ((span + want - 1) / want + 63) / 64 * 64);  // whole tiles of 64
+// The same for prompts, by how many workgroups its rows fill.
+constexpr int kPromptGroups = 256, kPromptShortest = 256;
+__host__ __device__ inline int prompt_split(int span, int groups, int kv_heads) {
+  const int want = max(1, kPromptGroups / (max(1, groups) * kv_heads));
+  return max(kPromptShortest, ((span + want - 1) / want + 63) / 64 * 64);  // whole tiles of 64
 }
 
 struct Fp4Args {
@@ -199,6 +205,7 @@ struct Rows {
       const int token = there ? r / a.group : 0, sub = there ? r - token * a.group : 0;
       last[t] = there ? rq.start + token : -1;
       low[t] = there && a.window > 0 ? max(0, last[t] - a.window + 1) : 0;
+      // (a row that is not there has row 0's queries: no branch, and its sums are nobody's)
       const T* from = static_cast<const T*>(a.q) + (long)(rq.first + token) * a.ldq + (long)(head * a.group + sub) * D;
 #pragma unroll
       for (int c = 0; c < kSections; ++c) {
@@ -207,25 +214,19 @@ struct Rows {
         for (int i = 0; i < e / 2; ++i) {
           const T* p = from + dim + (lane >> 4) * 4 * e + 8 * i;
           float x[8];
-          if (there) {
-            if constexpr (sizeof(T) == 2) {
-              typedef unsigned int any4 __attribute__((ext_vector_type(4), aligned(2)));
-              any4 w = *reinterpret_cast<const any4*>(p);
-              if (a.negative) w ^= any4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
-              q[0][t][dim / 32 + i] = as_operand(w[0], w[1], w[2], w[3]);
-            } else {
-              typedef float any4 __attribute__((ext_vector_type(4), aligned(4)));
-              const any4 u = *reinterpret_cast<const any4*>(p), w = *reinterpret_cast<const any4*>(reinterpret_cast<const float*>(p) + 4);
-#pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                x[y] = a.negative ? -u[y] : u[y];
-                x[4 + y] = a.negative ? -w[y] : w[y];
-              }
-            }
+          if constexpr (sizeof(T) == 2) {
+            typedef unsigned int any4 __attribute__((ext_vector_type(4), aligned(2)));
+            any4 w = *reinterpret_cast<const any4*>(p);
+            if (a.negative) w ^= any4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+            q[0][t][dim / 32 + i] = as_operand(w[0], w[1], w[2], w[3]);
           } else {
-            q[0][t][dim / 32 + i] = as_operand(0, 0, 0, 0);
+            typedef float any4 __attribute__((ext_vector_type(4), aligned(4)));
+            const any4 u = *reinterpret_cast<const any4*>(p), w = *reinterpret_cast<const any4*>(reinterpret_cast<const float*>(p) + 4);
 #pragma unroll
-            for (int y = 0; y < 8; ++y) x[y] = 0.f;
+            for (int y = 0; y < 4; ++y) {
+              x[y] = a.negative ? -u[y] : u[y];
+              x[4 + y] = a.negative ? -w[y] : w[y];
+            }
           }
           if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -424,41 +425,30 @@ struct Rows {
   // Values of groups that are not finite: zeros for the product, and NaN in the sums of the rows that see them.
   __device__ __forceinline__ void mark_values(KeyTile& tile, int t0, int lane) {
     const int j = lane >> 4;
+#pragma unroll
     for (int c = 0; c < kSections; ++c)
+#pragma unroll
       for (int s = 0; s < 2; ++s)
-        for (int y = 0; y < 4; ++y) {
-          unsigned int byte = 0u, word = 0u;
-          // (registers are not indexed by a loop's variable)
 #pragma unroll
-          for (int cc = 0; cc < kSections; ++cc)
-#pragma unroll
-            for (int ss = 0; ss < 2; ++ss)
-              if (cc == c && ss == s) {
-                byte = (tile.vs[ss][cc] >> (8 * y)) & 255u;
-                if (byte == kFp4Nan) {
-                  tile.vs[ss][cc] = (tile.vs[ss][cc] & ~(255u << (8 * y))) | (127u << (8 * y));
-#pragma unroll
-                  for (int yy = 0; yy < 4; ++yy)
-                    if (yy == y) tile.v[ss][cc][yy] = word;
-                }
-              }
-          const unsigned long long b = __ballot(byte == kFp4Nan);
+        for (int y = 0; y < 4; ++y) {  // (registers are not indexed by a loop's variable: unrolled)
+          const bool here = ((tile.vs[s][c] >> (8 * y)) & 255u) == kFp4Nan;
+          const unsigned long long b = __ballot(here);
+          tile.v[s][c][y] = here ? 0u : tile.v[s][c][y];
+          tile.vs[s][c] = here ? ((tile.vs[s][c] & ~(255u << (8 * y))) | (127u << (8 * y))) : tile.vs[s][c];
           if (b == 0ull) continue;
+#pragma unroll 1
           for (int block = 0; block < 4; ++block) {
             // the lane's sums are of the columns 4 j .. 4 j + 3, which lie in one group; lane 4 j of the block tells
             const bool mine = (b >> (4 * j + 16 * block)) & 1ull;
             const int key = t0 + 16 * s + 4 * block + y;
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-              {
-                const float add = mine && key >= low[t] && key <= last[t] ? __uint_as_float(0x7fc00000u) : 0.f;
+            for (int t = 0; t < NT; ++t) {
+              const float add = mine && key >= low[t] && key <= last[t] ? __uint_as_float(0x7fc00000u) : 0.f;
 #pragma unroll
-                for (int cc = 0; cc < kSections; ++cc)
+              for (int i = 0; i < section_elems(c); ++i)
 #pragma unroll
-                  for (int i = 0; i < section_elems(cc); ++i)
-#pragma unroll
-                    for (int z = 0; z < 4; ++z) acc[t][section_dim(cc) / 16 + i][z] += cc == c ? add : 0.f;
-              }
+                for (int z = 0; z < 4; ++z) acc[t][section_dim(c) / 16 + i][z] += add;
+            }
           }
         }
   }
@@ -478,6 +468,57 @@ __device__ __forceinline__ void walk_keys(Rows<T, NT>& rows, const Fp4Args& a, c
     const int t1 = t0 + stride < end ? t0 + stride : t0;  // (behind the last tile the same one again: within bounds)
     load_tile(next, a, ids, head, t1, lane);
     ids = load_ids(a, table_row, t1 + stride < end ? t1 + stride : t1, lane);
+    rows.step(a, tile, t0, lane);
+    tile = next;
+  }
+}
+
+// The same for pages of at least 16 tokens: 16 keys lie in one page, so a tile's addresses are two scalars and the lane's own
+// offsets, which never change.  The block table's entries come 64 at a time, one a lane, a run ahead.
+template <typename T, int NT>
+__device__ __forceinline__ void walk_keys_by_pages(Rows<T, NT>& rows, const Fp4Args& a, const int* __restrict__ table_row, int head,
+                                                   int first, int end, int stride, int lane) {
+  if (first >= end) return;
+  const int n = lane & 15, j = lane >> 4, shift = a.pool.page_shift, mask = (1 << shift) - 1;
+  const int final = first + (end - 1 - first) / stride * stride;
+  int base = first >> shift;  // the entry that lane 0 has
+  int now = table_row[min(base + lane, a.columns - 1)], later = table_row[min(base + 64 + lane, a.columns - 1)];
+  const auto load = [&](KeyTile& tile, int t0) LS_INLINED {
+    if (((t0 + 16) >> shift) - base >= 64) {  // (uniform; two neighbouring entries: never more than one run behind)
+      base += 64;
+      now = later;
+      later = table_row[min(base + 64 + lane, a.columns - 1)];
+      if ((t0 >> shift) - base >= 64 || (t0 >> shift) < base) {  // the tile lies across two runs, or far behind: begin there
+        base = t0 >> shift;
+        now = table_row[min(base + lane, a.columns - 1)];
+        later = table_row[min(base + 64 + lane, a.columns - 1)];
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int at = t0 + 16 * s;
+      const int page = __builtin_amdgcn_readlane(now, (at >> shift) - base);
+      tile.good[s] = (unsigned int)page < (unsigned int)a.pool.pages;
+      const long row = (((long)(tile.good[s] ? page : 0) * a.pool.kv_heads + head) << shift) + (at & mask);
+      const unsigned char* kc = a.pool.k_codes + row * (D / 2);
+      const unsigned char* ks = a.pool.k_scales + row * (D / 32);
+      const unsigned char* vc = a.pool.v_codes + row * (D / 2);
+      const unsigned char* vs = a.pool.v_scales + row * (D / 32);
+#pragma unroll
+      for (int c = 0; c < kSections; ++c) {
+        const int e = section_elems(c), dim = section_dim(c);
+        load_words(&tile.k[s][dim / 32], kc + (unsigned int)(n * (D / 2) + dim / 2 + j * 2 * e), e / 2);
+        tile.ks[s][c] = ks[(unsigned int)(n * (D / 32) + (dim + j * 4 * e) / 32)];
+        load_words(tile.v[s][c], vc + (unsigned int)(j * (2 * D) + (dim + n * e) / 8 * 16), 4);
+        load_words(&tile.vs[s][c], vs + (unsigned int)(j * (D / 8) + (dim + n * e) / 32 * 4), 1);
+      }
+    }
+  };
+  KeyTile tile;
+  load(tile, first);
+  for (int t0 = first; t0 <= final; t0 += stride) {
+    KeyTile next;
+    load(next, min(t0 + stride, final));
     rows.step(a, tile, t0, lane);
     tile = next;
   }
@@ -509,28 +550,37 @@ template <> __device__ __forceinline__ void store_run<bf16_t>(bf16_t* to, const 
   }
 }
 
-// Decoded tokens: grid (splits, kv heads, requests).
-template <typename T>
-__global__ __launch_bounds__(kThreads, (std::is_same_v<T, float> && D > 160 ? 1 : 2)) void fp4_decode_kernel(Fp4Args a) {
-  constexpr int kPad = D + 4;
-  __shared__ float fold_acc[4][16][kPad];
-  __shared__ float fold_m[4][16], fold_l[4][16];
-  const int split = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
+// Waves a SIMD: what is in flight is what the waves ask for, a tile each (64 requests of up to 8,192 keys: three waves
+// 108 us, four 101; a second tile ahead in two waves 124).
+template <typename T> constexpr int kDecodeWaves = std::is_same_v<T, float> ? (D > 160 ? 1 : 2) : kSections == 1 ? 4 : D <= 96 ? 3 : 2;
+
+// Decoded tokens: a workgroup has one split of one head of one request.
+constexpr int kFoldPad = D + 4;
+struct FoldShared {
+  float acc[4][16][kFoldPad];
+  float m[4][16], l[4][16];
+};
+template <typename T, bool kWholePages>
+__device__ __forceinline__ void decode_part(const Fp4Args& a, FoldShared& fold, int split, int head, int b) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Request rq(a, b);
   if (rq.rows == 0 || rq.rows > a.few) return;
-  const int span = rq.end - rq.base, len = decode_split(span);
+  const int span = rq.end - rq.base, len = decode_split(span, a.pool.kv_heads);
   const int splits = max(1, (span + len - 1) / len);
   if (split >= splits) return;
   const int begin = rq.base + split * len, end = min(rq.end, begin + len);
   Rows<T, 1> rows;
   rows.init(a, rq, head, 0, lane);
-  walk_keys<T, 1>(rows, a, a.table + (long)b * a.columns, head, begin + kTileKeys * w, end, 4 * kTileKeys, lane);
+  const int* row = a.table + (long)b * a.columns;
+  if constexpr (kWholePages)
+    walk_keys_by_pages<T, 1>(rows, a, row, head, begin + kTileKeys * w, end, 4 * kTileKeys, lane);
+  else
+    walk_keys<T, 1>(rows, a, row, head, begin + kTileKeys * w, end, 4 * kTileKeys, lane);
   const int n = lane & 15, j = lane >> 4;
   const float l = quad16_sum(rows.l[0]);
   if (j == 0) {
-    fold_m[w][n] = rows.m[0];
-    fold_l[w][n] = l;
+    fold.m[w][n] = rows.m[0];
+    fold.l[w][n] = l;
   }
 #pragma unroll
   for (int c = 0; c < kSections; ++c)
@@ -540,7 +590,7 @@ __global__ __launch_bounds__(kThreads, (std::is_same_v<T, float> && D > 160 ? 1 
       float x[8];
 #pragma unroll
       for (int i = 0; i < e; ++i) x[i] = rows.acc[0][section_dim(c) / 16 + i][y];
-      float* to = &fold_acc[w][n][section_dim(c) + e * (4 * j + y)];
+      float* to = &fold.acc[w][n][section_dim(c) + e * (4 * j + y)];
 #pragma unroll
       for (int i = 0; i < e; ++i) to[i] = x[i];
     }
@@ -548,16 +598,16 @@ __global__ __launch_bounds__(kThreads, (std::is_same_v<T, float> && D > 160 ? 1 
   const int there = min(rq.rows, 16);
   for (int i = threadIdx.x; i < there * (D / 4); i += kThreads) {
     const int r = i / (D / 4), d = 4 * (i % (D / 4));
-    float top = fold_m[0][r];
+    float top = fold.m[0][r];
 #pragma unroll
-    for (int k = 1; k < 4; ++k) top = fmaxf(top, fold_m[k][r]);
+    for (int k = 1; k < 4; ++k) top = fmaxf(top, fold.m[k][r]);
     float sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const float f = fold_m[k][r] == -INFINITY ? fold_l[k][r] : weight_exp2<T>(fold_m[k][r] - top);  // (no score: 0, or NaN)
-      sum = fmaf(fold_l[k][r], f, sum);
+      const float f = fold.m[k][r] == -INFINITY ? fold.l[k][r] : weight_exp2<T>(fold.m[k][r] - top);  // (no score: 0, or NaN)
+      sum = fmaf(fold.l[k][r], f, sum);
 #pragma unroll
-      for (int y = 0; y < 4; ++y) x[y] = fmaf(fold_acc[k][r][d + y], f, x[y]);
+      for (int y = 0; y < 4; ++y) x[y] = fmaf(fold.acc[k][r][d + y], f, x[y]);
     }
     if (splits == 1) {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -577,6 +627,12 @@ __global__ __launch_bounds__(kThreads, (std::is_same_v<T, float> && D > 160 ? 1 
       }
     }
   }
+}
+
+template <typename T, bool kWholePages>
+__global__ __launch_bounds__(kThreads, kDecodeWaves<T>) void fp4_decode_kernel(Fp4Args a) {
+  __shared__ FoldShared fold;
+  decode_part<T, kWholePages>(a, fold, blockIdx.x, blockIdx.y, blockIdx.z);  // grid (splits, kv heads, requests)
 }
 
 // Prompts: a workgroup's four waves share the tiles of 64 keys, as operands in LDS.  Wave w makes the operands of the
@@ -845,23 +901,25 @@ __device__ __forceinline__ void sum_shared(Rows<T, NT>& rows, const Fp4Args& a, 
     }
 }
 
-// Grid (row blocks of a workgroup, kv heads * splits, requests).
+struct PromptShared {
+  bf16x8 operands[2][kOperands * 64];
+  SharedFlags flags[2];
+};
+// A workgroup has four row blocks of a head of a request, and one split of its keys.
 template <typename T>
-__global__ __launch_bounds__(kThreads, kPromptWaves<T>) void fp4_prompt_kernel(Fp4Args a) {
+__device__ __forceinline__ void prompt_part(const Fp4Args& a, PromptShared& shared, int place, int head, int b) {
   constexpr int NT = kPromptTiles<T>, kBlock = 16 * NT;
-  __shared__ bf16x8 operands[2][kOperands * 64];
-  __shared__ SharedFlags flags[2];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int head = blockIdx.y % a.pool.kv_heads, split = blockIdx.y / a.pool.kv_heads;
-  const int b = blockIdx.z;
+  auto& operands = shared.operands;
+  auto& flags = shared.flags;
   const Request rq(a, b);
   if (rq.rows <= a.few) return;
   const int blocks = (rq.rows + kBlock - 1) / kBlock;
-  const int group = gridDim.x - 1 - blockIdx.x;  // the blocks that see most keys first
-  if (4 * group >= blocks) return;
-  const int span = rq.end - rq.base, len = prompt_split(span, blocks);
+  const int groups = (blocks + 3) / 4;
+  const int span = rq.end - rq.base, len = prompt_split(span, groups, a.pool.kv_heads);
   const int splits = max(1, (span + len - 1) / len);
-  if (split >= splits) return;
+  if (place >= groups * splits) return;
+  const int split = place / groups, group = groups - 1 - (place - split * groups);  // the rows that see most keys first
   const int row0 = (4 * group + w) * kBlock;
   Rows<T, NT> rows;
   rows.init(a, rq, head, row0, lane);
@@ -938,112 +996,173 @@ __global__ __launch_bounds__(kThreads, kPromptWaves<T>) void fp4_prompt_kernel(F
   }
 }
 
-// Fold the splits of every (row, head): a wave each, four a workgroup.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void fp4_combine_kernel(Fp4Args a) {
+// Steps with prompts: grid (places + splits, kv heads, requests); a request has as many places as row blocks of a workgroup
+// times splits.  Behind them in x is the decoding part, for the requests of few rows among them (only the device knows which; a
+// launch of its own cost 4.5 us with nothing to do).
+template <typename T, bool kWholePages>
+__global__ __launch_bounds__(kThreads, kPromptWaves<T>) void fp4_prompt_kernel(Fp4Args a, int places) {
+  __shared__ union Shared {
+    PromptShared prompt;
+    FoldShared fold;
+    __device__ Shared() {}
+  } shared;
+  const int x = blockIdx.x;
+  if (x < places) prompt_part<T>(a, shared.prompt, x, blockIdx.y, blockIdx.z);
+  else decode_part<T, kWholePages>(a, shared.fold, x - places, blockIdx.y, blockIdx.z);
+}
+
+// Fold the splits of a (row, head): the sums of the splits 0, 4, 8, ..., those of 1, 5, ..., and so on, then the four in order.
+// Few of them: a workgroup each, a wave a sum, the factors of all splits first so that the sums' loads do not wait for one
+// another (4 requests of 131,071 keys in 64 splits: 12 -> 5.4 us).  Many: a wave each, the same sums (bits) in its registers.
+constexpr int kMostSplits = kDecodeGroups;
+static_assert(kPromptGroups <= kMostSplits, "the combine kernel keeps a factor a split");
+template <typename T, bool kWaveEach>
+__global__ __launch_bounds__(kThreads) void fp4_combine_kernel(Fp4Args a) {  // grid ((row, head) pairs of a request, requests)
+  __shared__ float factor[kWaveEach ? 1 : kMostSplits];
+  __shared__ float part[kWaveEach ? 1 : 4][D];
   constexpr int kBlock = 16 * kPromptTiles<T>;
-  const int lane = threadIdx.x & 63;
-  const int heads = a.group * a.pool.kv_heads;
-  const long i = (long)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-  if (i >= (long)a.rows * heads) return;
-  const int row = (int)(i / heads), query_head = (int)(i - (long)row * heads);
-  int b = 0, e = a.requests;  // the last request that begins at or before the row
-  while (e - b > 1) {
-    const int mid = (b + e) >> 1;
-    if (a.offsets[mid] <= row) b = mid; else e = mid;
-  }
+  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int heads = a.group * a.pool.kv_heads, b = blockIdx.y;
   const Request rq(a, b);
-  if (row < rq.first || row >= rq.first + rq.rows / a.group) return;
   const int span = rq.end - rq.base;
-  const int head = query_head / a.group, r = (row - rq.first) * a.group + query_head % a.group;
   const bool few = rq.rows <= a.few;
   const int blocks = (rq.rows + kBlock - 1) / kBlock;
-  const int len = few ? decode_split(span) : prompt_split(span, blocks);
+  const int len = few ? decode_split(span, a.pool.kv_heads) : prompt_split(span, (blocks + 3) / 4, a.pool.kv_heads);
   const int splits = (span + len - 1) / len, stride = few ? 16 : blocks * kBlock;
-  if (splits <= 1) return;
-  const long base = ((long)b * a.pool.kv_heads + head) * a.region;
-  if ((long)(splits - 1) * stride + r >= a.region) return;
-  float top = -INFINITY;
-  for (int s = lane; s < splits; s += 64) top = fmaxf(top, a.part_ml[2 * (base + (long)s * stride + r)]);
-  top = wave_max(top);
+  if (splits <= 1 || splits > kMostSplits) return;
+  const int pairs = rq.rows * a.pool.kv_heads, stride_pairs = kWaveEach ? 4 * gridDim.x : gridDim.x;
   constexpr int kEach = (D + 63) / 64;
-  float sum = 0.f, x[kEach];
+  const int d0 = kEach * lane;
+  for (int place = kWaveEach ? 4 * blockIdx.x + w : blockIdx.x; place < pairs; place += stride_pairs) {
+    const int token = place / heads, query_head = place - token * heads, row = rq.first + token;
+    const int head = query_head / a.group, r = token * a.group + (query_head - head * a.group);
+    if ((long)(splits - 1) * stride + r >= a.region) return;
+    const long base = ((long)b * a.pool.kv_heads + head) * a.region + r;
+    T* out = static_cast<T*>(a.out) + (long)row * a.ldo + (long)query_head * D;
+    const auto sum_at = [&](int s, int y) LS_INLINED -> float { return a.part_acc[(base + (long)s * stride) * D + min(d0 + y, D - 1)]; };
+    // (asked for before the factors are known)
+    float ahead[kWaveEach ? 4 : 1][kEach];
 #pragma unroll
-  for (int y = 0; y < kEach; ++y) x[y] = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < splits; ++s) {
-    const long at = base + (long)s * stride + r;
-    const float m = a.part_ml[2 * at], l = a.part_ml[2 * at + 1];
-    const float f = m == -INFINITY ? l : weight_exp2<T>(m - top);  // (no score: 0, or NaN)
-    sum = fmaf(l, f, sum);
+    for (int k = 0; k < (kWaveEach ? 4 : 1); ++k)
 #pragma unroll
-    for (int y = 0; y < kEach; ++y) {
-      const int d = kEach * lane + y;
-      const float v = a.part_acc[at * D + min(d, D - 1)];
-      x[y] = fmaf(v, f, x[y]);
+      for (int y = 0; y < kEach; ++y) ahead[k][y] = sum_at(min(kWaveEach ? k : w, splits - 1), y);
+    // every wave the same: the largest reference, the factors, the sum of the weights
+    float top = -INFINITY;
+    for (int s = lane; s < splits; s += 64) top = fmaxf(top, a.part_ml[2 * (base + (long)s * stride)]);
+    top = wave_max(top);
+    const auto factor_of = [&](int s, float& l) LS_INLINED -> float {
+      const float m = a.part_ml[2 * (base + (long)s * stride)];
+      l = a.part_ml[2 * (base + (long)s * stride) + 1];
+      return m == -INFINITY ? l : weight_exp2<T>(m - top);  // (no score: 0, or NaN)
+    };
+    float sum = 0.f, l;
+    for (int s = lane; s < splits; s += 64) {
+      const float f = factor_of(s, l);
+      sum = fmaf(l, f, sum);
+      if (!kWaveEach && w == 0) factor[s] = f;
     }
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  T* out = static_cast<T*>(a.out) + (long)row * a.ldo + (long)query_head * D;
+    sum = wave_sum(sum);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if constexpr (kWaveEach) {
+      float x[4][kEach];
 #pragma unroll
-  for (int y = 0; y < kEach; ++y) {
-    const int d = kEach * lane + y;
-    if (d < D) out[d] = from_f32<T>(x[y] * inv);
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int y = 0; y < kEach; ++y) x[k][y] = 0.f;
+      for (int s0 = 0; s0 < splits; s0 += 4)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int s = min(s0 + k, splits - 1);
+          const float f = factor_of(s, l);
+#pragma unroll
+          for (int y = 0; y < kEach; ++y) {
+            const float v = fmaf(s0 == 0 ? ahead[k][y] : sum_at(s, y), f, x[k][y]);
+            x[k][y] = s0 + k < splits ? v : x[k][y];
+          }
+        }
+#pragma unroll
+      for (int y = 0; y < kEach; ++y)
+        if (d0 + y < D) out[d0 + y] = from_f32<T>((((x[0][y] + x[1][y]) + x[2][y]) + x[3][y]) * inv);
+    } else {
+      __syncthreads();
+      float x[kEach];
+#pragma unroll
+      for (int y = 0; y < kEach; ++y) x[y] = w < splits ? fmaf(ahead[0][y], factor[min(w, splits - 1)], 0.f) : 0.f;
+#pragma unroll 8
+      for (int s = w + 4; s < splits; s += 4) {
+        const float f = factor[s];
+#pragma unroll
+        for (int y = 0; y < kEach; ++y) x[y] = fmaf(sum_at(s, y), f, x[y]);
+      }
+#pragma unroll
+      for (int y = 0; y < kEach; ++y)
+        if (d0 + y < D) part[w][d0 + y] = x[y];
+      __syncthreads();
+      if (t < D) out[t] = from_f32<T>((((part[0][t] + part[1][t]) + part[2][t]) + part[3][t]) * inv);
+      __syncthreads();
+    }
   }
 }
 
 struct Plan {
-  int few, decode_splits, prompt_groups, prompt_splits, region;
+  int few, decode_splits, prompt_places, region;  // places: row blocks of a workgroup times splits, of a request's head
 };
 
-// What is launched for requests of at most `most` rows and `longest` keys.
+// What is launched for requests of at most `most` tokens and `longest` keys: bounds for every shorter one.
 template <typename T>
-Plan make_plan(int group, int most, int longest, int window) {
-  constexpr int kBlock = 16 * kPromptTiles<T>;
-  Plan p{16, 0, 0, 0, 0};
+Plan make_plan(int kv_heads, int group, int most, int longest, int window) {
+  constexpr int kGroupRows = 64 * kPromptTiles<T>;
+  Plan p{16, 1, 0, 0};
   // the keys that a request's rows see, at most: with a window those of its tokens and the window before, in whole tiles
   const auto seen = [&](int n) { return window > 0 ? (int)min((long)longest, (long)n + window - 1 + kSharedKeys) : longest; };
-  // (a request of few rows, and any number of keys up to `longest`: the splits do not shrink with the span but where
-  // the length of a split steps up)
-  const int few_tokens = max(1, 16 / group);
-  const int span = seen(min(few_tokens, most));
-  p.decode_splits = 1;
-  const int steps[4] = {span, min(span, 4096), min(span, 32768), min(span, 131072)};
-  for (int s : steps) p.decode_splits = max(p.decode_splits, (s + decode_split(s) - 1) / max(1, decode_split(s)));
-  if (p.decode_splits > 1) p.region = 16 * p.decode_splits;
+  const int span = seen(min(max(1, p.few / group), most));
+  if (span > kOneSplit) {
+    const auto most_of = [&](int n) { return (n + shortest_split(n, kv_heads) - 1) / shortest_split(n, kv_heads); };
+    p.decode_splits = min(max(most_of(span), most_of(min(span, 4096))), (kDecodeGroups + kv_heads - 1) / kv_heads);
+    p.region = 16 * p.decode_splits;
+  }
   const long rows = (long)most * group;
   if (rows > p.few) {
-    const int blocks = (int)((rows + kBlock - 1) / kBlock);
-    p.prompt_groups = (blocks + 3) / 4;
-    const int far = seen(most);
-    p.prompt_splits = min(kPromptBlocks, max(1, (far + 511) / 512));
-    if (p.prompt_splits > 1) p.region = max(p.region, kPromptBlocks * kBlock);
+    // a request with more than one split has `want` places at most, and no split is shorter than the shortest
+    const int want = max(1, kPromptGroups / kv_heads), far = seen(most);
+    p.prompt_places = (int)((rows + kGroupRows - 1) / kGroupRows);
+    if (want > 1 && far > kPromptShortest) {
+      p.prompt_places = (int)max((long)p.prompt_places, min((long)want, (long)p.prompt_places * ((far + kPromptShortest - 1) / kPromptShortest)));
+      p.region = max(p.region, want * kGroupRows);
+    }
   }
   return p;
 }
 
+template <typename T, bool kWholePages>
+void launch_parts(const Fp4Args& a, const Plan& p, hipStream_t stream) {
+  const int heads = a.pool.kv_heads;
+  if (p.prompt_places == 0)
+    fp4_decode_kernel<T, kWholePages><<<dim3(p.decode_splits, heads, a.requests), kThreads, 0, stream>>>(a);
+  else
+    fp4_prompt_kernel<T, kWholePages><<<dim3(p.prompt_places + p.decode_splits, heads, a.requests), kThreads, 0, stream>>>(a, p.prompt_places);
+}
+
 template <typename T>
 int run_fp4(Fp4Args& a, int most, int longest, void* scratch, long scratch_bytes, hipStream_t stream) {
-  const Plan p = make_plan<T>(a.group, most, longest, a.window);
+  const Plan p = make_plan<T>(a.pool.kv_heads, a.group, most, longest, a.window);
   a.few = p.few;
   a.region = p.region;
-  const long entries = (long)a.requests * a.pool.kv_heads * p.region;
+  const int heads = a.pool.kv_heads;
+  const long entries = (long)a.requests * heads * p.region;
   LS_REQUIRE(scratch_bytes >= entries * (D + 2) * (long)sizeof(float), "fp4_attention: %ld bytes of scratch, %ld needed",
              scratch_bytes, entries * (D + 2) * (long)sizeof(float));
   a.part_acc = static_cast<float*>(scratch);
   a.part_ml = a.part_acc + entries * D;
-  const int heads = a.pool.kv_heads;
-  if (p.prompt_groups > 0) {
-    LS_REQUIRE((long)heads * p.prompt_splits <= 65535, "fp4_attention: %d heads in %d splits", heads, p.prompt_splits);
-    fp4_prompt_kernel<T><<<dim3(p.prompt_groups, heads * p.prompt_splits, a.requests), kThreads, 0, stream>>>(a);
-  }
-  // all requests of the step bring `most` rows where the rows say so: then none is left for the other kernel
-  if (p.prompt_groups == 0 || (long)a.requests * most != a.rows)
-    fp4_decode_kernel<T><<<dim3(p.decode_splits, heads, a.requests), kThreads, 0, stream>>>(a);
+  if (a.pool.page_shift >= 4) launch_parts<T, true>(a, p, stream);
+  else launch_parts<T, false>(a, p, stream);
   if (p.region > 0) {
-    const long groups = ((long)a.rows * a.group * heads + 3) / 4;
-    LS_REQUIRE(groups <= 0x7fffffffl, "fp4_attention: %d rows", a.rows);
-    fp4_combine_kernel<T><<<(unsigned)groups, kThreads, 0, stream>>>(a);
+    const long pairs = (long)most * a.group * heads;  // of the request with most
+    LS_REQUIRE(pairs <= 0x7ffffff0l, "fp4_attention: %d rows of %d heads", most, a.group * heads);
+    if (pairs * a.requests >= 4096)
+      fp4_combine_kernel<T, true><<<dim3((unsigned)min((pairs + 3) / 4, 1024l), a.requests), kThreads, 0, stream>>>(a);
+    else
+      fp4_combine_kernel<T, false><<<dim3((unsigned)pairs, a.requests), kThreads, 0, stream>>>(a);
   }
   return check_launch("fp4_attention");
 }
@@ -1057,7 +1176,8 @@ extern "C" int ls_fp4_attention_head_dim() { return ls::D; }
 extern "C" long ls_fp4_attention_scratch_bytes(int dtype, int requests, int kv_heads, int group, int most, int longest, int window) {
   using namespace ls;
   if (requests <= 0 || kv_heads <= 0 || group <= 0 || most <= 0) return 0;
-  const Plan p = dtype == kF32 ? make_plan<float>(group, most, longest, window) : make_plan<bf16_t>(group, most, longest, window);
+  const Plan p = dtype == kF32 ? make_plan<float>(kv_heads, group, most, longest, window)
+                                : make_plan<bf16_t>(kv_heads, group, most, longest, window);
   return (long)requests * kv_heads * p.region * (D + 2) * (long)sizeof(float);
 }
 
@@ -1068,7 +1188,7 @@ extern "C" int ls_fp4_attention(int dtype, const void* q, long ldq, void* out, l
                                 void* scratch, long scratch_bytes, void* stream) {
   using namespace ls;
   LS_REQUIRE(dtype == kF32 || dtype == kBF16, "fp4_attention: dtype %d", dtype);
-  LS_REQUIRE(rows >= 0 && pages >= 1 && kv_heads >= 1 && kv_heads <= 65535 && group >= 1 && columns >= 1 && requests >= 1 &&
+  LS_REQUIRE(rows >= 0 && pages >= 1 && kv_heads >= 1 && kv_heads <= 32767 && group >= 1 && columns >= 1 && requests >= 1 &&
                  requests <= 65535 && most >= 0 && longest >= 0 && window >= 0 && ldq >= 0 && ldo >= 0,
              "fp4_attention: %d rows of %d requests, %d heads by %d, %d pages, %d columns", rows, requests, kv_heads, group,
              pages, columns);

@@ -47,6 +47,10 @@ __device__ __forceinline__ unsigned int logit_key(float f) {  // ascending; -0 c
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
+__device__ __forceinline__ float key_logit(unsigned int key) {  // (0 for -0)
+  return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+}
+
 __device__ __forceinline__ LaneSums fold_sums(const LaneSums& a, const LaneSums& b) {
   const float m = fmaxf(a.m, b.m);
   LaneSums r{m, 0.f, 0.f};
@@ -144,7 +148,7 @@ __device__ __forceinline__ LaneSums piece_sums(const float (&x)[kLaneElems], int
 struct FinishShared {
   float m[kStreams], s[kStreams], t[kStreams];
   int before[kStreams];
-  unsigned int part[kParts];
+  alignas(16) unsigned int part[kParts];
   unsigned int bound;
   int set_list[kMaxSets];
   unsigned int key[kMaxFound];
@@ -299,10 +303,13 @@ __device__ __forceinline__ void finish_row(FinishShared& sh, const float* __rest
     if (t < kParts) {
       const unsigned int key = sh.part[t];
       int larger = 0;
-#pragma unroll 8
-      for (int i = 0; i < kParts; ++i) {
-        const unsigned int other = sh.part[i];
-        larger += other > key || (other == key && i < t) ? 1 : 0;
+#pragma unroll
+      for (int i = 0; i < kParts; i += 4) {
+        const uint4 other = *reinterpret_cast<const uint4*>(&sh.part[i]);
+        larger += other.x > key || (other.x == key && i < t) ? 1 : 0;
+        larger += other.y > key || (other.y == key && i + 1 < t) ? 1 : 0;
+        larger += other.z > key || (other.z == key && i + 2 < t) ? 1 : 0;
+        larger += other.w > key || (other.w == key && i + 3 < t) ? 1 : 0;
       }
       if (larger == top - 1) sh.bound = key;
     }
@@ -324,19 +331,34 @@ __device__ __forceinline__ void finish_row(FinishShared& sh, const float* __rest
         key = id < vocab ? logit_key(to_f32(row[id])) : 0u;
         return id < vocab && key >= bound;
       };
-      int id;
-      unsigned int key;
+      // the first few entries of a thread stay in registers between counting and writing
+      constexpr int kKept = 4;
+      int id[kKept], late_id;
+      unsigned int key[kKept], late_key;
+      bool hit[kKept];
+#pragma unroll
+      for (int k = 0; k < kKept; ++k) {
+        const int i = t + k * kRowThreads;
+        hit[k] = entry(min(i, listed * kLaneElems - 1), id[k], key[k]) && i < listed * kLaneElems;
+      }
       hits = 0;
-      for (int i = t; i < listed * kLaneElems; i += kRowThreads) hits += entry(i, id, key) ? 1 : 0;
+#pragma unroll
+      for (int k = 0; k < kKept; ++k) hits += hit[k] ? 1 : 0;
+      for (int i = t + kKept * kRowThreads; i < listed * kLaneElems; i += kRowThreads) hits += entry(i, late_id, late_key) ? 1 : 0;
       at = row_scan(hits, sh.wave_count, reached);
       if (reached <= kMaxFound) {
         found = reached;
-        if (hits > 0)
-          for (int i = t; i < listed * kLaneElems; i += kRowThreads)
-            if (entry(i, id, key)) {
-              sh.key[at] = key;
-              sh.id[at++] = id;
-            }
+#pragma unroll
+        for (int k = 0; k < kKept; ++k)
+          if (hit[k]) {
+            sh.key[at] = key[k];
+            sh.id[at++] = id[k];
+          }
+        for (int i = t + kKept * kRowThreads; i < listed * kLaneElems; i += kRowThreads)
+          if (entry(i, late_id, late_key)) {
+            sh.key[at] = late_key;
+            sh.id[at++] = late_id;
+          }
         __syncthreads();
       }
     }
@@ -353,7 +375,7 @@ __device__ __forceinline__ void finish_row(FinishShared& sh, const float* __rest
     }
     if (place < top) {
       top_ids[(long)r * top + place] = id;
-      top_logprobs[(long)r * top + place] = (to_f32(row[id]) - all.m) - log_sum;
+      top_logprobs[(long)r * top + place] = (key_logit(key) - all.m) - log_sum;
     }
   }
 }

@@ -98,14 +98,17 @@ class Fp4Pages(NamedTuple):
 
     def geometry(self) -> tuple[int, int, int, int]:
         """(pages, kv heads, page size, d), checked."""
-        if not (self.k_codes.dim() == 4):
-            raise KernelError(f"pages in 4 bits: key codes must be 4-D, got {tuple(self.k_codes.shape)}")
-        pages, kv_heads, page_size, half = self.k_codes.shape
-        for name, t, shape in zip(self._fields, self, self.shapes(pages, kv_heads, page_size, 2 * half)):
-            if not (t.is_cuda and t.dtype == torch.uint8 and t.is_contiguous() and t.shape == shape
-                    and t.device == self.k_codes.device and t.data_ptr() % 16 == 0):
-                raise KernelError(f"pages in 4 bits: {name} must be contiguous, 16-byte aligned uint8 {list(shape)} on one GPU, got "
-                                  f"{t.dtype} {list(t.shape)} on {t.device}")
+        codes = self.k_codes
+        if not (codes.dim() == 4):
+            raise KernelError(f"pages in 4 bits: key codes must be 4-D, got {tuple(codes.shape)}")
+        pages, kv_heads, page_size, half = codes.shape
+        shapes = self.shapes(pages, kv_heads, page_size, 2 * half)
+        device = codes.get_device()
+        for t, shape in zip(self, shapes):
+            if not (t.dtype is torch.uint8 and t.get_device() == device >= 0 and t.is_contiguous() and t.shape == shape
+                    and t.data_ptr() & 15 == 0):
+                raise KernelError("pages in 4 bits: contiguous, 16-byte aligned uint8 tensors on one GPU of the shapes "
+                                  f"{[list(x) for x in shapes]}, got {[(list(x.shape), x.dtype, str(x.device)) for x in self]}")
         return pages, kv_heads, page_size, 2 * half
 
 
@@ -1990,6 +1993,7 @@ class Kernels:
             c_int(parts), _ptr(weight), c_float(eps), _ptr(out), c_long(out.stride(0)), _stream()))
 
     # -- around a step: tables, pages in 4 bits, log probabilities -------------------------
+    # (Checked and launched with plain numbers: with one launch a call, the host's part is what a small call costs.)
     @property
     def serving(self):
         if self._serving is None:
@@ -1997,8 +2001,16 @@ class Kernels:
             lib = ctypes.CDLL(str(path))
             lib.ls_last_error.restype = ctypes.c_char_p
             lib.ls_logprobs_scratch_bytes.restype = c_long
+            lib.ls_logprobs_scratch_bytes.argtypes = [c_int, c_int]
+            p, i, n = c_void_p, c_int, c_long
+            lib.ls_step_tables.argtypes = [p, p, i, p, i, i, p, i, p, p, p, p, i, p, p, p, p]
+            lib.ls_fp4_write.argtypes = [i, p, n, p, n, p, i, i, i, p, p, p, p, i, i, p]
+            lib.ls_fp4_read.argtypes = lib.ls_fp4_write.argtypes
+            lib.ls_token_logprobs.argtypes = [i, p, n, p, i, i, i, p, p, p, p, p, p, n, p]
             self._serving = lib
             self.serving_path = str(path)
+            self._serving_limits = (int(lib.ls_step_tables_max_requests()), int(lib.ls_logprobs_max_top()),
+                                    int(lib.ls_logprobs_max_vocab()))
         return self._serving
 
     def fp4_attention_lib(self, head_dim: int):
@@ -2007,25 +2019,37 @@ class Kernels:
             path = _build.build_fp4_attention(head_dim)
             lib = ctypes.CDLL(str(path))
             lib.ls_last_error.restype = ctypes.c_char_p
+            p, i, n = c_void_p, c_int, c_long
             lib.ls_fp4_attention_scratch_bytes.restype = c_long
+            lib.ls_fp4_attention_scratch_bytes.argtypes = [i, i, i, i, i, i, i]
+            lib.ls_fp4_attention.argtypes = [i, p, n, p, n, i, p, p, p, p, i, i, i, i, p, i, p, p, i, i, i, c_float, i, p, n, p]
             if not (lib.ls_fp4_attention_head_dim() == head_dim):
                 raise KernelError(f"{path} was built for another head size")
             self._fp4_attention[head_dim] = lib
             self.fp4_attention_paths[head_dim] = str(path)
         return lib
 
-    @staticmethod
-    def _here(device, what: str) -> None:
-        """Launches go to the current device's stream: operands on another device are refused."""
-        if device.index != (_raw_device() if _raw_device is not None else torch.cuda.current_device()):
-            raise KernelError(f"{what} works on {device}, which is not the current device")
+    def _launch_plain(self, lib, entry, args: tuple) -> None:
+        """``_launch`` with plain numbers for an entry point whose argument types are declared."""
+        if self.tape is not None:
+            self._launch(lib, entry, tuple(kind(value) for kind, value in zip(entry.argtypes, args)))
+        elif entry(*args) != 0:
+            raise KernelError(lib.ls_last_error().decode())
 
     @staticmethod
-    def _ints(t, n, what: str, device) -> None:
-        if not (t.is_cuda and t.device == device and t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous()
-                and (n is None or t.shape[0] == n)):
-            raise KernelError(f"{what} must be a contiguous int32 vector{'' if n is None else f' of {n}'} on {device}, got "
-                              f"{t.dtype} {list(t.shape)} on {t.device}")
+    def _current(device: int, what: str) -> int:
+        """The current stream, for operands on ``device``: another one than the current device's are refused."""
+        if device < 0:
+            raise KernelError(f"{what}: operands on the host")
+        here = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+        if device != here:
+            raise KernelError(f"{what}: operands on GPU {device}, the current device is {here}")
+        return _raw_stream(here) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+
+    @staticmethod
+    def _ints_refused(what: str, t, n, device: int) -> KernelError:
+        return KernelError(f"{what} must be a contiguous int32 vector{'' if n is None else f' of {n}'} on GPU {device}, got "
+                           f"{t.dtype} {list(t.shape)} on {t.device}")
 
     def step_tables(self, lengths: torch.Tensor, news: torch.Tensor, table: torch.Tensor, page_size: int,
                     free_pages: torch.Tensor, cursor: torch.Tensor, slots: torch.Tensor, tok_seq: torch.Tensor,
@@ -2044,80 +2068,80 @@ class Kernels:
         A request is refused (it brings no tokens and gets no pages) if its numbers are negative or exceed its row of the
         table; and from the first request on for which the free list, or the room of ``slots``, does not suffice, every
         later one that needs a page (brings a token).  Inputs and outputs must not overlap."""
-        requests = lengths.shape[0] if lengths.dim() == 1 else -1
-        device = lengths.device
-        self._ints(lengths, None, "step_tables lengths", device)
-        self._here(device, "step_tables")
-        for name, t, n in (("news", news, requests), ("cursor", cursor, 1), ("free_pages", free_pages, None),
-                           ("slots", slots, None), ("tok_seq", tok_seq, slots.shape[0]), ("tok_pos", tok_pos, slots.shape[0]),
-                           ("offsets", offsets, requests + 1), ("new_lengths", new_lengths, requests),
-                           ("progress", progress, 2)):
-            self._ints(t, n, f"step_tables {name}", device)
-        if not (table.is_cuda and table.device == device and table.dtype == torch.int32 and table.dim() == 2
-                and table.is_contiguous() and table.shape[0] == requests and table.shape[1] >= 1):
-            raise KernelError(f"step_tables table must be a contiguous int32 matrix of {requests} rows, got {list(table.shape)}")
-        if not (page_size >= 4 and page_size & (page_size - 1) == 0):
-            raise KernelError(f"step_tables: a page size is a power of two from 4 on, got {page_size}")
-        if table.shape[1] * page_size > 0x7FFFFFFF:
-            raise KernelError("step_tables: positions beyond 31 bits")
-        limit = self._memo(("tables_requests",), lambda: int(self.serving.ls_step_tables_max_requests()))
-        if requests > limit:
-            raise KernelError(f"step_tables takes at most {limit} requests, got {requests}")
-        ins = [(t.data_ptr(), t.data_ptr() + 4 * t.numel()) for t in (lengths, news, free_pages, cursor)]
-        outs = [(t.data_ptr(), t.data_ptr() + 4 * t.numel())
-                for t in (table, slots, tok_seq, tok_pos, offsets, new_lengths, progress)]
-        for i, (lo, hi) in enumerate(outs):
-            if any(lo < other_hi and other_lo < hi for other_lo, other_hi in ins + outs[:i]):
-                raise KernelError("step_tables: outputs overlap one another or an input")
+        device = lengths.get_device()
+        stream = self._current(device, "step_tables")
+        requests, tokens = lengths.numel(), slots.numel()
+        ins, outs = [], []
+        for name, t, n, to in (("lengths", lengths, requests, ins), ("news", news, requests, ins), ("free_pages", free_pages, None, ins),
+                               ("cursor", cursor, 1, ins), ("slots", slots, tokens, outs), ("tok_seq", tok_seq, tokens, outs),
+                               ("tok_pos", tok_pos, tokens, outs), ("offsets", offsets, requests + 1, outs),
+                               ("new_lengths", new_lengths, requests, outs), ("progress", progress, 2, outs)):
+            count = t.numel()
+            if not (t.dtype is torch.int32 and t.get_device() == device and t.dim() == 1 and (n is None or count == n)
+                    and t.is_contiguous()):
+                raise self._ints_refused(f"step_tables {name}", t, n, device)
+            to.append((t.data_ptr(), 4 * count))
+        if not (table.get_device() == device and table.dtype is torch.int32 and table.dim() == 2
+                and table.shape[0] == requests and table.shape[1] >= 1 and table.is_contiguous()):
+            raise KernelError(f"step_tables table must be a contiguous int32 matrix of {requests} rows, got {table.dtype} "
+                              f"{list(table.shape)} on {table.device}")
+        columns = table.shape[1]
+        if not (page_size >= 4 and page_size & (page_size - 1) == 0 and columns * page_size <= 0x7FFFFFFF):
+            raise KernelError(f"step_tables: a page size is a power of two from 4 on, got {page_size}; positions have 31 bits")
         lib = self.serving
-        self._launch(lib, lib.ls_step_tables, (
-            _ptr(lengths), _ptr(news), c_int(requests), _ptr(table), c_int(table.shape[1]), c_int(page_size),
-            _ptr(free_pages), c_int(free_pages.shape[0]), _ptr(cursor), _ptr(slots), _ptr(tok_seq), _ptr(tok_pos),
-            c_int(slots.shape[0]), _ptr(offsets), _ptr(new_lengths), _ptr(progress), _stream()))
+        if requests > self._serving_limits[0]:
+            raise KernelError(f"step_tables takes at most {self._serving_limits[0]} requests, got {requests}")
+        outs.append((table.data_ptr(), 4 * requests * columns))
+        # an output may lie in no other operand: in the order of their addresses each begins behind all before
+        end = written = 0
+        for (lo, size), output in sorted([(x, False) for x in ins if x[1]] + [(x, True) for x in outs if x[1]]):
+            if lo < (end if output else written):
+                raise KernelError("step_tables: outputs overlap one another or an input")
+            end = max(end, lo + size)
+            if output:
+                written = lo + size
+        self._launch_plain(lib, lib.ls_step_tables, (
+            ins[0][0], ins[1][0], requests, outs[6][0], columns, page_size, ins[2][0], free_pages.numel(), ins[3][0],
+            outs[0][0], outs[1][0], outs[2][0], tokens, outs[3][0], outs[4][0], outs[5][0], stream))
 
     def _fp4_rows(self, what: str, k, v, slots, pages: Fp4Pages):
         count, kv_heads, page_size, d = pages.geometry()
-        device = pages.k_codes.device
-        self._here(device, what)
+        device = pages.k_codes.get_device()
+        stream = self._current(device, what)
         if count * page_size > 0x7FFFFFFF:
             raise KernelError(f"{what}: slots beyond 31 bits")
+        shape = (slots.numel(), kv_heads * d)
         for name, t in (("keys", k), ("values", v)):
-            _rows_ok(t, f"{what} {name}")
-            if not (t.dtype in DTYPE_CODE and t.dtype == k.dtype and t.device == device
-                    and t.shape == (k.shape[0], kv_heads * d) and t.stride(0) >= 0):
-                raise KernelError(f"{what} {name} must be float32 or bfloat16 [{k.shape[0]},{kv_heads * d}] on {device}, got "
-                                  f"{t.dtype} {list(t.shape)} on {t.device}")
-        self._ints(slots, k.shape[0], f"{what} slots", device)
-        return count, kv_heads, page_size, d
+            if not (t.dtype in DTYPE_CODE and t.dtype is k.dtype and t.get_device() == device and t.shape == shape
+                    and t.stride(1) == 1 and t.stride(0) >= 0):
+                raise KernelError(f"{what} {name} must be float32 or bfloat16 {list(shape)} with contiguous rows on GPU {device}, "
+                                  f"got {t.dtype} {list(t.shape)} strides {t.stride()} on {t.device}")
+        if not (slots.dtype is torch.int32 and slots.get_device() == device and slots.dim() == 1 and slots.is_contiguous()):
+            raise self._ints_refused(f"{what} slots", slots, shape[0], device)
+        return (DTYPE_CODE[k.dtype], k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), slots.data_ptr(), shape[0], kv_heads,
+                d, *(t.data_ptr() for t in pages), count, page_size, stream)
 
     def fp4_write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pages: Fp4Pages) -> None:
         """Keys and values ``[tokens, kv heads * d]`` (float32 or bfloat16, rows may be parts of wider ones) rounded to 4
         bits into the slots (page * page size + place in the page) of ``pages``; a token whose slot is negative or
         beyond the pool is left out.  Every group of 32 elements gets a power of two as its scale; a group with an
         infinity or a NaN is held as NaN.  The slots of a call are distinct: of two tokens with one slot a mix remains."""
-        count, kv_heads, page_size, d = self._fp4_rows("fp4_write", k, v, slots, pages)
-        if k.shape[0] == 0:
+        args = self._fp4_rows("fp4_write", k, v, slots, pages)
+        if args[6] == 0:
             return
         lib = self.serving
-        self._launch(lib, lib.ls_fp4_write, (
-            c_int(DTYPE_CODE[k.dtype]), _ptr(k), c_long(k.stride(0)), _ptr(v), c_long(v.stride(0)), _ptr(slots),
-            c_int(k.shape[0]), c_int(kv_heads), c_int(d), _ptr(pages.k_codes), _ptr(pages.k_scales), _ptr(pages.v_codes),
-            _ptr(pages.v_scales), c_int(count), c_int(page_size), _stream()))
+        self._launch_plain(lib, lib.ls_fp4_write, args)
 
     def fp4_read(self, pages: Fp4Pages, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
         """The keys and values that the slots hold, as float32 or bfloat16 (both exact) rows ``[tokens, kv heads * d]``;
         rows whose slot is negative or beyond the pool stay as they are."""
-        count, kv_heads, page_size, d = self._fp4_rows("fp4_read", k, v, slots, pages)
-        for name, t in (("keys", k), ("values", v)):
-            if not (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]):
-                raise KernelError(f"fp4_read {name}: rows overlap")
-        if k.shape[0] == 0:
+        args = self._fp4_rows("fp4_read", k, v, slots, pages)
+        if not (args[6] <= 1 or (args[2] >= k.shape[1] and args[4] >= k.shape[1])):
+            raise KernelError("fp4_read: rows overlap")
+        if args[6] == 0:
             return
         lib = self.serving
-        self._launch(lib, lib.ls_fp4_read, (
-            c_int(DTYPE_CODE[k.dtype]), _ptr(k), c_long(k.stride(0)), _ptr(v), c_long(v.stride(0)), _ptr(slots),
-            c_int(k.shape[0]), c_int(kv_heads), c_int(d), _ptr(pages.k_codes), _ptr(pages.k_scales), _ptr(pages.v_codes),
-            _ptr(pages.v_scales), c_int(count), c_int(page_size), _stream()))
+        self._launch_plain(lib, lib.ls_fp4_read, args)
 
     def fp4_attention(self, q: torch.Tensor, nq: int, nkv: int, d: int, pages: Fp4Pages, table: torch.Tensor,
                       offsets: torch.Tensor, lengths: torch.Tensor, max_tokens: int, max_length: int,
@@ -2134,42 +2158,40 @@ class Kernels:
         own request only, not on what else is in the step, but for the rounding between requests of at most 16 rows a
         key/value head and longer ones, which go through different kernels."""
         count, kv_heads, page_size, dim = pages.geometry()
-        device = q.device
+        device = q.get_device()
+        stream = self._current(device, "fp4_attention")
         _rows_ok(q, "fp4_attention q"); _rows_ok(out, "fp4_attention out")
-        self._here(device, "fp4_attention")
-        if not (q.dtype in DTYPE_CODE and out.dtype == q.dtype and out.device == device and pages.k_codes.device == device):
+        if not (q.dtype in DTYPE_CODE and out.dtype is q.dtype and out.get_device() == device and pages.k_codes.get_device() == device):
             raise KernelError(f"fp4_attention: q {q.dtype} on {q.device}, out {out.dtype} on {out.device}, pages on "
                               f"{pages.k_codes.device}")
-        if not (dim == d and kv_heads == nkv and nkv >= 1 and nq >= nkv and nq % nkv == 0):
+        if not (dim == d and kv_heads == nkv and nq >= nkv and nq % nkv == 0):
             raise KernelError(f"fp4_attention: {nq} query heads over {nkv} of {d}, pages of {kv_heads} heads of {dim}")
-        if not (q.shape[1] >= nq * d and out.shape[1] >= nq * d and out.shape[0] == q.shape[0] and q.stride(0) >= 0
-                and (out.shape[0] <= 1 or out.stride(0) >= nq * d)):
+        rows, width = q.shape
+        ldq, ldo = q.stride(0), out.stride(0)
+        if not (width >= nq * d and out.shape[1] >= nq * d and out.shape[0] == rows and ldq >= 0 and (rows <= 1 or ldo >= nq * d)):
             raise KernelError(f"fp4_attention: rows q {list(q.shape)}, out {list(out.shape)} for {nq} heads of {d}")
-        if not (table.is_cuda and table.device == device and table.dtype == torch.int32 and table.dim() == 2
-                and table.is_contiguous() and table.shape[1] >= 1):
+        if not (table.get_device() == device and table.dtype is torch.int32 and table.dim() == 2 and table.is_contiguous()
+                and table.shape[1] >= 1):
             raise KernelError("fp4_attention block tables must be a contiguous int32 matrix on the GPU")
-        requests = table.shape[0]
-        self._ints(offsets, requests + 1, "fp4_attention offsets", device)
-        self._ints(lengths, requests, "fp4_attention lengths", device)
-        if not (0 <= max_tokens and 0 <= max_length <= table.shape[1] * page_size and window >= 0 and requests <= 65535
-                and nkv <= 1024):
+        requests, columns = table.shape
+        for name, t, n in (("offsets", offsets, requests + 1), ("lengths", lengths, requests)):
+            if not (t.dtype is torch.int32 and t.get_device() == device and t.dim() == 1 and t.numel() == n and t.is_contiguous()):
+                raise self._ints_refused(f"fp4_attention {name}", t, n, device)
+        if not (0 <= max_tokens and 0 <= max_length <= columns * page_size and window >= 0 and requests <= 65535 and nkv <= 1024):
             raise KernelError(f"fp4_attention: at most {max_tokens} rows and {max_length} keys a request, window {window}, "
-                              f"{requests} requests with {table.shape[1]} pages of {page_size}, {nkv} kv heads")
-        max_tokens = min(max_tokens, q.shape[0])
+                              f"{requests} requests with {columns} pages of {page_size}, {nkv} kv heads")
+        max_tokens = min(max_tokens, rows)
         if max_tokens == 0 or requests == 0:
             return
         lib = self.fp4_attention_lib(d)
-        code, group = DTYPE_CODE[q.dtype], nq // nkv
-        need = lib.ls_fp4_attention_scratch_bytes(c_int(code), c_int(requests), c_int(nkv), c_int(group), c_int(max_tokens),
-                                                  c_int(max_length), c_int(window))
+        code, group, window = DTYPE_CODE[q.dtype], nq // nkv, min(window, 0x7FFFFFFF)
+        need = lib.ls_fp4_attention_scratch_bytes(code, requests, nkv, group, max_tokens, max_length, window)
         # (of the call's stream, and of the graph's own memory while one is captured: no two calls share it)
-        scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        self._launch(lib, lib.ls_fp4_attention, (
-            c_int(code), _ptr(q), c_long(q.stride(0)), _ptr(out), c_long(out.stride(0)), c_int(q.shape[0]),
-            _ptr(pages.k_codes), _ptr(pages.k_scales), _ptr(pages.v_codes), _ptr(pages.v_scales), c_int(count),
-            c_int(page_size), c_int(nkv), c_int(group), _ptr(table), c_int(table.shape[1]), _ptr(offsets), _ptr(lengths),
-            c_int(requests), c_int(max_tokens), c_int(max_length), c_float(scale), c_int(window), _ptr(scratch),
-            c_long(need), _stream()))
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        self._launch_plain(lib, lib.ls_fp4_attention, (
+            code, q.data_ptr(), ldq, out.data_ptr(), ldo, rows, *(t.data_ptr() for t in pages), count, page_size, nkv, group,
+            table.data_ptr(), columns, offsets.data_ptr(), lengths.data_ptr(), requests, max_tokens, max_length, scale, window,
+            scratch.data_ptr() if need else 0, need, stream))
 
     def token_logprobs(self, logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tensor, entropy: torch.Tensor,
                        rank: torch.Tensor, top_ids: torch.Tensor, top_logprobs: torch.Tensor) -> None:
@@ -2180,35 +2202,37 @@ class Kernels:
 
         A token outside the vocabulary (-1: none) gets NaN and the rank -1.  A NaN counts as larger than every number; rows
         with a NaN, with an infinity of +, or with nothing but -inf have NaN for what the formula leaves undefined."""
+        device = logits.get_device()
+        stream = self._current(device, "token_logprobs logits")
         _rows_ok(logits, "token_logprobs logits")
-        device = logits.device
-        self._here(device, "token_logprobs")
         rows, vocab = logits.shape
-        if not (logits.dtype in DTYPE_CODE and logits.stride(0) >= 0):
+        ld = logits.stride(0)
+        if not (logits.dtype in DTYPE_CODE and ld >= 0):
             raise KernelError(f"token_logprobs logits must be float32 or bfloat16, got {logits.dtype}")
-        self._ints(tokens, rows, "token_logprobs tokens", device)
-        self._ints(rank, rows, "token_logprobs rank", device)
-        for name, t, shape in (("logprob", logprob, (rows,)), ("entropy", entropy, (rows,)),
-                               ("top_logprobs", top_logprobs, tuple(top_ids.shape))):
-            if not (t.is_cuda and t.device == device and t.dtype == torch.float32 and t.is_contiguous() and t.shape == shape):
-                raise KernelError(f"token_logprobs {name} must be contiguous float32 {list(shape)} on {device}, got "
-                                  f"{t.dtype} {list(t.shape)} on {t.device}")
+        for name, t, kind in (("tokens", tokens, torch.int32), ("rank", rank, torch.int32), ("logprob", logprob, torch.float32),
+                              ("entropy", entropy, torch.float32)):
+            if not (t.dtype is kind and t.get_device() == device and t.dim() == 1 and t.numel() == rows and t.is_contiguous()):
+                raise KernelError(f"token_logprobs {name} must be contiguous {kind} [{rows}] on GPU {device}, got {t.dtype} "
+                                  f"{list(t.shape)} on {t.device}")
         lib = self.serving
-        most, widest = self._memo(("logprobs",), lambda: (int(lib.ls_logprobs_max_top()), int(lib.ls_logprobs_max_vocab())))
-        if not (top_ids.is_cuda and top_ids.device == device and top_ids.dtype == torch.int32 and top_ids.is_contiguous()
-                and top_ids.dim() == 2 and top_ids.shape[0] == rows and top_ids.shape[1] <= min(most, vocab)):
-            raise KernelError(f"token_logprobs top_ids must be contiguous int32 [{rows}, at most {min(most, vocab)}], got "
-                              f"{top_ids.dtype} {list(top_ids.shape)}")
+        _, most, widest = self._serving_limits
+        shape = top_ids.shape
+        if not (top_ids.dtype is torch.int32 and top_ids.get_device() == device and len(shape) == 2 and shape[0] == rows
+                and shape[1] <= most and shape[1] <= vocab and top_ids.is_contiguous()
+                and top_logprobs.dtype is torch.float32 and top_logprobs.get_device() == device and top_logprobs.shape == shape
+                and top_logprobs.is_contiguous()):
+            raise KernelError(f"token_logprobs alternatives must be contiguous int32 and float32 [{rows}, at most {min(most, vocab)}] "
+                              f"on GPU {device}, got {top_ids.dtype} {list(shape)} and {top_logprobs.dtype} {list(top_logprobs.shape)}")
         if rows == 0:
             return
         if not (1 <= vocab <= widest):
             raise KernelError(f"token_logprobs takes 1 to {widest} logits a row, got {vocab}")
-        need = lib.ls_logprobs_scratch_bytes(c_int(rows), c_int(vocab))
-        scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        self._launch(lib, lib.ls_token_logprobs, (
-            c_int(DTYPE_CODE[logits.dtype]), _ptr(logits), c_long(logits.stride(0)), _ptr(tokens), c_int(rows), c_int(vocab),
-            c_int(top_ids.shape[1]), _ptr(logprob), _ptr(entropy), _ptr(rank), _ptr(top_ids), _ptr(top_logprobs),
-            _ptr(scratch), c_long(need), _stream()))
+        need = lib.ls_logprobs_scratch_bytes(rows, vocab)
+        scratch = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+        self._launch_plain(lib, lib.ls_token_logprobs, (
+            DTYPE_CODE[logits.dtype], logits.data_ptr(), ld, tokens.data_ptr(), rows, vocab, shape[1], logprob.data_ptr(),
+            entropy.data_ptr(), rank.data_ptr(), top_ids.data_ptr(), top_logprobs.data_ptr(), scratch.data_ptr() if need else 0,
+            need, stream))
 
 
 ATTENTION_ITEM_INTS = 32

@@ -66,23 +66,26 @@ def test_tensors_on_the_host_are_refused():
 def test_the_plan_of_the_splits_covers_every_request():
     """The launch's bounds (how many splits there are room and workgroups for) hold for every shorter request: the rule
     of csrc/fp4_attention.hip in whole numbers."""
-    def decode_split(span):
-        return 256 if span <= 4096 else 512 if span <= 32768 else 1024 * ((span + 131071) // 131072)
+    def shortest(span, heads):
+        return 256 if heads < 4 else 512 if span <= 4096 else 1024
 
-    def prompt_split(span, blocks):
-        want = max(1, 32 // max(1, blocks))
-        return max(512, ((span + want - 1) // want + 63) // 64 * 64)
+    def decode_split(span, heads):
+        return 768 if span <= 768 else max(shortest(span, heads), (-(-span * heads // 512) + 127) // 128 * 128)
 
-    def planned(span):
-        return max([1] + [-(-s // decode_split(s)) for s in (span, min(span, 4096), min(span, 32768), min(span, 131072)) if s])
+    def prompt_split(span, groups, heads):
+        want = max(1, 256 // (max(1, groups) * heads))
+        return max(256, ((span + want - 1) // want + 63) // 64 * 64)
+
+    def planned(span, heads):
+        return 1 if span <= 768 else min(max(-(-n // shortest(n, heads)) for n in (span, min(span, 4096))), -(-512 // heads))
 
     spans = list(range(0, 5000, 7)) + list(range(32000, 34000, 13)) + list(range(130000, 1100000, 1709)) + [131072, 131073, 262144, 262145]
-    worst = 0
-    for span in sorted(spans):
-        splits = -(-span // decode_split(span))
-        worst = max(worst, splits)
-        assert worst <= planned(span), span
-        for blocks in (1, 2, 3, 5, 11, 16, 31, 32, 33, 500):
-            many = -(-span // prompt_split(span, blocks))
-            assert many <= min(32, max(1, -(-span // 512)))
-            assert blocks * many <= 32 or many <= 1
+    for heads in (1, 2, 3, 4, 5, 8, 12, 64, 300, 600):
+        worst = 0
+        for span in sorted(spans):
+            worst = max(worst, -(-span // decode_split(span, heads)))
+            assert worst <= planned(span, heads) <= 512, (span, heads)
+            for groups in (1, 2, 3, 5, 11, 16, 31, 32, 33, 500):
+                many = -(-span // prompt_split(span, groups, heads))
+                assert many <= max(1, min(256 // heads, -(-span // 256)))
+                assert groups * many <= max(1, 256 // heads) or many <= 1

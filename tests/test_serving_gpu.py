@@ -368,6 +368,16 @@ def test_offsets_and_lengths_that_do_not_fit():
     assert not out[:3].any() and bool(out[3:].any())
 
 
+def test_rows_of_no_request_do_not_hide_a_decoded_token():
+    """As many rows as if every request brought the most: the last ones belong to none."""
+    g = torch.Generator().manual_seed(9)
+    pool, table = make_cache(g, [50, 70], 2, 64, 16)
+    q = torch.randn((80, 4 * 64), generator=g).to(DEV)
+    out = run_attention(q, 4, 2, 64, pool, table, [0, 40, 41], [50, 70], 0, most=40)
+    check_attention(out, q, 4, 2, 64, pool, table, [0, 40, 41], [50, 70], 16, 0)
+    assert bool((out[41:] == 9).all())
+
+
 def test_pages_beyond_32_bits():
     heads, d, page = 8, 128, 16
     pages = 2 ** 32 // (heads * page * d // 2) + 40             # codes of more than 4 GiB
