@@ -15,9 +15,10 @@
 //
 // The alternatives come without a sort.  The lanes' maxima of every piece are kept; the k-th largest of 128 maxima over
 // disjoint parts of the row is a bound that the k first tokens reach (each of those parts holds one that does), and only
-// the lanes that reach it, some k of them, are read again.  Rows where more tokens reach it than there is room for (equal
-// logits, rows that are masked but for a few tokens) and rows with an infinity or a NaN go by the digits of the k-th key
-// instead, which reads the row a dozen times.  A NaN counts as larger than all numbers, -0 as 0.
+// the lanes that reach it, some k of them, are read again.  Where more tokens reach it than there is room for, those above it
+// are taken and then the equal ones from the row's start on (rows that are masked but for a few tokens); rows where that is
+// no use either (ascending logits) and rows with an infinity or a NaN go by the digits of the k-th key, which reads the row
+// a dozen times.  A NaN counts as larger than all numbers, -0 as 0.
 
 #include "common.h"
 #include "serving_api.h"
@@ -32,8 +33,8 @@ constexpr int kMaxPieces = 256;
 constexpr int kMaxVocab = kPiece * kMaxPieces;
 constexpr int kMaxTop = 32;
 constexpr int kParts = 128;       // disjoint parts of the row whose maxima give the bound
-constexpr int kMaxSets = 512;     // lanes of a piece that are read again
-constexpr int kMaxFound = 512;    // tokens that reach the bound
+constexpr int kMaxSets = 64;      // a wave's lanes of pieces that are read again
+constexpr int kMaxFound = 64;     // a wave's tokens that reach the bound
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -149,10 +150,12 @@ struct FinishShared {
   float m[kStreams], s[kStreams], t[kStreams];
   int before[kStreams];
   alignas(16) unsigned int part[kParts];
+  int smaller[4][kParts];
   unsigned int bound;
-  int set_list[kMaxSets];
-  unsigned int key[kMaxFound];
-  int id[kMaxFound];
+  int set_list[kStreams][kMaxSets];
+  int found[kStreams];              // a wave's tokens that reach the bound; more than kMaxFound: too many
+  unsigned int key[kStreams * kMaxFound];
+  int id[kStreams * kMaxFound];
   int digits[kStreams][16];
   int wave_count[kStreams];
 };
@@ -220,7 +223,7 @@ __device__ __forceinline__ int find_by_digits(FinishShared& sh, const T* __restr
   if (mine > 0)
     for (int i = t; i < vocab; i += kRowThreads) {
       const unsigned int key = logit_key(to_f32(row[i]));
-      if (key > prefix && at < kMaxFound) {
+      if (key > prefix && at < top) {
         sh.key[at] = key;
         sh.id[at++] = i;
       }
@@ -240,6 +243,66 @@ __device__ __forceinline__ int find_by_digits(FinishShared& sh, const T* __restr
   return top;
 }
 
+// A wave lists the sets (lanes of pieces) of its own stream that reach the bound, then its tokens that do (sh.found: how many,
+// kMaxFound + 1 where there are more).  `lane_key`: the key of the lane's largest logit.
+template <typename T>
+__device__ __forceinline__ void list_tokens(FinishShared& sh, const float* __restrict__ set_max, unsigned int lane_key, unsigned int bound,
+                                            const T* __restrict__ row, int vocab, int pieces) {
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned long long below = (1ull << lane) - 1ull;
+  int listed = 0, reached = 0;  // (uniform in the wave)
+  if (__ballot(lane_key >= bound) != 0ull)
+#pragma unroll 4
+    for (int p = w; p < pieces; p += kStreams) {
+      const unsigned long long hit = __ballot(logit_key(set_max[p * 64 + lane]) >= bound);
+      const int at = listed + __popcll(hit & below);
+      if (((hit >> lane) & 1ull) && at < kMaxSets) sh.set_list[w][at] = p * 64 + lane;
+      listed += __popcll(hit);
+    }
+  if (listed <= kMaxSets) {
+    constexpr int VEC = Row<T>::VEC;
+#pragma unroll 4
+    for (int i = 0; i < listed * kLaneElems; i += 64) {  // (a wave reads what it has written itself)
+      const int j = i + lane, set = sh.set_list[w][min(j / kLaneElems, listed - 1)], e = j % kLaneElems;
+      const int id = (set >> 6) * kPiece + ((e / VEC) * 64 + (set & 63)) * VEC + e % VEC;
+      const unsigned int key = logit_key(to_f32(row[min(id, vocab - 1)]));
+      const unsigned long long hit = __ballot(j < listed * kLaneElems && id < vocab && key >= bound);
+      const int at = reached + __popcll(hit & below);
+      if (((hit >> lane) & 1ull) && at < kMaxFound) {
+        sh.key[w * kMaxFound + at] = key;
+        sh.id[w * kMaxFound + at] = id;
+      }
+      reached += __popcll(hit);
+    }
+  } else {
+    reached = kMaxFound + 1;
+  }
+  if (lane == 0) sh.found[w] = min(reached, kMaxFound + 1);
+}
+
+// The first `want` tokens (at most 32) whose key is `key`, in the order of their ids, behind what the last list holds.  All
+// lists are short of their room by that much, or this leaves them alone.
+template <typename T>
+__device__ __forceinline__ void first_equal(FinishShared& sh, const T* __restrict__ row, int vocab, unsigned int key, int want) {
+  const int t = threadIdx.x, at = sh.found[kStreams - 1];
+  __syncthreads();
+  if (at + want > kMaxFound) return;  // (uniform)
+  int ties = 0, all;
+  for (int base = 0; base < vocab && ties < want; base += kRowThreads) {
+    const int i = base + t;
+    const bool tie = i < vocab && logit_key(to_f32(row[min(i, vocab - 1)])) == key;
+    const int place = ties + row_scan(tie ? 1 : 0, sh.wave_count, all);
+    if (tie && place < want) {
+      sh.key[(kStreams - 1) * kMaxFound + at + place] = key;
+      sh.id[(kStreams - 1) * kMaxFound + at + place] = i;
+    }
+    ties += all;
+  }
+  __syncthreads();
+  if (t == 0) sh.found[kStreams - 1] = at + min(ties, want);
+  __syncthreads();
+}
+
 // What is left when every stream's lanes have their sums: a workgroup of kRowThreads, wave w with stream w.
 template <typename T>
 __device__ __forceinline__ void finish_row(FinishShared& sh, const float* __restrict__ set_max, LaneSums mine, int before,
@@ -247,7 +310,8 @@ __device__ __forceinline__ void finish_row(FinishShared& sh, const float* __rest
                                            int top, int r, float* __restrict__ logprob, float* __restrict__ entropy,
                                            int* __restrict__ rank, int* __restrict__ top_ids,
                                            float* __restrict__ top_logprobs) {
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const float stream_max = mine.m;
   // fold the lanes (butterfly: every lane the same bits)
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
@@ -289,91 +353,101 @@ __device__ __forceinline__ void finish_row(FinishShared& sh, const float* __rest
   }
   if (top == 0) return;
 
-  int found = -1;
   if (all.s == all.s && all.s != 0.f) {  // finite logits but for -inf
-    const int sets = pieces * 64;
-    float part = -INFINITY;
-    for (int i = t; i < sets; i += kRowThreads) part = fmaxf(part, set_max[i]);
-    with_lane_xor16(part, part, mine.m);
-    part = fmaxf(part, mine.m);
-    with_lane_xor32(part, part, mine.m);
-    part = fmaxf(part, mine.m);
-    if (lane < 16) sh.part[w * 16 + lane] = logit_key(part);
+    unsigned int part = logit_key(stream_max);  // of all the lane's sets
+    const unsigned int lane_key = part;
+    {
+      const auto x = __builtin_amdgcn_permlane16_swap(part, part, false, false);
+      part = max((unsigned int)x[0], (unsigned int)x[1]);
+      const auto y = __builtin_amdgcn_permlane32_swap(part, part, false, false);
+      part = max((unsigned int)y[0], (unsigned int)y[1]);
+    }
+    // (rows of one or two pieces: the lanes of their two waves are the parts)
+    if (pieces <= 2) {
+      if (w < 2) sh.part[w * 64 + lane] = lane_key;
+    } else if (lane < 16) {
+      sh.part[w * 16 + lane] = part;
+    }
     __syncthreads();
-    if (t < kParts) {
-      const unsigned int key = sh.part[t];
+    {  // how many parts are larger: a quarter of the comparisons a thread
+      const int mine = t & (kParts - 1), from = (t / kParts) * (kParts / 4);
+      const unsigned int key = sh.part[mine];
       int larger = 0;
 #pragma unroll
-      for (int i = 0; i < kParts; i += 4) {
-        const uint4 other = *reinterpret_cast<const uint4*>(&sh.part[i]);
-        larger += other.x > key || (other.x == key && i < t) ? 1 : 0;
-        larger += other.y > key || (other.y == key && i + 1 < t) ? 1 : 0;
-        larger += other.z > key || (other.z == key && i + 2 < t) ? 1 : 0;
-        larger += other.w > key || (other.w == key && i + 3 < t) ? 1 : 0;
+      for (int i = 0; i < kParts / 4; i += 4) {
+        const uint4 other = *reinterpret_cast<const uint4*>(&sh.part[from + i]);
+        larger += other.x > key || (other.x == key && from + i < mine) ? 1 : 0;
+        larger += other.y > key || (other.y == key && from + i + 1 < mine) ? 1 : 0;
+        larger += other.z > key || (other.z == key && from + i + 2 < mine) ? 1 : 0;
+        larger += other.w > key || (other.w == key && from + i + 3 < mine) ? 1 : 0;
       }
-      if (larger == top - 1) sh.bound = key;
+      sh.smaller[t / kParts][mine] = larger;
+      __syncthreads();
+      if (t < kParts && sh.smaller[0][t] + sh.smaller[1][t] + sh.smaller[2][t] + sh.smaller[3][t] == top - 1) sh.bound = key;
     }
     __syncthreads();
     const unsigned int bound = sh.bound;
-    // count, add up, write: the lists come out the same every time
-    int hits = 0, listed, reached;
-    for (int i = t; i < sets; i += kRowThreads) hits += logit_key(set_max[i]) >= bound ? 1 : 0;
-    int at = row_scan(hits, sh.wave_count, listed);
-    if (listed <= kMaxSets) {  // uniform
-      if (hits > 0)
-        for (int i = t; i < sets; i += kRowThreads)
-          if (logit_key(set_max[i]) >= bound) sh.set_list[at++] = i;
+    list_tokens<T>(sh, set_max, lane_key, bound, row, vocab, pieces);
+  } else if (lane == 0) {
+    sh.found[w] = kMaxFound + 1;
+    sh.bound = 0xffffffffu;
+  }
+  __syncthreads();
+  int found[kStreams], most = 0, listed = 0;
+  const auto take_lists = [&]() LS_INLINED {
+    most = listed = 0;
+#pragma unroll
+    for (int k = 0; k < kStreams; ++k) {
+      found[k] = sh.found[k];
+      most = max(most, found[k]);
+      listed += found[k];
+    }
+  };
+  take_lists();
+  if (most > kMaxFound) {  // (uniform) many tokens at the bound?  Those above it, and the first of the equal ones
+    const unsigned int bound = sh.bound;
+    if (bound < 0xffffffffu) {
       __syncthreads();
-      constexpr int VEC = Row<T>::VEC;
-      const auto entry = [&](int i, int& id, unsigned int& key) LS_INLINED -> bool {
-        const int set = sh.set_list[i / kLaneElems], e = i % kLaneElems;
-        id = (set >> 6) * kPiece + ((e / VEC) * 64 + (set & 63)) * VEC + e % VEC;
-        key = id < vocab ? logit_key(to_f32(row[id])) : 0u;
-        return id < vocab && key >= bound;
-      };
-      // the first few entries of a thread stay in registers between counting and writing
-      constexpr int kKept = 4;
-      int id[kKept], late_id;
-      unsigned int key[kKept], late_key;
-      bool hit[kKept];
+      list_tokens<T>(sh, set_max, logit_key(stream_max), bound + 1u, row, vocab, pieces);
+      __syncthreads();
+      take_lists();
+    }
+    if (most <= kMaxFound && listed < top) {
+      first_equal<T>(sh, row, vocab, bound, top - listed);
+      take_lists();
+    }
+    if (most > kMaxFound || listed < top) {
+      find_by_digits<T>(sh, row, vocab, top);
+      found[0] = top;
 #pragma unroll
-      for (int k = 0; k < kKept; ++k) {
-        const int i = t + k * kRowThreads;
-        hit[k] = entry(min(i, listed * kLaneElems - 1), id[k], key[k]) && i < listed * kLaneElems;
-      }
-      hits = 0;
-#pragma unroll
-      for (int k = 0; k < kKept; ++k) hits += hit[k] ? 1 : 0;
-      for (int i = t + kKept * kRowThreads; i < listed * kLaneElems; i += kRowThreads) hits += entry(i, late_id, late_key) ? 1 : 0;
-      at = row_scan(hits, sh.wave_count, reached);
-      if (reached <= kMaxFound) {
-        found = reached;
-#pragma unroll
-        for (int k = 0; k < kKept; ++k)
-          if (hit[k]) {
-            sh.key[at] = key[k];
-            sh.id[at++] = id[k];
-          }
-        for (int i = t + kKept * kRowThreads; i < listed * kLaneElems; i += kRowThreads)
-          if (entry(i, late_id, late_key)) {
-            sh.key[at] = late_key;
-            sh.id[at++] = late_id;
-          }
-        __syncthreads();
-      }
+      for (int k = 1; k < kStreams; ++k) found[k] = 0;
+      most = top;
     }
   }
-  if (found < 0) found = find_by_digits<T>(sh, row, vocab, top);
-  // their order: a token's place is how many of the others come before it
-  for (int c = t; c < found; c += kRowThreads) {
-    const unsigned int key = sh.key[c];
-    const int id = sh.id[c];
-    int place = 0;
-    for (int i = 0; i < found; ++i) {
-      const unsigned int other = sh.key[i];
-      place += other > key || (other == key && sh.id[i] < id) ? 1 : 0;
+  // Their order: a token's place is how many of the others come before it.  Eight lanes a token, a list each.
+  const int list = lane & 7;
+  for (int c0 = 0; c0 < kStreams * most; c0 += kRowThreads / 8) {  // (uniform)
+    const int c = c0 + (t >> 3), from = c / most, i = c - from * most;
+    int limit = 0, mine = 0;
+#pragma unroll
+    for (int k = 0; k < kStreams; ++k) {
+      limit = from == k ? found[k] : limit;
+      mine = list == k ? found[k] : mine;
     }
-    if (place < top) {
+    const bool there = from < kStreams && i < limit;
+    const int at = there ? from * kMaxFound + i : 0;
+    const unsigned int key = sh.key[at];
+    const int id = sh.id[at];
+    int place = 0;
+#pragma unroll 4
+    for (int k = 0; k < mine; ++k) {
+      const unsigned int other = sh.key[list * kMaxFound + k];
+      place += other > key || (other == key && sh.id[list * kMaxFound + k] < id) ? 1 : 0;
+    }
+    place += __shfl_xor(place, 1);
+    place += __shfl_xor(place, 2);
+    place += __shfl_xor(place, 4);
+    if (there && list == 0 && place < top) {
       top_ids[(long)r * top + place] = id;
       top_logprobs[(long)r * top + place] = (key_logit(key) - all.m) - log_sum;
     }
@@ -382,14 +456,14 @@ __device__ __forceinline__ void finish_row(FinishShared& sh, const float* __rest
 
 // A workgroup a row (many rows).
 template <typename T>
-__global__ __launch_bounds__(kRowThreads) void logprobs_rows_kernel(const T* __restrict__ logits, long ld,
+__global__ __launch_bounds__(kRowThreads, 8) void logprobs_rows_kernel(const T* __restrict__ logits, long ld,
                                                                     const int* __restrict__ tokens, int vocab, int top,
                                                                     float* __restrict__ logprob, float* __restrict__ entropy,
                                                                     int* __restrict__ rank, int* __restrict__ top_ids,
                                                                     float* __restrict__ top_logprobs) {
   extern __shared__ float set_max[];  // [pieces * 64] where alternatives are asked for
   __shared__ FinishShared sh;
-  const int r = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int r = blockIdx.x, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const T* row = logits + (long)r * ld;
   const int pieces = (vocab + kPiece - 1) / kPiece;
   const int given = tokens[r];
@@ -432,7 +506,7 @@ __global__ __launch_bounds__(kPieceThreads) void logprobs_pieces_kernel(const T*
 }
 
 template <typename T>
-__global__ __launch_bounds__(kRowThreads) void logprobs_fold_kernel(const T* __restrict__ logits, long ld,
+__global__ __launch_bounds__(kRowThreads, 8) void logprobs_fold_kernel(const T* __restrict__ logits, long ld,
                                                                     const int* __restrict__ tokens, int vocab, int pieces,
                                                                     const float* __restrict__ part, const int* __restrict__ count,
                                                                     int top, float* __restrict__ logprob,
@@ -440,7 +514,7 @@ __global__ __launch_bounds__(kRowThreads) void logprobs_fold_kernel(const T* __r
                                                                     int* __restrict__ top_ids, float* __restrict__ top_logprobs) {
   extern __shared__ float set_max[];
   __shared__ FinishShared sh;
-  const int r = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int r = blockIdx.x, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const T* row = logits + (long)r * ld;
   const int given = tokens[r];
   const float mine = given >= 0 && given < vocab ? to_f32(row[given]) : 0.f;
