@@ -632,7 +632,10 @@ __device__ __forceinline__ void decode_part(const Fp4Args& a, FoldShared& fold, 
 template <typename T, bool kWholePages>
 __global__ __launch_bounds__(kThreads, kDecodeWaves<T>) void fp4_decode_kernel(Fp4Args a) {
   __shared__ FoldShared fold;
-  decode_part<T, kWholePages>(a, fold, blockIdx.x, blockIdx.y, blockIdx.z);  // grid (splits, kv heads, requests)
+  // Grid (kv heads, requests, splits): neighbours in x go to one XCD after the other, so with heads there every XCD has as
+  // much to do, and the workgroups of splits that a request does not have come last.  (With splits in x the XCDs of the last
+  // ones had nothing: 64 requests of 4,608 keys in five of eight places 95 us, now 75.)
+  decode_part<T, kWholePages>(a, fold, blockIdx.z, blockIdx.x, blockIdx.y);
 }
 
 // Prompts: a workgroup's four waves share the tiles of 64 keys, as operands in LDS.  Wave w makes the operands of the
@@ -948,7 +951,6 @@ __device__ __forceinline__ void prompt_part(const Fp4Args& a, PromptShared& shar
     int buffer = 0;
     for (int t0 = begin; t0 <= final; t0 += kSharedKeys, buffer ^= 1) {
       const SharedFlags& f = flags[buffer];
-      const bool odd = __builtin_amdgcn_readfirstlane(f.any[0] | f.any[1] | f.any[2] | f.any[3]) != 0;
       check_tile(st, flags[buffer ^ 1], min(t0 + kSharedKeys, final), low, last, lane, w);
       // the products of the keys, and beside them the next tile's operands
       f32x4 sc[NT][4];
@@ -957,6 +959,7 @@ __device__ __forceinline__ void prompt_part(const Fp4Args& a, PromptShared& shar
       share_values(st, operands[buffer ^ 1], lane, w);
       stage_tile(st, a, from, ids, min(t0 + 2 * kSharedKeys, final), lane);
       ids = staged_ids(a, row, min(t0 + 3 * kSharedKeys, final), lane, w);
+      const bool odd = __builtin_amdgcn_readfirstlane(f.any[0] | f.any[1] | f.any[2] | f.any[3]) != 0;
       sum_shared<T, NT>(rows, a, sc, operands[buffer], f, odd, t0, lane);
       __syncthreads();
     }
@@ -996,8 +999,8 @@ __device__ __forceinline__ void prompt_part(const Fp4Args& a, PromptShared& shar
   }
 }
 
-// Steps with prompts: grid (places + splits, kv heads, requests); a request has as many places as row blocks of a workgroup
-// times splits.  Behind them in x is the decoding part, for the requests of few rows among them (only the device knows which; a
+// Steps with prompts: grid (kv heads, places + splits, requests); a request has as many places as row blocks of a workgroup
+// times splits, and with the heads in x an XCD reads few heads' pages again and again.  Behind them in y is the decoding part, for the requests of few rows among them (only the device knows which; a
 // launch of its own cost 4.5 us with nothing to do).
 template <typename T, bool kWholePages>
 __global__ __launch_bounds__(kThreads, kPromptWaves<T>) void fp4_prompt_kernel(Fp4Args a, int places) {
@@ -1006,9 +1009,9 @@ __global__ __launch_bounds__(kThreads, kPromptWaves<T>) void fp4_prompt_kernel(F
     FoldShared fold;
     __device__ Shared() {}
   } shared;
-  const int x = blockIdx.x;
-  if (x < places) prompt_part<T>(a, shared.prompt, x, blockIdx.y, blockIdx.z);
-  else decode_part<T, kWholePages>(a, shared.fold, x - places, blockIdx.y, blockIdx.z);
+  const int at = blockIdx.y, head = blockIdx.x;
+  if (at < places) prompt_part<T>(a, shared.prompt, at, head, blockIdx.z);
+  else decode_part<T, kWholePages>(a, shared.fold, at - places, head, blockIdx.z);
 }
 
 // Fold the splits of a (row, head): the sums of the splits 0, 4, 8, ..., those of 1, 5, ..., and so on, then the four in order.
@@ -1138,9 +1141,9 @@ template <typename T, bool kWholePages>
 void launch_parts(const Fp4Args& a, const Plan& p, hipStream_t stream) {
   const int heads = a.pool.kv_heads;
   if (p.prompt_places == 0)
-    fp4_decode_kernel<T, kWholePages><<<dim3(p.decode_splits, heads, a.requests), kThreads, 0, stream>>>(a);
+    fp4_decode_kernel<T, kWholePages><<<dim3(heads, a.requests, p.decode_splits), kThreads, 0, stream>>>(a);
   else
-    fp4_prompt_kernel<T, kWholePages><<<dim3(p.prompt_places + p.decode_splits, heads, a.requests), kThreads, 0, stream>>>(a, p.prompt_places);
+    fp4_prompt_kernel<T, kWholePages><<<dim3(heads, p.prompt_places + p.decode_splits, a.requests), kThreads, 0, stream>>>(a, p.prompt_places);
 }
 
 template <typename T>
@@ -1159,7 +1162,7 @@ int run_fp4(Fp4Args& a, int most, int longest, void* scratch, long scratch_bytes
   if (p.region > 0) {
     const long pairs = (long)most * a.group * heads;  // of the request with most
     LS_REQUIRE(pairs <= 0x7ffffff0l, "fp4_attention: %d rows of %d heads", most, a.group * heads);
-    if (pairs * a.requests >= 4096)
+    if (pairs * a.requests >= 2048)
       fp4_combine_kernel<T, true><<<dim3((unsigned)min((pairs + 3) / 4, 1024l), a.requests), kThreads, 0, stream>>>(a);
     else
       fp4_combine_kernel<T, false><<<dim3((unsigned)pairs, a.requests), kThreads, 0, stream>>>(a);
