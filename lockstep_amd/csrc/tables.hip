@@ -49,6 +49,8 @@ __device__ __forceinline__ long long block_scan(long long v, long long* __restri
   return before + inclusive - v;
 }
 
+// kEach: requests a thread adds up, their numbers in registers; 0: any, read again in every loop.
+template <int kEach>
 __global__ __launch_bounds__(kTableThreads) void step_tables_kernel(
     const int* __restrict__ lengths, const int* __restrict__ news, int requests, int* table, int columns, int page_shift,
     const int* __restrict__ free_pages, int free_count, const int* __restrict__ cursor, int* __restrict__ slots,
@@ -58,40 +60,52 @@ __global__ __launch_bounds__(kTableThreads) void step_tables_kernel(
   int* begin = held_in_lds;                 // [requests + 1] first row of every request
   int* first_page = begin + requests + 1;   // [requests] where its new pages begin in the free list
   __shared__ long long wave_sums[kTableWaves];
+  __shared__ int4 totals[kTableWaves];
   const int t = threadIdx.x;
-  const int each = (requests + kTableThreads - 1) / kTableThreads;  // neighbouring requests a thread adds up
+  const int each = kEach ? kEach : (requests + kTableThreads - 1) / kTableThreads;  // neighbouring requests a thread adds up
   const int lo = min(requests, t * each), hi = min(requests, lo + each);
   const long long room = (long long)columns << page_shift;
   const long long round = (1ll << page_shift) - 1;
+  int kept_have[kEach ? kEach : 1], kept_fresh[kEach ? kEach : 1];
+  if constexpr (kEach > 0) {
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      kept_have[k] = lo + k < hi ? lengths[lo + k] : -1;
+      kept_fresh[k] = lo + k < hi ? news[lo + k] : 0;
+    }
+  }
   const long long start = cursor[0];
 
-  auto need_of = [&](int i, long long& fresh) LS_INLINED -> long long {  // -1: it does not fit its block table
-    const long long have = lengths[i];
-    fresh = news[i];
-    if (have < 0 || fresh < 0 || have + fresh > room) return -1;
-    return ((have + fresh + round) >> page_shift) - ((have + round) >> page_shift);
+  // body(request, tokens held, new ones, pages needed; -1 where it does not fit its block table)
+  const auto each_request = [&](auto body) LS_INLINED {
+    const auto one = [&](int i, long long have, long long fresh) LS_INLINED {
+      const bool fits = have >= 0 && fresh >= 0 && have + fresh <= room;
+      body(i, have, fresh, fits ? ((have + fresh + round) >> page_shift) - ((have + round) >> page_shift) : -1ll);
+    };
+    if constexpr (kEach > 0) {
+#pragma unroll
+      for (int k = 0; k < kEach; ++k)
+        if (lo + k < hi) one(lo + k, kept_have[k], kept_fresh[k]);
+    } else {
+      for (int i = lo; i < hi; ++i) one(i, lengths[i], news[i]);
+    }
   };
-  long long mine = 0, fresh, all;
-  for (int i = lo; i < hi; ++i) {
-    const long long need = need_of(i, fresh);
-    mine += need > 0 ? need : 0;
-  }
+  long long mine = 0, all;
+  each_request([&](int, long long, long long, long long need) LS_INLINED { mine += need > 0 ? need : 0; });
   long long at = start + block_scan(mine, wave_sums, all);
   // which requests get their pages, and how many rows those bring
   mine = 0;
-  for (int i = lo; i < hi; ++i) {
-    const long long need = need_of(i, fresh);
+  each_request([&](int i, long long, long long fresh, long long need) LS_INLINED {
     const bool taken = need == 0 || (need > 0 && start >= 0 && at + need <= free_count);
     begin[i] = taken ? (int)fresh : -1;
     first_page[i] = taken && need > 0 ? (int)at : 0;
     if (need > 0) at += need;
     if (taken) mine += fresh;
-  }
+  });
   long long row = block_scan(mine, wave_sums, all);
   long long pages = 0, refused = 0, rows = 0;
-  for (int i = lo; i < hi; ++i) {
+  each_request([&](int i, long long have, long long, long long need) LS_INLINED {
     const long long n = begin[i];
-    const long long need = need_of(i, fresh);
     const bool taken = n == 0 || (n > 0 && row + n <= tokens);
     begin[i] = (int)min(row, (long long)tokens);
     if (n > 0) row += n;
@@ -101,21 +115,28 @@ __global__ __launch_bounds__(kTableThreads) void step_tables_kernel(
     } else {
       ++refused;
     }
-    if (blockIdx.x == 0) new_lengths[i] = lengths[i] + (taken ? (int)n : 0);
-  }
+    if (blockIdx.x == 0) new_lengths[i] = (int)have + (taken ? (int)n : 0);
+  });
   // The rows of the requests taken are one run from row 0 on, so the rows behind them are where that run ends; a request
-  // that is refused for its rows begins and ends there.
-  block_scan(rows, wave_sums, all);
-  const int used = (int)all;
+  // that is refused for its rows begins and ends there.  (What is taken fits 31 bits: it fits the outputs and the list.)
+  {
+    const int r = wave_sum((int)rows), p = wave_sum((int)pages), f = wave_sum((int)refused);
+    if ((t & 63) == 0) totals[t >> 6] = make_int4(r, p, f, 0);
+  }
+  __syncthreads();
+  int used = 0, pages_all = 0, refused_all = 0;
+#pragma unroll
+  for (int w = 0; w < kTableWaves; ++w) {
+    used += totals[w].x;
+    pages_all += totals[w].y;
+    refused_all += totals[w].z;
+  }
   for (int i = lo; i < hi; ++i) begin[i] = min(begin[i], used);
   if (t == 0) begin[requests] = used;
   if (blockIdx.x == 0) {
-    long long pages_all, refused_all;
-    block_scan(pages, wave_sums, pages_all);
-    block_scan(refused, wave_sums, refused_all);
     if (t == 0) {
-      progress[0] = (int)(start + pages_all);
-      progress[1] = (int)refused_all;
+      progress[0] = (int)start + pages_all;
+      progress[1] = refused_all;
       offsets[requests] = used;
     }
     for (int i = lo; i < hi; ++i) offsets[i] = begin[i];
@@ -169,12 +190,12 @@ extern "C" int ls_step_tables(const int* lengths, const int* news, int requests,
   const int run = requests > 1024 ? 4 * kTableThreads : kTableThreads;
   const int groups = tokens > run ? (tokens + run - 1) / run : 1;
   const size_t lds = sizeof(int) * (2 * (size_t)requests + 1);
-  if (lds + 64 > 64 * 1024) {
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(step_tables_kernel),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 1024);
+  auto* kernel = requests <= kTableThreads ? step_tables_kernel<1> : requests <= 4 * kTableThreads ? step_tables_kernel<4> : step_tables_kernel<0>;
+  if (lds + 128 > 64 * 1024) {
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 1024);
     LS_REQUIRE(e == hipSuccess, "step_tables: %s", hipGetErrorString(e));
   }
-  step_tables_kernel<<<groups < 1024 ? groups : 1024, kTableThreads, lds, (hipStream_t)stream>>>(
+  kernel<<<groups < 1024 ? groups : 1024, kTableThreads, lds, (hipStream_t)stream>>>(
       lengths, news, requests, table, columns, shift, free_pages, free_count, cursor, slots, tok_seq, tok_pos, tokens,
       offsets, new_lengths, progress);
   return check_launch("step_tables");

@@ -480,9 +480,9 @@ def test_tokens_outside_the_vocabulary():
 
 def test_a_row_has_the_same_bits_beside_others():
     g = torch.Generator().manual_seed(12)
-    for dtype in (torch.float32, torch.bfloat16):
-        x = (2.5 * torch.randn((600, 20011), generator=g)).to(dtype).to(DEV)
-        tokens = torch.randint(0, 20011, (600,), generator=g).tolist()
+    for dtype, vocab in ((torch.float32, 20011), (torch.bfloat16, 20011), (torch.float32, 50021), (torch.bfloat16, 50021)):
+        x = (2.5 * torch.randn((600, vocab), generator=g)).to(dtype).to(DEV)
+        tokens = torch.randint(0, vocab, (600,), generator=g).tolist()
         many = run_logprobs(x, tokens, 5)
         for lo, hi in ((0, 1), (5, 22), (599, 600)):
             few = run_logprobs(x[lo:hi], tokens[lo:hi], 5)
