@@ -22,6 +22,7 @@ _LAZY = {
     "LLM": ("lockstep_amd.engine.llm", "LLM"),
     "EngineConfig": ("lockstep_amd.engine.config", "EngineConfig"),
     "generate_greedy": ("lockstep_amd.engine.llm", "generate_greedy"),
+    "score": ("lockstep_amd.engine.llm", "score"),
     "DefaultPolicy": ("lockstep_amd.engine.policy", "DefaultPolicy"),
     "FixedChunkPolicy": ("lockstep_amd.engine.policy", "FixedChunkPolicy"),
     "OutOfPages": ("lockstep_amd.cache", "OutOfPages"),

@@ -14,6 +14,8 @@ from __future__ import annotations
 
 from typing import Iterable, Sequence
 
+import torch
+
 from .batch import StepEntry
 from .config import EngineConfig
 from .model import Model, load_model
@@ -49,6 +51,36 @@ def generate_greedy(model: Model, prompt_ids: Sequence[int], max_new_tokens: int
     return seq.generated, step_logits
 
 
+def score(model: Model, token_ids: Sequence[int], top: int = 0, portion: int = 256, page_size: int = 16) -> list[dict]:
+    """What the model makes of the tokens that are there: for every token but the first, its log probability given those before
+    it, the ``entropy`` of that distribution, the token's ``rank`` (0: the likeliest) and the ``top`` likeliest tokens as
+    (id, log probability) pairs.  ``portion``: how many positions' logits are held at a time."""
+    n = len(token_ids)
+    if n < 2:
+        return []
+    if portion < 1:
+        raise ValueError(f"portions of {portion} tokens")
+    kernels, device = model.rt.kernels, model.rt.device
+    cache = model.make_cache(num_pages=-(-n // page_size), page_size=page_size, max_requests=1, max_tokens_per_request=n)
+    cache.open("score")
+    found: list[dict] = []
+    for lo in range(0, n - 1, portion):
+        feed = list(token_ids[lo:min(n - 1, lo + portion)])
+        rows = len(feed)
+        logits = model.step(cache, [StepEntry("score", feed, range(rows))])
+        given = torch.tensor(list(token_ids[lo + 1:lo + 1 + rows]), dtype=torch.int32).to(device)
+        whole = torch.empty((2, rows), dtype=torch.float32, device=device)
+        rank = torch.empty(rows, dtype=torch.int32, device=device)
+        ids = torch.empty((rows, top), dtype=torch.int32, device=device)
+        logprobs = torch.empty((rows, top), dtype=torch.float32, device=device)
+        kernels.token_logprobs(logits, given, whole[0], whole[1], rank, ids, logprobs)
+        columns = whole.tolist()
+        for logprob, entropy, place, likeliest, theirs in zip(*columns, rank.tolist(), ids.tolist(), logprobs.tolist()):
+            found.append({"logprob": logprob, "entropy": entropy, "rank": place, "top": list(zip(likeliest, theirs))})
+    cache.close("score")
+    return found
+
+
 class LLM:
     """A loaded model plus what a workload needs to run on it.  Options are an ``EngineConfig``
     or its fields as keywords."""
@@ -72,3 +104,7 @@ class LLM:
 
     def generate_greedy(self, prompt_ids, max_new_tokens: int, eos_token_ids=None):
         return generate_greedy(self.model, prompt_ids, max_new_tokens, eos_token_ids)
+
+    def score(self, token_ids, top: int = 0) -> list[dict]:
+        """Log probabilities of the tokens that are there (``score``)."""
+        return score(self.model, token_ids, top, page_size=self.config.page_size)

@@ -607,3 +607,28 @@ def test_a_run_of_them_together_eager_captured_and_on_two_streams(dtype):
                                           last["new_lengths"].tolist(), 8, 0.125, 0)
     bound = 2 * spread * (68 * 2.0 ** -24 * reach + 2.0 ** -21) + spread * (U[torch.bfloat16] + 2.0 ** -16) + U[dtype] * want.abs() + 1e-30
     assert bool(((last["out"].double().cpu() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("tiny", ["A", "B"])
+def test_scores_of_a_model(tiny_dirs, tiny):
+    from plain.qwen3_plain import PlainModel
+
+    from lockstep_amd import LLM, score
+
+    folder = tiny_dirs[(tiny, "gen")]
+    g = torch.Generator().manual_seed(13)
+    tokens = torch.randint(0, 512, (41,), generator=g).tolist()
+    logits = PlainModel(folder).logits(tokens)[:-1].double()
+    want = plain.token_logprobs(logits, tokens[1:], 3)
+    llm = LLM(folder, dtype="float32", num_pages=16)
+    for found in (llm.score(tokens, top=3), score(llm.model, tokens, top=3, portion=7, page_size=8)):
+        assert len(found) == 40
+        # the float32 engine's logits agree with the plain ones to about 1e-6 of their spread
+        spread = 1e-4 * float(logits.abs().max())
+        assert max(abs(f["logprob"] - float(w)) for f, w in zip(found, want["logprob"])) < spread
+        assert max(abs(f["entropy"] - float(w)) for f, w in zip(found, want["entropy"])) < spread
+        assert [f["rank"] for f in found] == want["rank"]
+        assert [[t for t, _ in f["top"]] for f in found] == want["top_ids"]
+    assert llm.score(tokens[:1]) == [] and len(llm.score(tokens[:2])) == 1
+    with pytest.raises(KernelError):
+        llm.score(tokens, top=33)
