@@ -16,12 +16,17 @@
 // a key or value is exact, so the sums are those of 32-bit operands.
 //
 // Requests of at most 16 rows a head (decoded tokens): a workgroup's four waves take the key tiles of one split in turn
-// and fold at the end through LDS.  Others (prompts): every wave has a block of rows of its own.  In both a request's keys
-// are cut into splits by a rule of its own length (and rows) alone; where there are several, they leave sums that a second
-// launch folds in ascending order.  So a row's result does not depend on what else is in the step.
+// and fold at the end through LDS.  Others (prompts): every wave has a block of rows of its own, and the four waves of a
+// workgroup share the operands of tiles of 64 keys through LDS.  In both a request's keys are cut into splits by a rule of its
+// own length (and rows) and of the heads alone; where there are several, they leave sums that a second launch folds.  So a
+// row's result does not depend on what else is in the step.
 //
-// What bounds it: decoding reads 17/32 bytes a key element from HBM and spends about 1.2 vector instructions on each, some
-// two thirds of what the memory leaves room for; prompts are bound by the vector unit's softmax next to the matrix units.
+// What bounds it: decoding, the bytes (17/32 a key element): 4 requests of 131,071 keys are read at 5.3 TB/s, 64 of up to 8,192
+// at 4.1 with what their splits cost; some 6 vector instructions a key and lane column are two thirds of what that leaves
+// room for.  Prompts, the vector unit next to the matrix units: a tile of 16 rows by 32 keys has 16 products of 16 cycles and
+// some 60 vector instructions of 4, of them 8 exponentials of 16, and two waves a SIMD overlap them in part (830 TFLOP/s at
+// 8,192 keys in pages of 16 where a large product of the library reaches 1,190).  Two groups of waves a barrier apart, one at the
+// matrix and one at the vector units, were slower (885 us for 821: alone on its SIMD, a wave waits for its own results).
 
 #include "fp4.h"
 #include "fp4_attention_api.h"
@@ -104,6 +109,9 @@ struct Fp4Args {
   int few;                 // rows a head up to which a request belongs to the decoding kernel
 };
 
+// The first key that a row at `position` sees.
+__device__ __forceinline__ int first_seen(int position, int window) { return window > 0 && position >= window ? position - window + 1 : 0; }
+
 // One request as all kernels see it.
 struct Request {
   int first, rows, start, base, end;  // first packed row, rows a head, first position, keys that are seen: base .. end - 1
@@ -113,10 +121,10 @@ struct Request {
     first = ok ? from : 0;
     const int n = ok ? to - from : 0;
     rows = n * a.group;
-    const int room = (int)min((long)a.columns << a.pool.page_shift, 0x7fffffffl);
+    const int room = (int)min((long)a.columns << a.pool.page_shift, 0x7fff0000l);  // (a few tiles on stay below 2^31)
     end = min(max(a.lengths[b], 0), room);
     start = end - n;
-    base = a.window > 0 ? max(0, start - a.window + 1) & ~(kSharedKeys - 1) : 0;
+    base = first_seen(start, a.window) & ~(kSharedKeys - 1);
   }
 };
 
@@ -204,7 +212,7 @@ struct Rows {
       const bool there = r < rq.rows;
       const int token = there ? r / a.group : 0, sub = there ? r - token * a.group : 0;
       last[t] = there ? rq.start + token : -1;
-      low[t] = there && a.window > 0 ? max(0, last[t] - a.window + 1) : 0;
+      low[t] = there ? first_seen(last[t], a.window) : 0;
       // (a row that is not there has row 0's queries: no branch, and its sums are nobody's)
       const T* from = static_cast<const T*>(a.q) + (long)(rq.first + token) * a.ldq + (long)(head * a.group + sub) * D;
 #pragma unroll
@@ -252,8 +260,8 @@ struct Rows {
     if (row0 < row_end) {
       all_last = rq.start + row0 / a.group;
       any_last = rq.start + (row_end - 1) / a.group;
-      any_low = a.window > 0 ? max(0, all_last - a.window + 1) : 0;
-      all_low = a.window > 0 ? max(0, any_last - a.window + 1) : 0;
+      any_low = first_seen(all_last, a.window);
+      all_low = first_seen(any_last, a.window);
     }
   }
 
@@ -928,7 +936,7 @@ __device__ __forceinline__ void prompt_part(const Fp4Args& a, PromptShared& shar
   rows.init(a, rq, head, row0, lane);
   // the keys that the workgroup's rows see
   const int first_token = 4 * group * kBlock / a.group, last_token = (min((4 * group + 4) * kBlock, rq.rows) - 1) / a.group;
-  const int low = a.window > 0 ? max(0, rq.start + first_token - a.window + 1) : 0, last = rq.start + last_token;
+  const int low = first_seen(rq.start + first_token, a.window), last = rq.start + last_token;
   const int split_begin = rq.base + split * len;
   const int begin = low > split_begin ? split_begin + (low - split_begin) / kSharedKeys * kSharedKeys : split_begin;
   const int end = min(min(rq.end, split_begin + len), last + 1);
@@ -1152,6 +1160,7 @@ int run_fp4(Fp4Args& a, int most, int longest, void* scratch, long scratch_bytes
   a.few = p.few;
   a.region = p.region;
   const int heads = a.pool.kv_heads;
+  LS_REQUIRE((long)p.prompt_places + p.decode_splits <= 65535, "fp4_attention: %d rows a request", most);
   const long entries = (long)a.requests * heads * p.region;
   LS_REQUIRE(scratch_bytes >= entries * (D + 2) * (long)sizeof(float), "fp4_attention: %ld bytes of scratch, %ld needed",
              scratch_bytes, entries * (D + 2) * (long)sizeof(float));

@@ -506,7 +506,7 @@ __global__ __launch_bounds__(kPieceThreads) void logprobs_pieces_kernel(const T*
 }
 
 template <typename T>
-__global__ __launch_bounds__(kRowThreads, 8) void logprobs_fold_kernel(const T* __restrict__ logits, long ld,
+__global__ __launch_bounds__(kRowThreads, 4) void logprobs_fold_kernel(const T* __restrict__ logits, long ld,
                                                                     const int* __restrict__ tokens, int vocab, int pieces,
                                                                     const float* __restrict__ part, const int* __restrict__ count,
                                                                     int top, float* __restrict__ logprob,
@@ -520,13 +520,25 @@ __global__ __launch_bounds__(kRowThreads, 8) void logprobs_fold_kernel(const T* 
   const float mine = given >= 0 && given < vocab ? to_f32(row[given]) : 0.f;
   LaneSums sums{-INFINITY, 0.f, 0.f};
   int before = 0;
-#pragma unroll 4
-  for (int p = w; p < pieces; p += kStreams) {
-    const long at = (long)r * pieces + p;
-    const LaneSums here{part[at * 192 + lane], part[at * 192 + 64 + lane], part[at * 192 + 128 + lane]};
-    before += count[at];
-    if (top > 0) set_max[p * 64 + lane] = here.m;
-    sums = fold_sums(sums, here);
+  constexpr int kBatch = 10;  // pieces whose sums are asked for together
+  for (int p0 = w; p0 < pieces; p0 += kBatch * kStreams) {
+    LaneSums here[kBatch];
+    int counts[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const long at = (long)r * pieces + min(p0 + k * kStreams, pieces - 1);
+      here[k] = LaneSums{part[at * 192 + lane], part[at * 192 + 64 + lane], part[at * 192 + 128 + lane]};
+      counts[k] = count[at];
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int p = p0 + k * kStreams;
+      if (p < pieces) {  // (uniform)
+        before += counts[k];
+        if (top > 0) set_max[p * 64 + lane] = here[k].m;
+        sums = fold_sums(sums, here[k]);
+      }
+    }
   }
   finish_row<T>(sh, set_max, sums, before, row, vocab, pieces, given, mine, top, r, logprob, entropy, rank, top_ids,
                 top_logprobs);

@@ -2184,7 +2184,9 @@ class Kernels:
         if max_tokens == 0 or requests == 0:
             return
         lib = self.fp4_attention_lib(d)
-        code, group, window = DTYPE_CODE[q.dtype], nq // nkv, min(window, 0x7FFFFFFF)
+        code, group = DTYPE_CODE[q.dtype], nq // nkv
+        if window >= max_length:
+            window = 0                         # every row sees all keys before it
         need = lib.ls_fp4_attention_scratch_bytes(code, requests, nkv, group, max_tokens, max_length, window)
         # (of the call's stream, and of the graph's own memory while one is captured: no two calls share it)
         scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None

@@ -368,6 +368,18 @@ def test_offsets_and_lengths_that_do_not_fit():
     assert not out[:3].any() and bool(out[3:].any())
 
 
+@pytest.mark.parametrize("news", [1, 30])
+def test_windows_as_wide_as_the_context(news):
+    g = torch.Generator().manual_seed(10)
+    pool, table = make_cache(g, [300, 90], 2, 64, 16)
+    q = torch.randn((2 * news, 4 * 64), generator=g).to(DEV)
+    args = (q, 4, 2, 64, pool, table, [0, news, 2 * news], [300, 90])
+    whole = run_attention(*args, 0)
+    for window in (300, 301, 2 ** 31 - 1, 2 ** 40):
+        assert torch.equal(run_attention(*args, window), whole)
+    check_attention(run_attention(*args, 299), q, 4, 2, 64, pool, table, [0, news, 2 * news], [300, 90], 16, 299)
+
+
 def test_rows_of_no_request_do_not_hide_a_decoded_token():
     """As many rows as if every request brought the most: the last ones belong to none."""
     g = torch.Generator().manual_seed(9)
