@@ -58,17 +58,12 @@ constexpr float kSlack = 8.f;  // how far a score may pass the reference, in pow
 constexpr float kToLog2 = 1.4426950408889634f;
 
 template <typename T> constexpr int kTerms = std::is_same_v<T, float> ? 3 : 1;
-#ifndef LS_FP4_PROMPT_TILES
-#define LS_FP4_PROMPT_TILES 2
-#endif
-// Row tiles a wave holds where every wave has rows of its own: what its registers allow.
-template <typename T> constexpr int kPromptTiles = std::is_same_v<T, float> ? 1 : (D <= 128 ? LS_FP4_PROMPT_TILES : 1);
+// Row tiles a wave holds where every wave has rows of its own: what its registers allow (2 of 2,048 rows a head of 160 behind
+// 4,096 keys: one tile 752 us, two 498; heads of 128 with three or four tiles spill or leave one wave a SIMD).
+template <typename T> constexpr int kPromptTiles = std::is_same_v<T, float> ? 1 : (D <= 160 ? 2 : 1);
 
 // Waves a SIMD of the prompt kernel.
-#ifndef LS_FP4_PROMPT_WAVES
-#define LS_FP4_PROMPT_WAVES 2
-#endif
-template <typename T> constexpr int kPromptWaves = D <= 128 ? LS_FP4_PROMPT_WAVES : 1;
+template <typename T> constexpr int kPromptWaves = D <= 128 ? 2 : 1;
 
 // Keys a split of a request of few rows covers, by how many keys its rows see and how many heads do so: some 512 workgroups
 // a request at most, and no split too short to be worth its launch.  One split leaves out the second launch.  (8 requests of
@@ -82,7 +77,7 @@ __host__ __device__ inline int decode_split(int span, int kv_heads) {
   return max(shortest_split(span, kv_heads), (even + 127) / 128 * 128);
 }
 // The same for prompts, by how many workgroups its rows fill.
-constexpr int kPromptGroups = 256, kPromptShortest = 256;
+constexpr int kPromptGroups = 512, kPromptShortest = 256;
 __host__ __device__ inline int prompt_split(int span, int groups, int kv_heads) {
   const int want = max(1, kPromptGroups / (max(1, groups) * kv_heads));
   return max(kPromptShortest, ((span + want - 1) / want + 63) / 64 * 64);  // whole tiles of 64
@@ -103,9 +98,10 @@ struct Fp4Args {
   float factor;            // |scale| * log2(e)
   bool negative;           // the scale is: queries change their sign
   int window;
-  float* part_acc;         // [requests * kv heads][region][D]
-  float* part_ml;          // [requests * kv heads][region][2]
-  int region;
+  float* part_acc;         // [entries][D]: the sums of a row's split (see split_entry)
+  float* part_ml;          // [entries][2]: reference, sum of the weights
+  int region;              // entries a request's head, or (by_row) a query head of a row of q
+  bool by_row;
   int few;                 // rows a head up to which a request belongs to the decoding kernel
 };
 
@@ -127,6 +123,19 @@ struct Request {
     base = first_seen(start, a.window) & ~(kSharedKeys - 1);
   }
 };
+
+// Where the sums of a split of row r (of `stride` rows, padding included) of a head lie, -1 where there is no room.  By request
+// or by row of q, whichever takes less: prompts of one length lie close together by request, a prompt beside many decoded
+// tokens does by row.
+__device__ __forceinline__ long split_entry(const Fp4Args& a, const Request& rq, int b, int head, int split, int stride, int r) {
+  if (a.by_row) {
+    const int token = r / a.group;
+    const long row = (long)(rq.first + token) * a.pool.kv_heads * a.group + head * a.group + (r - token * a.group);
+    return split < a.region ? row * a.region + split : -1;
+  }
+  const long entry = (long)split * stride + r;
+  return entry < a.region ? ((long)b * a.pool.kv_heads + head) * a.region + entry : -1;
+}
 
 struct KeyTile {  // what a lane has of 32 keys and values, as they lie in the pages
   unsigned int k[2][D / 32];
@@ -624,9 +633,8 @@ __device__ __forceinline__ void decode_part(const Fp4Args& a, FoldShared& fold, 
       const int token = r / a.group, sub = r - token * a.group;
       store_run<T>(static_cast<T*>(a.out) + (long)(rq.first + token) * a.ldo + (long)(head * a.group + sub) * D + d, x, 4);
     } else {
-      const int entry = split * 16 + r;
-      if (entry < a.region) {
-        const long at = ((long)b * a.pool.kv_heads + head) * a.region + entry;
+      const long at = split_entry(a, rq, b, head, split, 16, r);
+      if (at >= 0) {
         store_run<float>(a.part_acc + at * D + d, x, 4);
         if (d == 0) {
           a.part_ml[2 * at] = top;
@@ -981,9 +989,8 @@ __device__ __forceinline__ void prompt_part(const Fp4Args& a, PromptShared& shar
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int token = there ? r / a.group : 0, sub = there ? r - token * a.group : 0;
     T* out = static_cast<T*>(a.out) + (long)(rq.first + token) * a.ldo + (long)(head * a.group + sub) * D;
-    const int entry = split * blocks * kBlock + r;
-    const bool keep = there && entry < a.region;
-    const long at = ((long)b * a.pool.kv_heads + head) * a.region + (keep ? entry : 0);
+    const long at = there ? split_entry(a, rq, b, head, split, blocks * kBlock, r) : -1;
+    const bool keep = at >= 0;
     if (splits > 1 && keep && j == 0) {
       a.part_ml[2 * at] = rows.m[t];
       a.part_ml[2 * at + 1] = l;
@@ -1047,10 +1054,10 @@ __global__ __launch_bounds__(kThreads) void fp4_combine_kernel(Fp4Args a) {  // 
   for (int place = kWaveEach ? 4 * blockIdx.x + w : blockIdx.x; place < pairs; place += stride_pairs) {
     const int token = place / heads, query_head = place - token * heads, row = rq.first + token;
     const int head = query_head / a.group, r = token * a.group + (query_head - head * a.group);
-    if ((long)(splits - 1) * stride + r >= a.region) return;
-    const long base = ((long)b * a.pool.kv_heads + head) * a.region + r;
+    const long base = split_entry(a, rq, b, head, 0, stride, r), apart = a.by_row ? 1 : stride;
+    if (split_entry(a, rq, b, head, splits - 1, stride, r) < 0) return;
     T* out = static_cast<T*>(a.out) + (long)row * a.ldo + (long)query_head * D;
-    const auto sum_at = [&](int s, int y) LS_INLINED -> float { return a.part_acc[(base + (long)s * stride) * D + min(d0 + y, D - 1)]; };
+    const auto sum_at = [&](int s, int y) LS_INLINED -> float { return a.part_acc[(base + s * apart) * D + min(d0 + y, D - 1)]; };
     // (asked for before the factors are known)
     float ahead[kWaveEach ? 4 : 1][kEach];
 #pragma unroll
@@ -1059,11 +1066,11 @@ __global__ __launch_bounds__(kThreads) void fp4_combine_kernel(Fp4Args a) {  // 
       for (int y = 0; y < kEach; ++y) ahead[k][y] = sum_at(min(kWaveEach ? k : w, splits - 1), y);
     // every wave the same: the largest reference, the factors, the sum of the weights
     float top = -INFINITY;
-    for (int s = lane; s < splits; s += 64) top = fmaxf(top, a.part_ml[2 * (base + (long)s * stride)]);
+    for (int s = lane; s < splits; s += 64) top = fmaxf(top, a.part_ml[2 * (base + s * apart)]);
     top = wave_max(top);
     const auto factor_of = [&](int s, float& l) LS_INLINED -> float {
-      const float m = a.part_ml[2 * (base + (long)s * stride)];
-      l = a.part_ml[2 * (base + (long)s * stride) + 1];
+      const float m = a.part_ml[2 * (base + s * apart)];
+      l = a.part_ml[2 * (base + s * apart) + 1];
       return m == -INFINITY ? l : weight_exp2<T>(m - top);  // (no score: 0, or NaN)
     };
     float sum = 0.f, l;
@@ -1116,14 +1123,14 @@ __global__ __launch_bounds__(kThreads) void fp4_combine_kernel(Fp4Args a) {  // 
 }
 
 struct Plan {
-  int few, decode_splits, prompt_places, region;  // places: row blocks of a workgroup times splits, of a request's head
+  int few, decode_splits, prompt_places, region, most_splits;  // places: row blocks of a workgroup times splits, of a request's head
 };
 
 // What is launched for requests of at most `most` tokens and `longest` keys: bounds for every shorter one.
 template <typename T>
 Plan make_plan(int kv_heads, int group, int most, int longest, int window) {
   constexpr int kGroupRows = 64 * kPromptTiles<T>;
-  Plan p{16, 1, 0, 0};
+  Plan p{16, 1, 0, 0, 1};
   // the keys that a request's rows see, at most: with a window those of its tokens and the window before, in whole tiles
   const auto seen = [&](int n) { return window > 0 ? (int)min((long)longest, (long)n + window - 1 + kSharedKeys) : longest; };
   const int span = seen(min(max(1, p.few / group), most));
@@ -1131,6 +1138,7 @@ Plan make_plan(int kv_heads, int group, int most, int longest, int window) {
     const auto most_of = [&](int n) { return (n + shortest_split(n, kv_heads) - 1) / shortest_split(n, kv_heads); };
     p.decode_splits = min(max(most_of(span), most_of(min(span, 4096))), (kDecodeGroups + kv_heads - 1) / kv_heads);
     p.region = 16 * p.decode_splits;
+    p.most_splits = p.decode_splits;
   }
   const long rows = (long)most * group;
   if (rows > p.few) {
@@ -1140,9 +1148,15 @@ Plan make_plan(int kv_heads, int group, int most, int longest, int window) {
     if (want > 1 && far > kPromptShortest) {
       p.prompt_places = (int)max((long)p.prompt_places, min((long)want, (long)p.prompt_places * ((far + kPromptShortest - 1) / kPromptShortest)));
       p.region = max(p.region, want * kGroupRows);
+      p.most_splits = max(p.most_splits, min(want, (far + kPromptShortest - 1) / kPromptShortest));
     }
   }
   return p;
+}
+
+// Splits' sums that a step may leave.
+inline long entries_of(const Plan& p, int kv_heads, int group, int requests, int rows) {
+  return p.region == 0 ? 0 : min((long)requests * kv_heads * p.region, (long)rows * kv_heads * group * p.most_splits);
 }
 
 template <typename T, bool kWholePages>
@@ -1157,11 +1171,12 @@ void launch_parts(const Fp4Args& a, const Plan& p, hipStream_t stream) {
 template <typename T>
 int run_fp4(Fp4Args& a, int most, int longest, void* scratch, long scratch_bytes, hipStream_t stream) {
   const Plan p = make_plan<T>(a.pool.kv_heads, a.group, most, longest, a.window);
-  a.few = p.few;
-  a.region = p.region;
   const int heads = a.pool.kv_heads;
+  a.few = p.few;
+  const long entries = entries_of(p, heads, a.group, a.requests, a.rows);
+  a.by_row = entries != (long)a.requests * heads * p.region;
+  a.region = a.by_row ? p.most_splits : p.region;
   LS_REQUIRE((long)p.prompt_places + p.decode_splits <= 65535, "fp4_attention: %d rows a request", most);
-  const long entries = (long)a.requests * heads * p.region;
   LS_REQUIRE(scratch_bytes >= entries * (D + 2) * (long)sizeof(float), "fp4_attention: %ld bytes of scratch, %ld needed",
              scratch_bytes, entries * (D + 2) * (long)sizeof(float));
   a.part_acc = static_cast<float*>(scratch);
@@ -1185,12 +1200,12 @@ LS_DEFINE_ERROR_API
 
 extern "C" int ls_fp4_attention_head_dim() { return ls::D; }
 
-extern "C" long ls_fp4_attention_scratch_bytes(int dtype, int requests, int kv_heads, int group, int most, int longest, int window) {
+extern "C" long ls_fp4_attention_scratch_bytes(int dtype, int rows, int requests, int kv_heads, int group, int most, int longest, int window) {
   using namespace ls;
-  if (requests <= 0 || kv_heads <= 0 || group <= 0 || most <= 0) return 0;
+  if (rows <= 0 || requests <= 0 || kv_heads <= 0 || group <= 0 || most <= 0) return 0;
   const Plan p = dtype == kF32 ? make_plan<float>(kv_heads, group, most, longest, window)
-                                : make_plan<bf16_t>(kv_heads, group, most, longest, window);
-  return (long)requests * kv_heads * p.region * (D + 2) * (long)sizeof(float);
+                               : make_plan<bf16_t>(kv_heads, group, most, longest, window);
+  return entries_of(p, kv_heads, group, requests, rows) * (D + 2) * (long)sizeof(float);
 }
 
 extern "C" int ls_fp4_attention(int dtype, const void* q, long ldq, void* out, long ldo, int rows, const void* k_codes,

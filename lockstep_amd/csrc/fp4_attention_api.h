@@ -11,7 +11,7 @@ int ls_fp4_attention_head_dim();
 
 // most, longest: the most rows and the most keys of any request (bounds; the device's numbers say what is computed).
 // scratch: ls_fp4_attention_scratch_bytes(...) bytes.
-long ls_fp4_attention_scratch_bytes(int dtype, int requests, int kv_heads, int group, int most, int longest, int window);
+long ls_fp4_attention_scratch_bytes(int dtype, int rows, int requests, int kv_heads, int group, int most, int longest, int window);
 int ls_fp4_attention(int dtype, const void* q, long ldq, void* out, long ldo, int rows, const void* k_codes,
                      const void* k_scales, const void* v_codes, const void* v_scales, int pages, int page_size, int kv_heads,
                      int group, const int* table, int columns, const int* offsets, const int* lengths, int requests,

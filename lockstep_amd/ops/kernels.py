@@ -2021,7 +2021,7 @@ class Kernels:
             lib.ls_last_error.restype = ctypes.c_char_p
             p, i, n = c_void_p, c_int, c_long
             lib.ls_fp4_attention_scratch_bytes.restype = c_long
-            lib.ls_fp4_attention_scratch_bytes.argtypes = [i, i, i, i, i, i, i]
+            lib.ls_fp4_attention_scratch_bytes.argtypes = [i, i, i, i, i, i, i, i]
             lib.ls_fp4_attention.argtypes = [i, p, n, p, n, i, p, p, p, p, i, i, i, i, p, i, p, p, i, i, i, c_float, i, p, n, p]
             if not (lib.ls_fp4_attention_head_dim() == head_dim):
                 raise KernelError(f"{path} was built for another head size")
@@ -2187,7 +2187,7 @@ class Kernels:
         code, group = DTYPE_CODE[q.dtype], nq // nkv
         if window >= max_length:
             window = 0                         # every row sees all keys before it
-        need = lib.ls_fp4_attention_scratch_bytes(code, requests, nkv, group, max_tokens, max_length, window)
+        need = lib.ls_fp4_attention_scratch_bytes(code, rows, requests, nkv, group, max_tokens, max_length, window)
         # (of the call's stream, and of the graph's own memory while one is captured: no two calls share it)
         scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
         self._launch_plain(lib, lib.ls_fp4_attention, (

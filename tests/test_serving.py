@@ -73,7 +73,7 @@ def test_the_plan_of_the_splits_covers_every_request():
         return 768 if span <= 768 else max(shortest(span, heads), (-(-span * heads // 512) + 127) // 128 * 128)
 
     def prompt_split(span, groups, heads):
-        want = max(1, 256 // (max(1, groups) * heads))
+        want = max(1, 512 // (max(1, groups) * heads))
         return max(256, ((span + want - 1) // want + 63) // 64 * 64)
 
     def planned(span, heads):
@@ -87,5 +87,5 @@ def test_the_plan_of_the_splits_covers_every_request():
             assert worst <= planned(span, heads) <= 512, (span, heads)
             for groups in (1, 2, 3, 5, 11, 16, 31, 32, 33, 500):
                 many = -(-span // prompt_split(span, groups, heads))
-                assert many <= max(1, min(256 // heads, -(-span // 256)))
-                assert groups * many <= max(1, 256 // heads) or many <= 1
+                assert many <= max(1, min(512 // heads, -(-span // 256)))
+                assert groups * many <= max(1, 512 // heads) or many <= 1

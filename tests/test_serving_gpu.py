@@ -266,6 +266,8 @@ SHAPES = [
     ([1500, 700], [40, 1], 2, 2, 128, 16, 400),
     ([70], [70], 40, 1, 32, 16, 0),
     ([30, 9], [1, 1], 40, 2, 64, 16, 0),
+    # many rows in several splits: their sums lie by request, not by row
+    ([2300], [2048], 4, 1, 32, 16, 0),
 ]
 
 
