@@ -9,9 +9,10 @@
 // lane takes vectors of 16 bytes, 64 vectors apart, and has its 32 logits in registers for the maximum first and the sums
 // then, so a piece costs one maximum and one rescaling a lane and the row is read once.  Everything is held a lane (m, S,
 // T) and a lane's pieces are folded in the order of a stream: piece i belongs to stream i mod 8.  Only at the end are a
-// stream's lanes folded (butterfly) and the streams after one another.  So the order of every sum depends on the row's
+// stream's lanes folded and the streams after one another.  So the order of every sum depends on the row's
 // length alone: with many rows a workgroup of eight waves takes a row, a wave a stream; with few rows every piece is a
-// wave of its own that leaves its lanes' (m, S, T), and a second launch folds them -- the same bits.
+// wave of its own that leaves its lanes' (m, S, T), and a second launch folds them; rows of one or two pieces, and many rows of
+// up to eight, go to a wave each -- the same bits.
 //
 // The alternatives come without a sort.  The lanes' maxima of every piece are kept; the k-th largest of 128 maxima over
 // disjoint parts of the row is a bound that the k first tokens reach (each of those parts holds one that does), and only
@@ -81,17 +82,17 @@ template <> struct Row<bf16_t> {
 };
 
 // The lane's 32 logits of a piece as floats; -inf behind the row's end.
-template <typename T>
+// VEC: neighbouring logits a lane has (1 where rows are so short that vectors would leave lanes without any).
+template <typename T, int VEC = Row<T>::VEC>
 __device__ __forceinline__ void load_piece(float (&x)[kLaneElems], const T* __restrict__ row, int piece, int vocab, int lane) {
-  constexpr int VEC = Row<T>::VEC;
   const int base = piece * kPiece;
-  if (base + kPiece <= vocab) {  // uniform
-    typename Row<T>::vec_t raw[kLaneElems / VEC];
+  if (VEC > 1 && base + kPiece <= vocab) {  // uniform
+    typename Row<T>::vec_t raw[kLaneElems / Row<T>::VEC];
 #pragma unroll
-    for (int i = 0; i < kLaneElems / VEC; ++i)
-      raw[i] = *reinterpret_cast<const typename Row<T>::vec_t*>(row + base + (i * 64 + lane) * VEC);
+    for (int i = 0; i < kLaneElems / Row<T>::VEC; ++i)
+      raw[i] = *reinterpret_cast<const typename Row<T>::vec_t*>(row + base + (i * 64 + lane) * Row<T>::VEC);
 #pragma unroll
-    for (int i = 0; i < kLaneElems / VEC; ++i)
+    for (int i = 0; i < kLaneElems / Row<T>::VEC; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if constexpr (sizeof(T) == 4) {
@@ -103,47 +104,76 @@ __device__ __forceinline__ void load_piece(float (&x)[kLaneElems], const T* __re
       }
   } else {
 #pragma unroll
-    for (int i = 0; i < kLaneElems; ++i) {
-      const int at = base + ((i / VEC) * 64 + lane) * VEC + i % VEC;
-      x[i] = at < vocab ? to_f32(row[min(at, vocab - 1)]) : -INFINITY;
-    }
+    for (int i = 0; i < kLaneElems / VEC; ++i)
+      if (base + i * 64 * VEC < vocab) {  // (uniform)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const int at = base + (i * 64 + lane) * VEC + e;
+          const float v = to_f32(row[min(at, vocab - 1)]);
+          x[i * VEC + e] = at < vocab ? v : -INFINITY;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[i * VEC + e] = -INFINITY;
+      }
   }
 }
 
 // The piece's sums of a lane, and (uniform) how many of the piece's tokens come before the token `given` of logit `mine`.
-template <typename T>
-__device__ __forceinline__ LaneSums piece_sums(const float (&x)[kLaneElems], int piece, int given, float mine, int& before, int lane) {
-  constexpr int VEC = Row<T>::VEC;
+// kWhole: the piece ends inside the row; else vectors behind the row's end are left out.
+template <typename T, bool kWhole, int VEC = Row<T>::VEC>
+__device__ __forceinline__ LaneSums piece_sums(const float (&x)[kLaneElems], int piece, int vocab, int given, float mine, int& before, int lane) {
+  constexpr int kVecs = kLaneElems / VEC;
+  const int base = piece * kPiece;
+  const auto here = [&](int v) LS_INLINED -> bool { return kWhole || base + v * 64 * VEC < vocab; };  // (uniform)
   LaneSums r;
   r.m = x[0];
 #pragma unroll
-  for (int i = 1; i < kLaneElems; ++i) r.m = fmaxf(r.m, x[i]);
+  for (int v = 0; v < kVecs; ++v)
+    if (here(v)) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) r.m = fmaxf(r.m, x[v * VEC + e]);
+    }
   const float ref = r.m == -INFINITY ? 0.f : r.m;
   r.s = 0.f;
   r.t = 0.f;
 #pragma unroll
-  for (int i = 0; i < kLaneElems; ++i) {
-    const float d = x[i] - ref;
-    const float e = __builtin_amdgcn_exp2f(d * kLog2e);
-    r.s = r.s + e;
-    r.t = fmaf(e, fmaxf(d, -1e4f), r.t);  // (a logit of -inf: 0 times a number)
-  }
-  // A NaN compares false with everything, so "not smaller" counts it as larger.
-  const int base = piece * kPiece;
-  if (base > given) {  // uniform: equal logits of this piece come later
+  for (int v = 0; v < kVecs; ++v)
+    if (here(v)) {
 #pragma unroll
-    for (int i = 0; i < kLaneElems; ++i) before += __popcll(__ballot(!(x[i] <= mine)));
-  } else if (base + kPiece <= given) {  // or before
-#pragma unroll
-    for (int i = 0; i < kLaneElems; ++i) before += __popcll(__ballot(!(x[i] < mine)));
-  } else {
-#pragma unroll
-    for (int i = 0; i < kLaneElems; ++i) {
-      const int at = base + ((i / VEC) * 64 + lane) * VEC + i % VEC;
-      before += __popcll(__ballot(at < given ? !(x[i] < mine) : !(x[i] <= mine)));
+      for (int e = 0; e < VEC; ++e) {
+        const float d = x[v * VEC + e] - ref;
+        const float w = __builtin_amdgcn_exp2f(d * kLog2e);
+        r.s = r.s + w;
+        r.t = fmaf(w, fmaxf(d, -1e4f), r.t);  // (a logit of -inf: 0 times a number)
+      }
     }
-  }
+  // A NaN compares false with everything, so "not smaller" counts it as larger.
+  const auto count = [&](auto comes_before) LS_INLINED {
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v)
+      if (here(v)) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) before += __popcll(__ballot(comes_before(x[v * VEC + e], base + (v * 64 + lane) * VEC + e)));
+      }
+  };
+  if (base > given) count([&](float l, int) LS_INLINED { return !(l <= mine); });  // (uniform) equal logits of this piece come later
+  else if (base + kPiece <= given) count([&](float l, int) LS_INLINED { return !(l < mine); });  // or before
+  else count([&](float l, int at) LS_INLINED { return at < given ? !(l < mine) : !(l <= mine); });
   return r;
+}
+
+template <typename T>
+__device__ __forceinline__ LaneSums sums_of_piece(const float (&x)[kLaneElems], int piece, int vocab, int given, float mine, int& before, int lane) {
+  if ((piece + 1) * kPiece <= vocab) return piece_sums<T, true>(x, piece, vocab, given, mine, before, lane);  // (uniform)
+  return piece_sums<T, false>(x, piece, vocab, given, mine, before, lane);
+}
+
+// The sums of the wave's lanes, the same in every lane.
+__device__ __forceinline__ LaneSums fold_lanes(const LaneSums& mine) {
+  const float m = wave_max(mine.m);
+  const float d = fmaxf(mine.m - m, -1e4f), f = __builtin_amdgcn_exp2f(d * kLog2e);  // (no logit yet: 0 times a number)
+  return LaneSums{m, wave_sum(mine.s * f), wave_sum(f * fmaf(mine.s, d, mine.t))};
 }
 
 struct FinishShared {
@@ -312,12 +342,7 @@ __device__ __forceinline__ void finish_row(FinishShared& sh, const float* __rest
                                            float* __restrict__ top_logprobs) {
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const float stream_max = mine.m;
-  // fold the lanes (butterfly: every lane the same bits)
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    LaneSums other{__shfl_xor(mine.m, off), __shfl_xor(mine.s, off), __shfl_xor(mine.t, off)};
-    mine = (lane & off) ? fold_sums(other, mine) : fold_sums(mine, other);
-  }
+  mine = fold_lanes(mine);
   if (lane == 0) {
     sh.m[w] = mine.m; sh.s[w] = mine.s; sh.t[w] = mine.t;
     sh.before[w] = before;
@@ -473,7 +498,7 @@ __global__ __launch_bounds__(kRowThreads, 8) void logprobs_rows_kernel(const T* 
   for (int p = w; p < pieces; p += kStreams) {
     float x[kLaneElems];
     load_piece<T>(x, row, p, vocab, lane);
-    const LaneSums here = piece_sums<T>(x, p, given, mine, before, lane);
+    const LaneSums here = piece_sums<T, true>(x, p, vocab, given, mine, before, lane);  // (-inf behind the row's end adds nothing)
     if (top > 0) set_max[p * 64 + lane] = here.m;
     sums = fold_sums(sums, here);
   }
@@ -497,7 +522,7 @@ __global__ __launch_bounds__(kPieceThreads) void logprobs_pieces_kernel(const T*
   const int given = tokens[r];
   const float mine = given >= 0 && given < vocab ? to_f32(row[given]) : 0.f;
   int before = 0;
-  const LaneSums here = piece_sums<T>(x, p, given, mine, before, lane);
+  const LaneSums here = sums_of_piece<T>(x, p, vocab, given, mine, before, lane);
   const long at = (long)r * pieces + p;
   part[at * 192 + lane] = here.m;
   part[at * 192 + 64 + lane] = here.s;
@@ -544,7 +569,188 @@ __global__ __launch_bounds__(kRowThreads, 4) void logprobs_fold_kernel(const T* 
                 top_logprobs);
 }
 
+// Short rows: a wave a row, four a workgroup; no wave waits for another.  The same sums (bits) as a workgroup a row, whose streams
+// have one piece at most there.  The bound is the k-th largest of the 64 lanes' maxima; the tokens that reach it are listed in
+// LDS, and a lane orders two of them.  (75,000 rows of 2,000 logits in float32: 526 us a workgroup each, 152 a wave each.)
+constexpr int kShortPieces = kStreams, kShortThreads = 256;
+constexpr int kNarrowVocab = 512;  // up to here a lane has single logits: vectors would leave lanes without any
+constexpr int kShortList = 128;
+struct ShortShared {
+  unsigned int key[kShortThreads / 64][kShortList];
+  int id[kShortThreads / 64][kShortList];
+  int sets[kShortThreads / 64][kShortList];
+};
+
+// Appends the tokens (in the order of their ids) for which `wanted(key)` holds to the wave's list; returns how many there are then,
+// kShortList + 1 where there are more than room.  `most`: how many are to be taken.
+template <typename T, typename F>
+__device__ __forceinline__ int list_in_order(ShortShared& sh, int w, int lane, const T* __restrict__ row, int vocab, int listed, int most, F wanted) {
+  const unsigned long long below = (1ull << lane) - 1ull;
+  const int until = listed + most;
+  for (int base = 0; base < vocab && listed < until; base += 64) {
+    const int id = base + lane;
+    const unsigned int key = logit_key(to_f32(row[min(id, vocab - 1)]));
+    const unsigned long long hit = __ballot(id < vocab && wanted(key));
+    const int at = listed + __popcll(hit & below);
+    if (((hit >> lane) & 1ull) && at < until && at < kShortList) {
+      sh.key[w][at] = key;
+      sh.id[w][at] = id;
+    }
+    listed = min(until, listed + __popcll(hit));
+  }
+  return min(listed, kShortList + 1);
+}
+
+// kPieces: the most pieces of a row (their lanes' maxima stay in registers).
+template <typename T, bool kNarrow, int kPieces>
+__global__ __launch_bounds__(kShortThreads) void logprobs_short_kernel(const T* __restrict__ logits, long ld, const int* __restrict__ tokens,
+                                                                       int rows, int vocab, int top, float* __restrict__ logprob,
+                                                                       float* __restrict__ entropy, int* __restrict__ rank,
+                                                                       int* __restrict__ top_ids, float* __restrict__ top_logprobs) {
+  __shared__ ShortShared sh;
+  constexpr int VEC = kNarrow ? 1 : Row<T>::VEC;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = blockIdx.x * (kShortThreads / 64) + w;
+  if (r >= rows) return;
+  const T* row = logits + (long)r * ld;
+  const int pieces = (vocab + kPiece - 1) / kPiece;
+  const int given = tokens[r];
+  const bool valid = given >= 0 && given < vocab;
+  const float given_logit = valid ? to_f32(row[given]) : 0.f;
+  LaneSums all{-INFINITY, 0.f, 0.f};
+  float set_max[kPieces], lane_max = -INFINITY;
+  int before = 0;
+#pragma unroll
+  for (int p = 0; p < kPieces; ++p) {
+    set_max[p] = -INFINITY;
+    if (p < pieces) {  // (uniform)
+      float x[kLaneElems];
+      load_piece<T, VEC>(x, row, p, vocab, lane);
+      const LaneSums here = kNarrow ? piece_sums<T, false, VEC>(x, p, vocab, given, given_logit, before, lane)
+                                    : sums_of_piece<T>(x, p, vocab, given, given_logit, before, lane);
+      set_max[p] = here.m;
+      lane_max = fmaxf(lane_max, here.m);
+      all = fold_sums(all, fold_lanes(here));
+    }
+  }
+  const float log_sum = logf(all.s);
+  if (valid && given_logit != given_logit) {  // (uniform) before a NaN come only the NaN of lower ids
+    before = 0;
+    for (int base = 0; base < given; base += 64) {
+      const float x = to_f32(row[min(base + lane, vocab - 1)]);
+      before += __popcll(__ballot(base + lane < given && x != x));
+    }
+  }
+  if (lane == 0) {
+    logprob[r] = valid ? (given_logit - all.m) - log_sum : __uint_as_float(0x7fc00000u);
+    entropy[r] = log_sum - all.t / all.s;
+    rank[r] = valid ? before : -1;
+  }
+  if (top == 0) return;
+
+  int listed = kShortList + 1;
+  unsigned int bound = 0u;
+  if (all.s == all.s && all.s != 0.f) {  // (uniform) finite logits but for -inf
+    if (top <= 12) {  // the largest again and again
+      float rest = lane_max;
+      for (int got = 0; got < top;) {
+        const float m = wave_max(rest);
+        const unsigned long long at = __ballot(rest == m);
+        got += __popcll(at);
+        bound = logit_key(m);
+        rest = rest == m ? -INFINITY : rest;
+        if (m == -INFINITY) break;
+      }
+    } else {
+      const unsigned int mine = logit_key(lane_max);
+      int larger = 0;
+#pragma unroll
+      for (int i = 0; i < 64; ++i) {
+        const unsigned int other = (unsigned int)__builtin_amdgcn_readlane((int)mine, i);
+        larger += other > mine || (other == mine && i < lane) ? 1 : 0;
+      }
+      bound = (unsigned int)__builtin_amdgcn_readlane((int)mine, __ffsll((long long)__ballot(larger == top - 1)) - 1);
+    }
+    const unsigned long long below = (1ull << lane) - 1ull;
+    int sets = 0;
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p)
+      if (p < pieces) {
+        const unsigned long long hit = __ballot(logit_key(set_max[p]) >= bound);
+        const int at = sets + __popcll(hit & below);
+        if (((hit >> lane) & 1ull) && at < kShortList) sh.sets[w][at] = p * 64 + lane;
+        sets += __popcll(hit);
+      }
+    if (sets <= kShortList) {
+      __builtin_amdgcn_wave_barrier();
+      listed = 0;
+      // two sets of 32 at a time; vectors behind the row's end do not count
+      for (int i = 0; i < sets * kLaneElems; i += 64) {
+        const int j = i + lane, set = sh.sets[w][min(j / kLaneElems, sets - 1)], e = j % kLaneElems;
+        const int id = (set >> 6) * kPiece + ((e / VEC) * 64 + (set & 63)) * VEC + e % VEC;
+        const bool inside = j < sets * kLaneElems && id < vocab;
+        if (__ballot(inside) == 0ull) continue;
+        const unsigned int key = logit_key(to_f32(row[inside ? id : 0]));
+        const unsigned long long hit = __ballot(inside && key >= bound);
+        const int at = listed + __popcll(hit & below);
+        if (((hit >> lane) & 1ull) && at < kShortList) {
+          sh.key[w][at] = key;
+          sh.id[w][at] = id;
+        }
+        listed += __popcll(hit);
+      }
+    }
+  }
+  if (listed > kShortList) {
+    // many tokens at the bound?  Those above it, and the first of the equal ones
+    const int above = bound == 0u ? kShortList + 1 : list_in_order<T>(sh, w, lane, row, vocab, 0, kShortList + 1, [&](unsigned int key) LS_INLINED { return key > bound; });
+    if (above > kShortList) {
+      // the k-th key bit by bit: the largest value that k keys reach
+      unsigned int value = 0u;
+      for (int bit = 31; bit >= 0; --bit) {
+        const unsigned int next = value | (1u << bit);
+        int n = 0;
+        for (int base = 0; base < vocab; base += 64) {
+          const int id = base + lane;
+          n += __popcll(__ballot(id < vocab && logit_key(to_f32(row[min(id, vocab - 1)])) >= next));
+        }
+        if (n >= top) value = next;
+      }
+      bound = value;
+      listed = list_in_order<T>(sh, w, lane, row, vocab, 0, kShortList + 1, [&](unsigned int key) LS_INLINED { return key > bound; });
+    } else {
+      listed = above;
+    }
+    if (listed < top)
+      listed = list_in_order<T>(sh, w, lane, row, vocab, listed, top - listed, [&](unsigned int key) LS_INLINED { return key == bound; });
+  }
+  __builtin_amdgcn_wave_barrier();
+  // their order: a token's place is how many of the others come before it
+  for (int c0 = 0; c0 < listed; c0 += 64) {  // (uniform)
+    const int c = min(c0 + lane, listed - 1);
+    const unsigned int key = sh.key[w][c];
+    const int id = sh.id[w][c];
+    int place = 0;
+#pragma unroll 8
+    for (int i = 0; i < listed; ++i) {
+      const unsigned int other = sh.key[w][i];
+      place += other > key || (other == key && sh.id[w][i] < id) ? 1 : 0;
+    }
+    if (c0 + lane < listed && place < top) {
+      top_ids[(long)r * top + place] = id;
+      top_logprobs[(long)r * top + place] = (key_logit(key) - all.m) - log_sum;
+    }
+  }
+}
+
 inline int logprob_pieces(int vocab) { return (vocab + kPiece - 1) / kPiece; }
+// Where a wave takes a row: always those of one or two pieces; of up to eight where the rows are many (10,000 logits in float32, 20
+// wanted: 512 rows 14.4 us a workgroup each, 20.9 a wave each; 1,024 rows 20.1 and 25.5, 2,048 rows 36.4 and 30.1, 15,000 rows 223
+// and 150).
+inline bool logprobs_short(int rows, int vocab) {
+  const int pieces = logprob_pieces(vocab);
+  return pieces <= 2 || (pieces <= kShortPieces && rows >= 1536);
+}
 // With fewer rows than compute units a workgroup a row leaves units idle; a wave a piece pays for its second launch once the
 // streams have more than two pieces (8 rows of 15,000 logits: 6.5 us by rows, 7.8 by pieces; of 60,000: 9.9 and 8.4).
 inline bool logprobs_by_pieces(int rows, int vocab) { return rows < compute_units() && logprob_pieces(vocab) > 2 * kStreams; }
@@ -555,7 +761,12 @@ int run_logprobs(const void* logits, long ld, const int* tokens, int rows, int v
   const int pieces = logprob_pieces(vocab);
   const size_t lds = top > 0 ? sizeof(float) * 64 * (size_t)pieces : 0;
   const T* x = static_cast<const T*>(logits);
-  if (logprobs_by_pieces(rows, vocab)) {
+  if (logprobs_short(rows, vocab)) {
+    const int waves = kShortThreads / 64;
+    (vocab <= kNarrowVocab ? logprobs_short_kernel<T, true, 1> : pieces <= 2 ? logprobs_short_kernel<T, false, 2>
+                                                                             : logprobs_short_kernel<T, false, kShortPieces>)<<<
+        (unsigned)((rows + (long)waves - 1) / waves), kShortThreads, 0, stream>>>(x, ld, tokens, rows, vocab, top, logprob, entropy, rank, top_ids, top_logprobs);
+  } else if (logprobs_by_pieces(rows, vocab)) {
     LS_REQUIRE(rows <= 65535, "token_logprobs: %d rows", rows);
     if (lds > 48 * 1024) {
       const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(logprobs_fold_kernel<T>),

@@ -454,7 +454,10 @@ def check_logprobs(logits, tokens, top):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,vocab,top", [(1, 1, 0), (1, 1, 1), (3, 2, 2), (2, 63, 5), (5, 100, 32), (2, 513, 32), (4, 2047, 20),
                                             (3, 2048, 1), (2, 2049, 32), (3, 4099, 7), (2, 50001, 20), (300, 700, 5), (260, 5003, 32),
-                                            (1, 151936, 20), (2, 300007, 32)])
+                                            (1, 151936, 20), (2, 300007, 32),
+                                            (3, 64, 32), (5, 65, 12), (4, 127, 13), (9, 256, 32), (7, 257, 20), (6, 512, 32),
+                                            (5, 515, 12), (6, 2050, 12), (3, 4096, 32), (5, 4097, 13), (1540, 4097, 32),
+                                            (1539, 8193, 12), (1537, 16384, 32), (3, 16384, 32), (1600, 16385, 5)])
 def test_logprobs(rows, vocab, top, dtype):
     g = torch.Generator().manual_seed(rows * vocab)
     wide = (2.5 * torch.randn((rows, vocab + 3), generator=g)).to(dtype).to(DEV)
@@ -464,9 +467,9 @@ def test_logprobs(rows, vocab, top, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("rows", [11, 280])
-def test_logprobs_of_odd_rows(rows, dtype):
-    vocab, top = 3001, 20
+@pytest.mark.parametrize("rows,vocab", [(11, 3001), (280, 3001), (11, 9001), (1540, 9001), (11, 40001), (280, 40001)])
+def test_logprobs_of_odd_rows(rows, vocab, dtype):
+    top = 20
     g = torch.Generator().manual_seed(rows)
     x = (2.5 * torch.randn((rows, vocab), generator=g)).to(dtype)
     inf = float("inf")
@@ -483,7 +486,8 @@ def test_logprobs_of_odd_rows(rows, dtype):
     x[9, 30] = float("nan"); x[9, 35] = float("nan"); x[9, 2000] = float("nan"); tokens[9] = 35
     x[10, 17] = 3e38; tokens[10] = 18              # one large logit
     check_logprobs(x.to(DEV), tokens, top)
-    check_logprobs(x.to(DEV)[:, :40], [t % 40 for t in tokens], 32)
+    for short in (40, 300, 515):
+        check_logprobs(x.to(DEV)[:64, :short], [t % short for t in tokens[:64]], 32)
 
 
 def test_tokens_outside_the_vocabulary():
@@ -494,9 +498,10 @@ def test_tokens_outside_the_vocabulary():
 
 def test_a_row_has_the_same_bits_beside_others():
     g = torch.Generator().manual_seed(12)
-    for dtype, vocab in ((torch.float32, 20011), (torch.bfloat16, 20011), (torch.float32, 50021), (torch.bfloat16, 50021)):
-        x = (2.5 * torch.randn((600, vocab), generator=g)).to(dtype).to(DEV)
-        tokens = torch.randint(0, vocab, (600,), generator=g).tolist()
+    for dtype, vocab, rows in ((torch.float32, 20011, 600), (torch.bfloat16, 20011, 600), (torch.float32, 50021, 600),
+                               (torch.bfloat16, 50021, 600), (torch.float32, 5003, 1600), (torch.bfloat16, 16381, 1600)):
+        x = (2.5 * torch.randn((rows, vocab), generator=g)).to(dtype).to(DEV)
+        tokens = torch.randint(0, vocab, (rows,), generator=g).tolist()
         many = run_logprobs(x, tokens, 5)
         for lo, hi in ((0, 1), (5, 22), (599, 600)):
             few = run_logprobs(x[lo:hi], tokens[lo:hi], 5)
