@@ -682,7 +682,9 @@ __global__ __launch_bounds__(kShortThreads) void logprobs_short_kernel(const T* 
         sets += __popcll(hit);
       }
     if (sets <= kShortList) {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
       listed = 0;
       // two sets of 32 at a time; vectors behind the row's end do not count
       for (int i = 0; i < sets * kLaneElems; i += 64) {
@@ -724,7 +726,9 @@ __global__ __launch_bounds__(kShortThreads) void logprobs_short_kernel(const T* 
     if (listed < top)
       listed = list_in_order<T>(sh, w, lane, row, vocab, listed, top - listed, [&](unsigned int key) LS_INLINED { return key == bound; });
   }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   // their order: a token's place is how many of the others come before it
   for (int c0 = 0; c0 < listed; c0 += 64) {  // (uniform)
     const int c = min(c0 + lane, listed - 1);
