@@ -21,12 +21,13 @@
 // own length (and rows) and of the heads alone; where there are several, they leave sums that a second launch folds.  So a
 // row's result does not depend on what else is in the step.
 //
-// What bounds it: decoding, the bytes (17/32 a key element): 4 requests of 131,071 keys are read at 5.3 TB/s, 64 of up to 8,192
-// at 4.1 with what their splits cost; some 6 vector instructions a key and lane column are two thirds of what that leaves
-// room for.  Prompts, the vector unit next to the matrix units: a tile of 16 rows by 32 keys has 16 products of 16 cycles and
-// some 60 vector instructions of 4, of them 8 exponentials of 16, and two waves a SIMD overlap them in part (830 TFLOP/s at
-// 8,192 keys in pages of 16 where a large product of the library reaches 1,190).  Two groups of waves a barrier apart, one at the
-// matrix and one at the vector units, were slower (885 us for 821: alone on its SIMD, a wave waits for its own results).
+// What bounds it: decoding, the bytes (17/32 a key element): 4 requests of 131,071 keys (32 heads over 8, 570 MB) are read in
+// 107 us, 5.3 TB/s, and their splits folded in 5; 64 of 1 to 8,192 (367 MB) take 84 and 5, 64 of 4,608 each (321 MB) 75 in all.
+// Some 6 vector instructions a key and lane column are two thirds of what that leaves room for.  Prompts, the vector unit next
+// to the matrix units: a tile of 16 rows by 32 keys has 16 products of 16 cycles and some 60 vector instructions of 4, of them
+// 8 exponentials of 16, and two waves a SIMD overlap them in part (6,660 rows of 32 heads behind up to 8,192 keys in pages of 16:
+// 770 us, 880 TFLOP/s, where a large product of the library reaches 1,190).  Two groups of waves a barrier apart, one at the matrix and
+// one at the vector units, were slower (885 us for 770: alone on its SIMD, a wave waits for its own results).
 
 #include "fp4.h"
 #include "fp4_attention_api.h"
