@@ -95,6 +95,7 @@ struct Fp4Args {
   const int* offsets;
   const int* lengths;
   int requests, rows;      // rows: of q and out
+  int most, longest;       // what the launches are sized for: a request of more rows is left out, a length counts as no more
   int group;               // query heads a key/value head
   float factor;            // |scale| * log2(e)
   bool negative;           // the scale is: queries change their sign
@@ -114,11 +115,11 @@ struct Request {
   int first, rows, start, base, end;  // first packed row, rows a head, first position, keys that are seen: base .. end - 1
   __device__ __forceinline__ Request(const Fp4Args& a, int b) {
     const int from = a.offsets[b], to = a.offsets[b + 1];
-    const bool ok = from >= 0 && to >= from && to <= a.rows;
+    const bool ok = from >= 0 && to >= from && to <= a.rows && to - from <= a.most;
     first = ok ? from : 0;
     const int n = ok ? to - from : 0;
     rows = n * a.group;
-    const int room = (int)min((long)a.columns << a.pool.page_shift, 0x7fff0000l);  // (a few tiles on stay below 2^31)
+    const int room = (int)min((long)a.columns << a.pool.page_shift, (long)a.longest);  // (a few tiles on stay below 2^31)
     end = min(max(a.lengths[b], 0), room);
     start = end - n;
     base = first_seen(start, a.window) & ~(kSharedKeys - 1);
@@ -1230,7 +1231,7 @@ extern "C" int ls_fp4_attention(int dtype, const void* q, long ldq, void* out, l
                    static_cast<const unsigned char*>(v_codes), static_cast<const unsigned char*>(v_scales), pages,
                    __builtin_ctz((unsigned)page_size), kv_heads};
   a.table = table; a.columns = columns; a.offsets = offsets; a.lengths = lengths; a.requests = requests; a.rows = rows;
-  a.group = group; a.window = window;
+  a.group = group; a.window = window; a.most = most; a.longest = longest;
   a.factor = fmaxf(fabsf(scale) * kToLog2, 1.1754944e-38f);  // (never 0: a masked score stays -inf times it)
   a.negative = scale < 0.f;
   return dtype == kF32 ? run_fp4<float>(a, most, longest, scratch, scratch_bytes, (hipStream_t)stream)

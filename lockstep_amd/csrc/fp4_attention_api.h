@@ -9,7 +9,7 @@ extern "C" {
 const char* ls_last_error();
 int ls_fp4_attention_head_dim();
 
-// most, longest: the most rows and the most keys of any request (bounds; the device's numbers say what is computed).
+// most, longest: the most rows and the most keys of any request (a request of more rows is left out, more keys count as the most).
 // scratch: ls_fp4_attention_scratch_bytes(...) bytes.
 long ls_fp4_attention_scratch_bytes(int dtype, int rows, int requests, int kv_heads, int group, int most, int longest, int window);
 int ls_fp4_attention(int dtype, const void* q, long ldq, void* out, long ldo, int rows, const void* k_codes,

@@ -165,7 +165,7 @@ inline int check_pages(const char* what, int dtype, int tokens, int kv_heads, in
   LS_REQUIRE(page_size >= 4 && (page_size & (page_size - 1)) == 0, "%s: pages of %d tokens", what, page_size);
   LS_REQUIRE(ldk >= 0 && ldv >= 0, "%s: row strides %ld, %ld", what, ldk, ldv);
   const long groups = ((tokens + 3l) / 4 * 4 * kv_heads * (dim / 8) + kPagesThreads - 1) / kPagesThreads;
-  LS_REQUIRE(groups <= 0x7fffffffl, "%s: %d tokens of %d heads", what, tokens, kv_heads);
+  LS_REQUIRE(groups * kPagesThreads <= 0xffffffffl, "%s: %d tokens of %d heads", what, tokens, kv_heads);  // (a grid's limit)
   return 0;
 }
 

@@ -765,11 +765,20 @@ int run_logprobs(const void* logits, long ld, const int* tokens, int rows, int v
   const int pieces = logprob_pieces(vocab);
   const size_t lds = top > 0 ? sizeof(float) * 64 * (size_t)pieces : 0;
   const T* x = static_cast<const T*>(logits);
+  // (a grid has less than 2^32 threads: rows in runs, of which all but absurd calls have one)
+  const auto in_runs = [&](int run, auto launch) {
+    for (long from = 0; from < rows; from += run)
+      launch(x + from * ld, tokens + from, (int)min((long)run, rows - from), logprob + from, entropy + from, rank + from,
+             top_ids + from * top, top_logprobs + from * top);
+  };
   if (logprobs_short(rows, vocab)) {
-    const int waves = kShortThreads / 64;
-    (vocab <= kNarrowVocab ? logprobs_short_kernel<T, true, 1> : pieces <= 2 ? logprobs_short_kernel<T, false, 2>
-                                                                             : logprobs_short_kernel<T, false, kShortPieces>)<<<
-        (unsigned)((rows + (long)waves - 1) / waves), kShortThreads, 0, stream>>>(x, ld, tokens, rows, vocab, top, logprob, entropy, rank, top_ids, top_logprobs);
+    in_runs(1 << 24, [&](const T* x, const int* tokens, int rows, float* logprob, float* entropy, int* rank, int* top_ids, float* top_logprobs) {
+      const int waves = kShortThreads / 64;
+      auto* kernel = vocab <= kNarrowVocab ? logprobs_short_kernel<T, true, 1> : pieces <= 2 ? logprobs_short_kernel<T, false, 2>
+                                                                                             : logprobs_short_kernel<T, false, kShortPieces>;
+      kernel<<<(rows + waves - 1) / waves, kShortThreads, 0, stream>>>(x, ld, tokens, rows, vocab, top, logprob, entropy, rank, top_ids,
+                                                                       top_logprobs);
+    });
   } else if (logprobs_by_pieces(rows, vocab)) {
     LS_REQUIRE(rows <= 65535, "token_logprobs: %d rows", rows);
     if (lds > 48 * 1024) {
@@ -790,8 +799,9 @@ int run_logprobs(const void* logits, long ld, const int* tokens, int rows, int v
                                                hipFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024 + 1024);
       LS_REQUIRE(e == hipSuccess, "token_logprobs: %s", hipGetErrorString(e));
     }
-    logprobs_rows_kernel<T><<<rows, kRowThreads, lds, stream>>>(x, ld, tokens, vocab, top, logprob, entropy, rank, top_ids,
-                                                               top_logprobs);
+    in_runs(1 << 22, [&](const T* x, const int* tokens, int rows, float* logprob, float* entropy, int* rank, int* top_ids, float* top_logprobs) {
+      logprobs_rows_kernel<T><<<rows, kRowThreads, lds, stream>>>(x, ld, tokens, vocab, top, logprob, entropy, rank, top_ids, top_logprobs);
+    });
   }
   return check_launch("token_logprobs");
 }

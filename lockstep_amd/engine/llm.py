@@ -58,8 +58,8 @@ def score(model: Model, token_ids: Sequence[int], top: int = 0, portion: int = 2
     n = len(token_ids)
     if n < 2:
         return []
-    if portion < 1:
-        raise ValueError(f"portions of {portion} tokens")
+    if portion < 1 or top < 0:
+        raise ValueError(f"portions of {portion} tokens, {top} alternatives")
     kernels, device = model.rt.kernels, model.rt.device
     cache = model.make_cache(num_pages=-(-n // page_size), page_size=page_size, max_requests=1, max_tokens_per_request=n)
     cache.open("score")

@@ -2046,6 +2046,15 @@ class Kernels:
             raise KernelError(f"{what}: operands on GPU {device}, the current device is {here}")
         return _raw_stream(here) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
+    def _call_scratch(self, need: int, like: torch.Tensor, what: str):
+        """``need`` bytes for one call: of its stream, and of the graph's own memory while one is captured, so that no two calls
+        share them.  Launches that are noted to be made again for other layers would outlive them."""
+        if not need:
+            return None
+        if self.tape is not None:
+            raise KernelError(f"{what} takes memory for the call: a part that calls it is not repeatable")
+        return torch.empty(need, dtype=torch.uint8, device=like.device)
+
     @staticmethod
     def _ints_refused(what: str, t, n, device: int) -> KernelError:
         return KernelError(f"{what} must be a contiguous int32 vector{'' if n is None else f' of {n}'} on GPU {device}, got "
@@ -2089,8 +2098,9 @@ class Kernels:
         if not (page_size >= 4 and page_size & (page_size - 1) == 0 and columns * page_size <= 0x7FFFFFFF):
             raise KernelError(f"step_tables: a page size is a power of two from 4 on, got {page_size}; positions have 31 bits")
         lib = self.serving
-        if requests > self._serving_limits[0]:
-            raise KernelError(f"step_tables takes at most {self._serving_limits[0]} requests, got {requests}")
+        if requests > self._serving_limits[0] or tokens > 0x7FFFFFFF or ins[2][1] > 4 * 0x7FFFFFFF:
+            raise KernelError(f"step_tables takes at most {self._serving_limits[0]} requests, got {requests} (tokens {tokens}, free pages "
+                              f"{free_pages.numel()}: 31 bits)")
         outs.append((table.data_ptr(), 4 * requests * columns))
         # an output may lie in no other operand: in the order of their addresses each begins behind all before
         end = written = 0
@@ -2108,9 +2118,9 @@ class Kernels:
         count, kv_heads, page_size, d = pages.geometry()
         device = pages.k_codes.get_device()
         stream = self._current(device, what)
-        if count * page_size > 0x7FFFFFFF:
-            raise KernelError(f"{what}: slots beyond 31 bits")
         shape = (slots.numel(), kv_heads * d)
+        if count * page_size > 0x7FFFFFFF or shape[0] > 0x7FFFFFFF:
+            raise KernelError(f"{what}: slots or tokens beyond 31 bits")
         for name, t in (("keys", k), ("values", v)):
             if not (t.dtype in DTYPE_CODE and t.dtype is k.dtype and t.get_device() == device and t.shape == shape
                     and t.stride(1) == 1 and t.stride(0) >= 0):
@@ -2136,7 +2146,7 @@ class Kernels:
         """The keys and values that the slots hold, as float32 or bfloat16 (both exact) rows ``[tokens, kv heads * d]``;
         rows whose slot is negative or beyond the pool stay as they are."""
         args = self._fp4_rows("fp4_read", k, v, slots, pages)
-        if not (args[6] <= 1 or (args[2] >= k.shape[1] and args[4] >= k.shape[1])):
+        if not ((args[6] <= 1 or (args[2] >= k.shape[1] and args[4] >= k.shape[1])) and (args[6] == 0 or args[1] != args[3])):
             raise KernelError("fp4_read: rows overlap")
         if args[6] == 0:
             return
@@ -2152,8 +2162,8 @@ class Kernels:
         ``offsets[i + 1] - 1``, the last of them at position ``lengths[i] - 1`` (its key and value are in the pages
         already); ``table [requests, columns]`` are the block tables (int32, as are offsets and lengths).  With a
         ``window`` a row sees that many keys, its own among them.  ``max_tokens`` and ``max_length``: the most rows and
-        the greatest length of any request; they size the launches, so rows or keys beyond them are not computed.  Rows
-        that belong to no request stay as they are; a row that sees no key (a length of 0, pages that the table does not
+        the greatest length of any request; they size the launches, so a request of more rows is left out (its rows stay as
+        they are) and a greater length counts as that one.  Rows that belong to no request stay as they are; a row that sees no key (a length of 0, pages that the table does not
         have) becomes zeros.  Keys whose page is negative or beyond the pool are not seen.  A row's result depends on its
         own request only, not on what else is in the step, but for the rounding between requests of at most 16 rows a
         key/value head and longer ones, which go through different kernels."""
@@ -2177,9 +2187,12 @@ class Kernels:
         for name, t, n in (("offsets", offsets, requests + 1), ("lengths", lengths, requests)):
             if not (t.dtype is torch.int32 and t.get_device() == device and t.dim() == 1 and t.numel() == n and t.is_contiguous()):
                 raise self._ints_refused(f"fp4_attention {name}", t, n, device)
-        if not (0 <= max_tokens and 0 <= max_length <= columns * page_size and window >= 0 and requests <= 65535 and nkv <= 1024):
-            raise KernelError(f"fp4_attention: at most {max_tokens} rows and {max_length} keys a request, window {window}, "
-                              f"{requests} requests with {columns} pages of {page_size}, {nkv} kv heads")
+        if not (0 <= max_tokens and 0 <= max_length <= columns * page_size and window >= 0 and requests <= 65535 and nkv <= 1024
+                and rows <= 0x7FFFFFFF and columns <= 0x7FFFFFFF and count <= 0x7FFFFFFF and -1e30 <= scale <= 1e30):
+            raise KernelError(f"fp4_attention: {rows} rows, at most {max_tokens} rows and {max_length} keys a request, window "
+                              f"{window}, {requests} requests with {columns} of {count} pages of {page_size}, {nkv} kv heads, scale {scale}")
+        if q.data_ptr() == out.data_ptr() and rows:
+            raise KernelError("fp4_attention: q and out are the same rows")
         max_tokens = min(max_tokens, rows)
         if max_tokens == 0 or requests == 0:
             return
@@ -2188,8 +2201,7 @@ class Kernels:
         if window >= max_length:
             window = 0                         # every row sees all keys before it
         need = lib.ls_fp4_attention_scratch_bytes(code, rows, requests, nkv, group, max_tokens, max_length, window)
-        # (of the call's stream, and of the graph's own memory while one is captured: no two calls share it)
-        scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        scratch = self._call_scratch(need, q, "fp4_attention")
         self._launch_plain(lib, lib.ls_fp4_attention, (
             code, q.data_ptr(), ldq, out.data_ptr(), ldo, rows, *(t.data_ptr() for t in pages), count, page_size, nkv, group,
             table.data_ptr(), columns, offsets.data_ptr(), lengths.data_ptr(), requests, max_tokens, max_length, scale, window,
@@ -2227,10 +2239,10 @@ class Kernels:
                               f"on GPU {device}, got {top_ids.dtype} {list(shape)} and {top_logprobs.dtype} {list(top_logprobs.shape)}")
         if rows == 0:
             return
-        if not (1 <= vocab <= widest):
-            raise KernelError(f"token_logprobs takes 1 to {widest} logits a row, got {vocab}")
+        if not (1 <= vocab <= widest and rows <= 0x7FFFFFFF):
+            raise KernelError(f"token_logprobs takes 1 to {widest} logits a row and 31 bits of rows, got {rows} of {vocab}")
         need = lib.ls_logprobs_scratch_bytes(rows, vocab)
-        scratch = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+        scratch = self._call_scratch(need, logits, "token_logprobs")
         self._launch_plain(lib, lib.ls_token_logprobs, (
             DTYPE_CODE[logits.dtype], logits.data_ptr(), ld, tokens.data_ptr(), rows, vocab, shape[1], logprob.data_ptr(),
             entropy.data_ptr(), rank.data_ptr(), top_ids.data_ptr(), top_logprobs.data_ptr(), scratch.data_ptr() if need else 0,

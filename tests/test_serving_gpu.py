@@ -188,6 +188,8 @@ def test_page_refusals():
     one = torch.zeros((1, 128), device=DEV)
     with pytest.raises(KernelError, match="overlap"):
         k.fp4_read(pool, s, one.expand(3, 128), x)
+    with pytest.raises(KernelError, match="overlap"):
+        k.fp4_read(pool, s, x, x)
     torch.cuda.synchronize()
 
 
@@ -370,6 +372,28 @@ def test_offsets_and_lengths_that_do_not_fit():
     assert not out[:3].any() and bool(out[3:].any())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads", [4, 64])
+def test_more_rows_or_keys_than_stated(heads, dtype):
+    """A request of more rows than stated is left out, also where the fold of splits would find its rows; a greater length counts as
+    the greatest one."""
+    g = torch.Generator().manual_seed(14)
+    lengths, news = [2000, 900, 1300, 5000], [1, 40, 2, 1]
+    pool, table = make_cache(g, lengths, 2, 64, 16)
+    offsets = [0, 1, 41, 43, 44]
+    q = torch.randn((44, heads * 64), generator=g).to(dtype).to(DEV)
+    for most in (1, 2):
+        out = run_attention(q, heads, 2, 64, pool, table, offsets, lengths, 0, most=most, longest=2100)
+        left = [i for i, n in enumerate(news) if n > most]
+        for i in left:
+            assert bool((out[offsets[i]:offsets[i + 1]] == 9).all()), i
+        for i in set(range(4)) - set(left):
+            check_attention(out[offsets[i]:offsets[i + 1]], q[offsets[i]:offsets[i + 1]], heads, 2, 64, pool, [table[i]], [0, news[i]],
+                            [min(lengths[i], 2100)], 16, 0)
+    out = run_attention(q, heads, 2, 64, pool, table, offsets, lengths, 0, most=40, longest=950)
+    check_attention(out, q, heads, 2, 64, pool, table, offsets, [min(n, 950) for n in lengths], 16, 0)
+
+
 @pytest.mark.parametrize("news", [1, 30])
 def test_windows_as_wide_as_the_context(news):
     g = torch.Generator().manual_seed(10)
@@ -416,9 +440,32 @@ def test_attention_refusals():
     k.fp4_attention(**base)
     for change in (dict(nq=5), dict(nkv=1), dict(d=32), dict(q=base["q"].half()), dict(out=base["out"].bfloat16()), dict(q=base["q"][:, :128]),
                    dict(out=base["out"][:2]), dict(offsets=i32([0, 3])), dict(lengths=i32([5])), dict(max_length=33), dict(window=-1),
-                   dict(table=base["table"].long()), dict(table=base["table"][0]), dict(out=base["out"][:1].expand(3, 256)), dict(max_tokens=-1)):
+                   dict(table=base["table"].long()), dict(table=base["table"][0]), dict(out=base["out"][:1].expand(3, 256)), dict(max_tokens=-1),
+                   dict(scale=float("nan")), dict(scale=float("inf")), dict(out=base["q"])):
         with pytest.raises(KernelError):
             k.fp4_attention(**{**base, **change})
+    torch.cuda.synchronize()
+
+
+def test_no_memory_of_a_call_in_noted_launches():
+    """Launches that are noted to be made again would use a call's memory after its end; those without any may be noted."""
+    k = kernels()
+    pool = Fp4Pages.empty(100, 2, 16, 64, device=DEV)
+    table = torch.zeros((1, 100), dtype=torch.int32, device=DEV)
+    q, out = torch.zeros((1, 256), device=DEV), torch.zeros((1, 256), device=DEV)
+    f, i = (lambda *s: torch.zeros(s, device=DEV)), (lambda *s: torch.zeros(s, dtype=torch.int32, device=DEV))
+    try:
+        k.tape = []
+        k.fp4_attention(q, 4, 2, 64, pool, table, i32([0, 1]), i32([40]), 1, 40, out, 0.1)
+        k.token_logprobs(f(2, 400), i(2), f(2), f(2), i(2), i(2, 1), f(2, 1))
+        assert len(k.tape) == 2
+        with pytest.raises(KernelError, match="repeatable"):
+            k.fp4_attention(q, 4, 2, 64, pool, table, i32([0, 1]), i32([1600]), 1, 1600, out, 0.1)
+        with pytest.raises(KernelError, match="repeatable"):
+            k.token_logprobs(f(2, 60000), i(2), f(2), f(2), i(2), i(2, 1), f(2, 1))
+        assert len(k.tape) == 2
+    finally:
+        k.tape = None
     torch.cuda.synchronize()
 
 
@@ -507,6 +554,21 @@ def test_a_row_has_the_same_bits_beside_others():
             few = run_logprobs(x[lo:hi], tokens[lo:hi], 5)
             for name in few:
                 assert torch.equal(few[name], many[name][lo:hi]), name
+
+
+@pytest.mark.parametrize("rows,vocab,top", [((1 << 24) + 5, 3, 1), ((1 << 22) + 3, 16385, 0)])
+def test_more_rows_than_a_launch_takes(rows, vocab, top):
+    g = torch.Generator().manual_seed(15)
+    some = torch.randn((1 if top == 0 else 64, vocab), generator=g).bfloat16().to(DEV)
+    logits = some.expand(rows, vocab) if top == 0 else some[torch.arange(rows, device=DEV) % 64]
+    f = lambda *s: torch.full(s, 9.0, device=DEV)  # noqa: E731
+    i = lambda *s: torch.full(s, 9, dtype=torch.int32, device=DEV)  # noqa: E731
+    out = [f(rows), f(rows), i(rows), i(rows, top), f(rows, top)]
+    kernels().token_logprobs(logits, torch.ones(rows, dtype=torch.int32, device=DEV), *out)
+    few = run_logprobs(some, [1] * len(some), top)
+    for x, one in zip(out, few.values()):
+        whole = rows // len(some) * len(some)
+        assert bool((x[:whole].view(rows // len(some), *one.shape) == one).all()) and torch.equal(x[whole:], one[:rows - whole])
 
 
 def test_logprobs_refusals():
