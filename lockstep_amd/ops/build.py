@@ -24,6 +24,8 @@ Two kinds of library exist:
                     probabilities of given tokens;
 ``fp4attention<D>`` attention over pages of keys and values in 4 bits for one head
                     size ``D``;
+``calls``           (a Python extension module of host code) checks and launches the
+                    entry points of the two above without Python's part of it;
 ``experts``         routing of tokens to a few of many small feed-forward experts
                     and the grouped products of those experts.
 
@@ -43,6 +45,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 import threading
 import time
@@ -131,7 +134,7 @@ def _run(cmd, what: str) -> None:
         env["HOME"] = tempfile.gettempdir()
     proc = subprocess.run(cmd, capture_output=True, text=True, env=env)
     if proc.returncode != 0:
-        raise BuildError(f"hipcc failed for {what}:\n{' '.join(cmd)}\n{proc.stderr[-4000:]}")
+        raise BuildError(f"{Path(cmd[0]).name} failed for {what}:\n{' '.join(cmd)}\n{proc.stderr[-4000:]}")
 
 
 def _compile(kind: str, sources, defines, out: Path) -> None:
@@ -259,6 +262,48 @@ def build_fp4_attention(head_dim: int, force: bool = False) -> Path:
     return build(f"fp4attention{head_dim}", FP4_ATTENTION_SOURCES, (f"-DLS_HEAD_DIM={head_dim}",), force)
 
 
+CALLS_SOURCE = "checked_calls.cpp"
+
+
+def build_calls(force: bool = False) -> Path:
+    """The extension module ``lockstep_calls`` (host code), for the torch and the Python that run."""
+    import torch
+
+    torch_dir = Path(torch.__file__).resolve().parent
+    include = torch_dir / "include"
+    flags = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    where = [f"-I{include}", f"-I{include / 'torch' / 'csrc' / 'api' / 'include'}", f"-I{sysconfig.get_paths()['include']}",
+             f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    version = (torch.__version__, sys.implementation.cache_tag, *flags)
+    name = f"lockstep_calls-{_hash((CALLS_SOURCE,), version)}.so"
+    if not force:
+        for folder in lib_dirs():
+            if (folder / name).is_file():
+                return folder / name
+    compiler = next((c for c in (os.environ.get("CXX"), shutil.which("g++"), shutil.which("c++")) if c and Path(c).is_file()), None)
+    if compiler is None:
+        raise BuildError("no C++ compiler was found (looked at $CXX, g++ and c++); the checked calls cannot be built")
+    for folder in lib_dirs():
+        if not _writable(folder):
+            continue
+        for stale in folder.glob("lockstep_calls-*.so"):
+            if stale.name != name:
+                try:
+                    stale.unlink()
+                except OSError:
+                    pass
+        tmp = folder / f".{name}.{os.getpid()}.{threading.get_ident()}.tmp"
+        try:
+            _run([compiler, *flags, str(CSRC / CALLS_SOURCE), "-o", str(tmp), *where], "the checked calls")
+            os.replace(tmp, folder / name)
+        finally:
+            if tmp.exists():
+                tmp.unlink()
+        return folder / name
+    raise BuildError(f"no writable folder for the checked calls among {[str(d) for d in lib_dirs()]}")
+
+
 MUTANT_DEFINE = "-DLS_MUTANTS"
 
 
@@ -290,11 +335,11 @@ def build_all(head_dims=DEFAULT_HEAD_DIMS, force: bool = True, mutants: bool = T
               fp4_head_dims=DEFAULT_FP4_HEAD_DIMS) -> list[Path]:
     """Compile the core library, the mixers library, the attention library of each head size and the
     talking-heads attention library of each shape, the sink attention
-    library of each key and value size, the experts and the serving library and attention over pages in 4 bits for each of
-    its head sizes, a few at a time; with ``mutants`` also the control
+    library of each key and value size, the experts and the serving library, the checked calls and attention over pages in 4 bits for each
+    of its head sizes, a few at a time; with ``mutants`` also the control
     libraries of the tests."""
     jobs = [lambda: build_core(force), lambda: build_mixers(force), lambda: build_experts(force)]
-    jobs += [lambda: build_serving(force)] + [lambda d=d: build_fp4_attention(d, force) for d in fp4_head_dims]
+    jobs += [lambda: build_serving(force), lambda: build_calls(force)] + [lambda d=d: build_fp4_attention(d, force) for d in fp4_head_dims]
     jobs += [lambda shape=shape: build_sink(*shape, force) for shape in sink_shapes]
     jobs += [lambda d=d: build_attention(d, force) for d in head_dims]
     jobs += [lambda shape=shape: build_talking(*shape, force) for shape in talking_shapes]

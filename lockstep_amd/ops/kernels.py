@@ -11,6 +11,7 @@ constructor raises.
 from __future__ import annotations
 
 import ctypes
+import sys
 from ctypes import c_float, c_int, c_long, c_void_p
 from typing import NamedTuple
 
@@ -64,6 +65,25 @@ def _rows_ok(t: torch.Tensor, name: str) -> None:
     if not (t.is_cuda and t.dim() == 2 and t.stride(1) == 1):
         raise KernelError(f"{name} must be 2-D with contiguous rows on the GPU, got shape {tuple(t.shape)} "
                           f"strides {t.stride()} on {t.device}")
+
+
+def _load_calls():
+    """The extension module of checked calls, or None where it cannot be built (Python's checks do without it)."""
+    from importlib.machinery import ExtensionFileLoader
+    from importlib.util import module_from_spec, spec_from_loader
+
+    try:
+        loader = ExtensionFileLoader("lockstep_calls", str(_build.build_calls()))
+        module = module_from_spec(spec_from_loader("lockstep_calls", loader))
+        loader.exec_module(module)
+        return module
+    except (_build.BuildError, ImportError) as exc:
+        print(f"[lockstep_amd] calls go through Python's checks: {exc}", file=sys.stderr, flush=True)
+        return None
+
+
+def _address(entry) -> int:
+    return ctypes.cast(entry, c_void_p).value
 
 
 class Fp4Pages(NamedTuple):
@@ -136,6 +156,7 @@ class Kernels:
         self.experts_path = None
         self._serving = None
         self.serving_path = None
+        self._calls = None
         self._fp4_attention: dict[int, ctypes.CDLL] = {}
         self.fp4_attention_paths: dict[int, str] = {}
         self._argmax_scratch: dict = {}
@@ -1993,7 +2014,9 @@ class Kernels:
             c_int(parts), _ptr(weight), c_float(eps), _ptr(out), c_long(out.stride(0)), _stream()))
 
     # -- around a step: tables, pages in 4 bits, log probabilities -------------------------
-    # (Checked and launched with plain numbers: with one launch a call, the host's part is what a small call costs.)
+    # With one launch a call, the host's part is what a small call costs.  So once its library is loaded a call goes through the
+    # extension module first (csrc/checked_calls.cpp: a quarter of the time), which launches what it finds in order; what it does
+    # not accept, and launches that are noted, come to the checks here, with plain numbers all the same.
     @property
     def serving(self):
         if self._serving is None:
@@ -2011,6 +2034,11 @@ class Kernels:
             self.serving_path = str(path)
             self._serving_limits = (int(lib.ls_step_tables_max_requests()), int(lib.ls_logprobs_max_top()),
                                     int(lib.ls_logprobs_max_vocab()))
+            if _raw_stream is not None and _raw_device is not None and torch.cuda.is_available():
+                self._calls = _load_calls()
+                if self._calls is not None:
+                    entries = (lib.ls_step_tables, lib.ls_fp4_write, lib.ls_fp4_read, lib.ls_token_logprobs, lib.ls_logprobs_scratch_bytes)
+                    self._calls.bind_serving(*map(_address, entries), *self._serving_limits)
         return self._serving
 
     def fp4_attention_lib(self, head_dim: int):
@@ -2027,6 +2055,9 @@ class Kernels:
                 raise KernelError(f"{path} was built for another head size")
             self._fp4_attention[head_dim] = lib
             self.fp4_attention_paths[head_dim] = str(path)
+            self.serving                        # (loads the extension module)
+            if self._calls is not None:
+                self._calls.bind_attention(head_dim, _address(lib.ls_fp4_attention), _address(lib.ls_fp4_attention_scratch_bytes))
         return lib
 
     def _launch_plain(self, lib, entry, args: tuple) -> None:
@@ -2077,6 +2108,11 @@ class Kernels:
         A request is refused (it brings no tokens and gets no pages) if its numbers are negative or exceed its row of the
         table; and from the first request on for which the free list, or the room of ``slots``, does not suffice, every
         later one that needs a page (brings a token).  Inputs and outputs must not overlap."""
+        calls = self._calls
+        if calls is not None and self.tape is None and calls.step_tables(
+                here := _raw_device(), _raw_stream(here), lengths, news, table, page_size, free_pages, cursor, slots, tok_seq, tok_pos,
+                offsets, new_lengths, progress):
+            return
         device = lengths.get_device()
         stream = self._current(device, "step_tables")
         requests, tokens = lengths.numel(), slots.numel()
@@ -2136,6 +2172,9 @@ class Kernels:
         bits into the slots (page * page size + place in the page) of ``pages``; a token whose slot is negative or
         beyond the pool is left out.  Every group of 32 elements gets a power of two as its scale; a group with an
         infinity or a NaN is held as NaN.  The slots of a call are distinct: of two tokens with one slot a mix remains."""
+        calls = self._calls
+        if calls is not None and self.tape is None and calls.fp4_write(here := _raw_device(), _raw_stream(here), k, v, slots, pages):
+            return
         args = self._fp4_rows("fp4_write", k, v, slots, pages)
         if args[6] == 0:
             return
@@ -2145,6 +2184,9 @@ class Kernels:
     def fp4_read(self, pages: Fp4Pages, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
         """The keys and values that the slots hold, as float32 or bfloat16 (both exact) rows ``[tokens, kv heads * d]``;
         rows whose slot is negative or beyond the pool stay as they are."""
+        calls = self._calls
+        if calls is not None and self.tape is None and calls.fp4_read(here := _raw_device(), _raw_stream(here), k, v, slots, pages):
+            return
         args = self._fp4_rows("fp4_read", k, v, slots, pages)
         if not ((args[6] <= 1 or (args[2] >= k.shape[1] and args[4] >= k.shape[1])) and (args[6] == 0 or args[1] != args[3])):
             raise KernelError("fp4_read: rows overlap")
@@ -2167,6 +2209,11 @@ class Kernels:
         have) becomes zeros.  Keys whose page is negative or beyond the pool are not seen.  A row's result depends on its
         own request only, not on what else is in the step, but for the rounding between requests of at most 16 rows a
         key/value head and longer ones, which go through different kernels."""
+        calls = self._calls
+        if calls is not None and self.tape is None and calls.fp4_attention(
+                here := _raw_device(), _raw_stream(here), q, nq, nkv, d, pages, table, offsets, lengths, max_tokens, max_length, out,
+                scale, window):
+            return
         count, kv_heads, page_size, dim = pages.geometry()
         device = q.get_device()
         stream = self._current(device, "fp4_attention")
@@ -2216,6 +2263,10 @@ class Kernels:
 
         A token outside the vocabulary (-1: none) gets NaN and the rank -1.  A NaN counts as larger than every number; rows
         with a NaN, with an infinity of +, or with nothing but -inf have NaN for what the formula leaves undefined."""
+        calls = self._calls
+        if calls is not None and self.tape is None and calls.token_logprobs(
+                here := _raw_device(), _raw_stream(here), logits, tokens, logprob, entropy, rank, top_ids, top_logprobs):
+            return
         device = logits.get_device()
         stream = self._current(device, "token_logprobs logits")
         _rows_ok(logits, "token_logprobs logits")

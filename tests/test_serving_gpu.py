@@ -586,6 +586,60 @@ def test_logprobs_refusals():
     torch.cuda.synchronize()
 
 
+# -- the two ways of a call ------------------------------------------------------------------------------------------------
+def test_calls_by_the_module_and_by_python():
+    """What the extension module accepts, it launches as Python does; what it does not accept, it leaves alone."""
+    k = kernels()
+    g = torch.Generator().manual_seed(16)
+    make = lambda dtype, *s: torch.full(s, 9, dtype=dtype, device=DEV)  # noqa: E731
+    ints = lambda *s: make(torch.int32, *s)  # noqa: E731
+    kv = torch.randn((2, 9, 128), generator=g).to(DEV)
+    q = torch.randn((9, 256), generator=g).to(DEV)
+    logits = torch.randn((3, 70000), generator=g).to(DEV)
+
+    def pass_over():
+        pool = Fp4Pages.empty(120, 2, 16, 64, device=DEV)
+        table = torch.full((2, 60), -1, dtype=torch.int32, device=DEV)
+        table[0, :55] = torch.arange(55, dtype=torch.int32, device=DEV)
+        tables = [ints(9), ints(9), ints(9), ints(3), ints(2), ints(2)]
+        read = [make(torch.bfloat16, 9, 128), make(torch.bfloat16, 9, 128)]
+        out, scores = make(torch.float32, 9, 256), [make(torch.float32, 3), make(torch.float32, 3), ints(3), ints(3, 4), make(torch.float32, 3, 4)]
+        calls = [("step_tables", (i32([870, 0]), i32([1, 8]), table, 16, i32(list(range(60, 80))), i32([3]), *tables)),
+                 ("fp4_write", (kv[0], kv[1], tables[0], pool)), ("fp4_read", None),
+                 ("fp4_attention", (q, 4, 2, 64, pool, table, tables[3], tables[4], 8, 871, out, 0.125, 0)),
+                 ("token_logprobs", (logits, i32([5, -1, 69999]), *scores))]
+        for name, args in calls:
+            if name == "fp4_read":
+                args = (pool, tables[0], *read)
+            getattr(k, name)(*args)
+        torch.cuda.synchronize()
+        calls[2] = ("fp4_read", (read[0], read[1], tables[0], pool))
+        return calls, [table, *tables, *pool, *read, out, *scores]
+
+    k.serving, k.fp4_attention_lib(64)
+    assert k._calls is not None
+    calls, by_module = pass_over()
+    here, stream = torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream
+    for name, args in calls:
+        entry = getattr(k._calls, name)
+        assert entry(here, stream, *args) is True, name
+        for i, x in enumerate(args):            # another device, another type, not a tensor, one operand less
+            if torch.is_tensor(x):
+                assert entry(here, stream, *args[:i], x.cpu(), *args[i + 1:]) is False, (name, i)
+                assert entry(here, stream, *args[:i], x.double(), *args[i + 1:]) is False, (name, i)
+                assert entry(here, stream, *args[:i], None, *args[i + 1:]) is False, (name, i)
+        assert entry(here + 1, stream, *args) is False and entry(here, stream, *args[:-1]) is False, name
+    torch.cuda.synchronize()
+    module, k._calls = k._calls, None
+    try:
+        _, by_python = pass_over()
+    finally:
+        k._calls = module
+    for i, (a, b) in enumerate(zip(by_module, by_python)):
+        # (step_tables ran twice on the first pass's table, with the same result)
+        assert torch.equal(a.view(torch.uint8) if a.is_floating_point() else a, b.view(torch.uint8) if b.is_floating_point() else b), i
+
+
 # -- together ---------------------------------------------------------------------------------------------------------------
 class Serving:
     """A small decoder's serving state: a linear model of keys, values, queries and logits from token ids."""
