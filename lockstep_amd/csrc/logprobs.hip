@@ -82,9 +82,9 @@ template <> struct Row<bf16_t> {
 };
 
 // The lane's 32 logits of a piece as floats; -inf behind the row's end.
-// VEC: neighbouring logits a lane has (1 where rows are so short that vectors would leave lanes without any).
-template <typename T, int VEC = Row<T>::VEC>
-__device__ __forceinline__ void load_piece(float (&x)[kLaneElems], const T* __restrict__ row, int piece, int vocab, int lane) {
+// VEC: neighbouring logits a lane has (1 where rows are so short that vectors would leave lanes without any); kElems: how many in all.
+template <typename T, int VEC = Row<T>::VEC, int kElems = kLaneElems>
+__device__ __forceinline__ void load_piece(float (&x)[kElems], const T* __restrict__ row, int piece, int vocab, int lane) {
   const int base = piece * kPiece;
   if (VEC > 1 && base + kPiece <= vocab) {  // uniform
     typename Row<T>::vec_t raw[kLaneElems / Row<T>::VEC];
@@ -104,7 +104,7 @@ __device__ __forceinline__ void load_piece(float (&x)[kLaneElems], const T* __re
       }
   } else {
 #pragma unroll
-    for (int i = 0; i < kLaneElems / VEC; ++i)
+    for (int i = 0; i < kElems / VEC; ++i)
       if (base + i * 64 * VEC < vocab) {  // (uniform)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
@@ -121,9 +121,9 @@ __device__ __forceinline__ void load_piece(float (&x)[kLaneElems], const T* __re
 
 // The piece's sums of a lane, and (uniform) how many of the piece's tokens come before the token `given` of logit `mine`.
 // kWhole: the piece ends inside the row; else vectors behind the row's end are left out.
-template <typename T, bool kWhole, int VEC = Row<T>::VEC>
-__device__ __forceinline__ LaneSums piece_sums(const float (&x)[kLaneElems], int piece, int vocab, int given, float mine, int& before, int lane) {
-  constexpr int kVecs = kLaneElems / VEC;
+template <typename T, bool kWhole, int VEC = Row<T>::VEC, int kElems = kLaneElems>
+__device__ __forceinline__ LaneSums piece_sums(const float (&x)[kElems], int piece, int vocab, int given, float mine, int& before, int lane) {
+  constexpr int kVecs = kElems / VEC;
   const int base = piece * kPiece;
   const auto here = [&](int v) LS_INLINED -> bool { return kWhole || base + v * 64 * VEC < vocab; };  // (uniform)
   LaneSums r;
@@ -571,7 +571,7 @@ __global__ __launch_bounds__(kRowThreads, 4) void logprobs_fold_kernel(const T* 
 
 // Short rows: a wave a row, four a workgroup; no wave waits for another.  The same sums (bits) as a workgroup a row, whose streams
 // have one piece at most there.  The bound is the k-th largest of the 64 lanes' maxima; the tokens that reach it are listed in
-// LDS, and a lane orders two of them.  (75,000 rows of 2,000 logits in float32: 526 us a workgroup each, 152 a wave each.)
+// LDS, and a lane orders two of them.  (75,000 rows of 2,000 logits in float32: 526 us a workgroup each, 155 a wave each.)
 constexpr int kShortPieces = kStreams, kShortThreads = 256;
 constexpr int kNarrowVocab = 512;  // up to here a lane has single logits: vectors would leave lanes without any
 constexpr int kShortList = 128;
@@ -601,14 +601,15 @@ __device__ __forceinline__ int list_in_order(ShortShared& sh, int w, int lane, c
   return min(listed, kShortList + 1);
 }
 
-// kPieces: the most pieces of a row (their lanes' maxima stay in registers).
-template <typename T, bool kNarrow, int kPieces>
+// kPieces: the most pieces of a row (their lanes' maxima stay in registers).  kNarrow: logits a lane has of a narrow row, or 0 (a
+// million rows of 150 logits: with four 0.31 ms; with 32, most of them behind the row's end, 0.80, spent on branches over those).
+template <typename T, int kNarrow, int kPieces>
 __global__ __launch_bounds__(kShortThreads) void logprobs_short_kernel(const T* __restrict__ logits, long ld, const int* __restrict__ tokens,
                                                                        int rows, int vocab, int top, float* __restrict__ logprob,
                                                                        float* __restrict__ entropy, int* __restrict__ rank,
                                                                        int* __restrict__ top_ids, float* __restrict__ top_logprobs) {
   __shared__ ShortShared sh;
-  constexpr int VEC = kNarrow ? 1 : Row<T>::VEC;
+  constexpr int VEC = kNarrow ? 1 : Row<T>::VEC, kElems = kNarrow ? kNarrow : kLaneElems;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = blockIdx.x * (kShortThreads / 64) + w;
   if (r >= rows) return;
@@ -624,10 +625,11 @@ __global__ __launch_bounds__(kShortThreads) void logprobs_short_kernel(const T* 
   for (int p = 0; p < kPieces; ++p) {
     set_max[p] = -INFINITY;
     if (p < pieces) {  // (uniform)
-      float x[kLaneElems];
-      load_piece<T, VEC>(x, row, p, vocab, lane);
-      const LaneSums here = kNarrow ? piece_sums<T, false, VEC>(x, p, vocab, given, given_logit, before, lane)
-                                    : sums_of_piece<T>(x, p, vocab, given, given_logit, before, lane);
+      float x[kElems];
+      load_piece<T, VEC, kElems>(x, row, p, vocab, lane);
+      LaneSums here;
+      if constexpr (kNarrow) here = piece_sums<T, false, VEC, kElems>(x, p, vocab, given, given_logit, before, lane);
+      else here = sums_of_piece<T>(x, p, vocab, given, given_logit, before, lane);
       set_max[p] = here.m;
       lane_max = fmaxf(lane_max, here.m);
       all = fold_sums(all, fold_lanes(here));
@@ -686,11 +688,11 @@ __global__ __launch_bounds__(kShortThreads) void logprobs_short_kernel(const T* 
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
       listed = 0;
-      // two sets of 32 at a time; vectors behind the row's end do not count
-      for (int i = 0; i < sets * kLaneElems; i += 64) {
-        const int j = i + lane, set = sh.sets[w][min(j / kLaneElems, sets - 1)], e = j % kLaneElems;
+      // two sets of 32 at a time (or more of fewer); vectors behind the row's end do not count
+      for (int i = 0; i < sets * kElems; i += 64) {
+        const int j = i + lane, set = sh.sets[w][min(j / kElems, sets - 1)], e = j % kElems;
         const int id = (set >> 6) * kPiece + ((e / VEC) * 64 + (set & 63)) * VEC + e % VEC;
-        const bool inside = j < sets * kLaneElems && id < vocab;
+        const bool inside = j < sets * kElems && id < vocab;
         if (__ballot(inside) == 0ull) continue;
         const unsigned int key = logit_key(to_f32(row[inside ? id : 0]));
         const unsigned long long hit = __ballot(inside && key >= bound);
@@ -774,8 +776,10 @@ int run_logprobs(const void* logits, long ld, const int* tokens, int rows, int v
   if (logprobs_short(rows, vocab)) {
     in_runs(1 << 24, [&](const T* x, const int* tokens, int rows, float* logprob, float* entropy, int* rank, int* top_ids, float* top_logprobs) {
       const int waves = kShortThreads / 64;
-      auto* kernel = vocab <= kNarrowVocab ? logprobs_short_kernel<T, true, 1> : pieces <= 2 ? logprobs_short_kernel<T, false, 2>
-                                                                                             : logprobs_short_kernel<T, false, kShortPieces>;
+      auto* kernel = vocab <= kNarrowVocab / 2 ? logprobs_short_kernel<T, kNarrowVocab / 128, 1>
+                     : vocab <= kNarrowVocab   ? logprobs_short_kernel<T, kNarrowVocab / 64, 1>
+                     : pieces <= 2             ? logprobs_short_kernel<T, 0, 2>
+                                               : logprobs_short_kernel<T, 0, kShortPieces>;
       kernel<<<(rows + waves - 1) / waves, kShortThreads, 0, stream>>>(x, ld, tokens, rows, vocab, top, logprob, entropy, rank, top_ids,
                                                                        top_logprobs);
     });
