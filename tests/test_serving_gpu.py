@@ -289,6 +289,30 @@ def test_attention(shape, dtype):
     assert bool((out[offsets[-1]:] == 9).all()) and bool((out[:, heads * d:] == 9).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [32, 96, 128, 256])
+def test_rows_off_every_boundary(d, dtype):
+    """Queries and outputs at odd elements of rows of odd length: one split, several, single tokens, prompts."""
+    g = torch.Generator().manual_seed(17)
+    lengths, news = [9, 1700, 40, 1300], [1, 1, 33, 60]
+    pool, table = make_cache(g, lengths, 2, d, 16)
+    offsets = [0, 1, 2, 35, 95]
+    wide = torch.randn((95, 4 * d + 7), generator=g).to(dtype).to(DEV)
+    q = wide[:, 3:4 * d + 3]
+    rows = torch.full((95, 4 * d + 9), 9.0, dtype=dtype, device=DEV)
+    out = rows[:, 5:4 * d + 5]
+    for first, last in ((0, 4), (0, 2), (2, 4)):
+        rows.fill_(9.0)
+        lo, hi = offsets[first], offsets[last]
+        kernels().fp4_attention(q[lo:hi], 4, 2, d, pool, torch.tensor(table[first:last], dtype=torch.int32, device=DEV),
+                                i32([o - lo for o in offsets[first:last + 1]]), i32(lengths[first:last]), max(news[first:last]),
+                                max(lengths[first:last]), out[lo:hi], d ** -0.5)
+        check_attention(out[lo:hi], q[lo:hi], 4, 2, d, pool, table[first:last], [o - lo for o in offsets[first:last + 1]],
+                        lengths[first:last], 16, 0)
+        assert bool((rows[:, :5] == 9).all()) and bool((rows[:, 4 * d + 5:] == 9).all())
+        assert bool((rows[:lo] == 9).all()) and bool((rows[hi:] == 9).all())
+
+
 def test_attention_of_one_key_is_its_value():
     g = torch.Generator().manual_seed(3)
     pool, table = make_cache(g, [1], 1, 64, 8)
