@@ -57,6 +57,7 @@ constexpr int kSharedKeys = 64;  // where a workgroup shares the tiles
 constexpr int kThreads = 256;
 constexpr float kSlack = 8.f;  // how far a score may pass the reference, in powers of two
 constexpr float kToLog2 = 1.4426950408889634f;
+constexpr float kLargestBf16 = 3.38953139e38f;
 
 template <typename T> constexpr int kTerms = std::is_same_v<T, float> ? 3 : 1;
 // Row tiles a wave holds where every wave has rows of its own: what its registers allow (2 of 2,048 rows a head of 160 behind
@@ -253,7 +254,8 @@ struct Rows {
               float rest = x[y];
 #pragma unroll
               for (int term = 0; term < 3; ++term) {
-                const bf16_t part = static_cast<bf16_t>(rest);
+                // (the numbers between bfloat16's largest and float32's would round to an infinity)
+                const bf16_t part = static_cast<bf16_t>(term == 0 ? fminf(fmaxf(rest, -kLargestBf16), kLargestBf16) : rest);
                 q[term][t][dim / 32 + i][y] = part;
                 rest = rest - static_cast<float>(part);
               }

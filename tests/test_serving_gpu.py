@@ -396,6 +396,21 @@ def test_offsets_and_lengths_that_do_not_fit():
     assert not out[:3].any() and bool(out[3:].any())
 
 
+@pytest.mark.parametrize("news", [1, 40])
+def test_queries_beyond_the_largest_bfloat16(news):
+    """The largest float32 numbers round to an infinity in bfloat16; with keys as small as they get the scores are ordinary."""
+    g = torch.Generator().manual_seed(21)
+    length, page, d = 50, 16, 32
+    pool, table = make_cache(g, [length], 1, d, page)
+    pool.k_scales[pool.k_scales < 255] = 2                  # keys of at most 6 times 2^-125
+    q = torch.randn((news, 2 * d), generator=g)
+    q[:, 3], q[:, 7], q[:, d + 1] = torch.finfo(torch.float32).max, -3.395e38, 3.4e38
+    q = q.to(DEV)
+    out = run_attention(q, 2, 1, d, pool, table, [0, news], [length], 0, scale=0.25)
+    got, _ = check_attention(out, q, 2, 1, d, pool, table, [0, news], [length], page, 0, scale=0.25)
+    assert bool(torch.isfinite(got).all())
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("heads", [4, 64])
 def test_more_rows_or_keys_than_stated(heads, dtype):
