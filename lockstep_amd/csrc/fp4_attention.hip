@@ -32,6 +32,7 @@
 #include "fp4.h"
 #include "fp4_attention_api.h"
 
+#include <algorithm>
 #include <type_traits>
 
 #ifndef LS_HEAD_DIM
@@ -1130,13 +1131,14 @@ struct Plan {
   int few, decode_splits, prompt_places, region, most_splits;  // places: row blocks of a workgroup times splits, of a request's head
 };
 
-// What is launched for requests of at most `most` tokens and `longest` keys: bounds for every shorter one.
+// What is launched for requests of at most `most` tokens and `longest` keys: bounds for every shorter one.  (In host code the plain
+// min and max are those of int: what may pass 31 bits takes the standard library's.)
 template <typename T>
 Plan make_plan(int kv_heads, int group, int most, int longest, int window) {
   constexpr int kGroupRows = 64 * kPromptTiles<T>;
   Plan p{16, 1, 0, 0, 1};
   // the keys that a request's rows see, at most: with a window those of its tokens and the window before, in whole tiles
-  const auto seen = [&](int n) { return window > 0 ? (int)min((long)longest, (long)n + window - 1 + kSharedKeys) : longest; };
+  const auto seen = [&](int n) { return window > 0 ? (int)std::min<long>(longest, (long)n + window - 1 + kSharedKeys) : longest; };
   const int span = seen(min(max(1, p.few / group), most));
   if (span > kOneSplit) {
     const auto most_of = [&](int n) { return (n + shortest_split(n, kv_heads) - 1) / shortest_split(n, kv_heads); };
@@ -1150,7 +1152,7 @@ Plan make_plan(int kv_heads, int group, int most, int longest, int window) {
     const int want = max(1, kPromptGroups / kv_heads), far = seen(most);
     p.prompt_places = (int)((rows + kGroupRows - 1) / kGroupRows);
     if (want > 1 && far > kPromptShortest) {
-      p.prompt_places = (int)max((long)p.prompt_places, min((long)want, (long)p.prompt_places * ((far + kPromptShortest - 1) / kPromptShortest)));
+      p.prompt_places = (int)std::max<long>(p.prompt_places, std::min<long>(want, (long)p.prompt_places * ((far + kPromptShortest - 1) / kPromptShortest)));
       p.region = max(p.region, want * kGroupRows);
       p.most_splits = max(p.most_splits, min(want, (far + kPromptShortest - 1) / kPromptShortest));
     }
@@ -1160,7 +1162,7 @@ Plan make_plan(int kv_heads, int group, int most, int longest, int window) {
 
 // Splits' sums that a step may leave.
 inline long entries_of(const Plan& p, int kv_heads, int group, int requests, int rows) {
-  return p.region == 0 ? 0 : min((long)requests * kv_heads * p.region, (long)rows * kv_heads * group * p.most_splits);
+  return p.region == 0 ? 0 : std::min<long>((long)requests * kv_heads * p.region, (long)rows * kv_heads * group * p.most_splits);
 }
 
 template <typename T, bool kWholePages>
@@ -1191,7 +1193,7 @@ int run_fp4(Fp4Args& a, int most, int longest, void* scratch, long scratch_bytes
     const long pairs = (long)most * a.group * heads;  // of the request with most
     LS_REQUIRE(pairs <= 0x7ffffff0l, "fp4_attention: %d rows of %d heads", most, a.group * heads);
     if (pairs * a.requests >= 2048)
-      fp4_combine_kernel<T, true><<<dim3((unsigned)min((pairs + 3) / 4, 1024l), a.requests), kThreads, 0, stream>>>(a);
+      fp4_combine_kernel<T, true><<<dim3((unsigned)std::min<long>((pairs + 3) / 4, 1024), a.requests), kThreads, 0, stream>>>(a);
     else
       fp4_combine_kernel<T, false><<<dim3((unsigned)pairs, a.requests), kThreads, 0, stream>>>(a);
   }

@@ -24,6 +24,8 @@
 #include "common.h"
 #include "serving_api.h"
 
+#include <algorithm>
+
 namespace ls {
 
 constexpr int kPiece = 2048;
@@ -770,7 +772,7 @@ int run_logprobs(const void* logits, long ld, const int* tokens, int rows, int v
   // (a grid has less than 2^32 threads: rows in runs, of which all but absurd calls have one)
   const auto in_runs = [&](int run, auto launch) {
     for (long from = 0; from < rows; from += run)
-      launch(x + from * ld, tokens + from, (int)min((long)run, rows - from), logprob + from, entropy + from, rank + from,
+      launch(x + from * ld, tokens + from, (int)std::min<long>(run, rows - from), logprob + from, entropy + from, rank + from,
              top_ids + from * top, top_logprobs + from * top);
   };
   if (logprobs_short(rows, vocab)) {

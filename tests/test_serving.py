@@ -3,6 +3,8 @@ plain implementations against one another (no GPU needed)."""
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 from plain import serving_plain as plain
@@ -89,3 +91,14 @@ def test_the_plan_of_the_splits_covers_every_request():
                 many = -(-span // prompt_split(span, groups, heads))
                 assert many <= max(1, min(512 // heads, -(-span // 256)))
                 assert groups * many <= max(1, 512 // heads) or many <= 1
+
+
+@pytest.mark.parametrize("rows,requests,heads,group,most,longest", [
+    (160, 40, 8, 4, 160, 8192), (65, 65, 8, 1, 1, 8192), (5000, 65, 8, 4, 256, 8192), (4500, 64, 8, 16, 300, 131072)])
+def test_memory_of_large_steps_is_counted_in_64_bits(rows, requests, heads, group, most, longest):
+    """A thousand times the rows and requests take a thousand times the memory."""
+    lib = ctypes.CDLL(str(kernel_build.build_fp4_attention(128)))
+    count = lib.ls_fp4_attention_scratch_bytes
+    count.restype = ctypes.c_long
+    one = count(1, rows, requests, heads, group, most, longest, 0)
+    assert 0 < one < 2 ** 33 and count(1, 1000 * rows, 1000 * requests, heads, group, most, longest, 0) == 1000 * one
