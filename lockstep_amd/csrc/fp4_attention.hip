@@ -86,6 +86,24 @@ __host__ __device__ inline int prompt_split(int span, int groups, int kv_heads) 
   return max(kPromptShortest, ((span + want - 1) / want + 63) / 64 * 64);  // whole tiles of 64
 }
 
+// How a request of `rows` rows a head whose rows see `span` keys is cut: the same in the kernels and on the host.
+constexpr int kFewRows = 16;  // rows a head up to which a request belongs to the decoding part
+template <typename T> constexpr int kGroupRows = 64 * kPromptTiles<T>;  // rows of a prompt's workgroup
+struct Cut {
+  int groups, len, splits;  // workgroups of rows (0: few rows), keys a split, splits
+};
+template <typename T>
+__host__ __device__ inline Cut cut_request(int rows, int span, int kv_heads) {
+  Cut c;
+  c.groups = rows <= kFewRows ? 0 : (rows + kGroupRows<T> - 1) / kGroupRows<T>;
+  c.len = c.groups == 0 ? decode_split(span, kv_heads) : prompt_split(span, c.groups, kv_heads);
+  c.splits = max(1, (span + c.len - 1) / c.len);
+  return c;
+}
+// The first key that a row at `position` sees, and the first tile of the rows from there on.
+__host__ __device__ inline int first_seen(int position, int window) { return window > 0 && position >= window ? position - window + 1 : 0; }
+__host__ __device__ inline int first_tile(int position, int window) { return first_seen(position, window) & ~(kSharedKeys - 1); }
+
 struct Fp4Args {
   const void* q;
   long ldq;
@@ -106,11 +124,7 @@ struct Fp4Args {
   float* part_ml;          // [entries][2]: reference, sum of the weights
   int region;              // entries a request's head, or (by_row) a query head of a row of q
   bool by_row;
-  int few;                 // rows a head up to which a request belongs to the decoding kernel
 };
-
-// The first key that a row at `position` sees.
-__device__ __forceinline__ int first_seen(int position, int window) { return window > 0 && position >= window ? position - window + 1 : 0; }
 
 // One request as all kernels see it.
 struct Request {
@@ -124,7 +138,7 @@ struct Request {
     const int room = (int)min((long)a.columns << a.pool.page_shift, (long)a.longest);  // (a few tiles on stay below 2^31)
     end = min(max(a.lengths[b], 0), room);
     start = end - n;
-    base = first_seen(start, a.window) & ~(kSharedKeys - 1);
+    base = first_tile(start, a.window);
   }
 };
 
@@ -586,9 +600,9 @@ template <typename T, bool kWholePages>
 __device__ __forceinline__ void decode_part(const Fp4Args& a, FoldShared& fold, int split, int head, int b) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Request rq(a, b);
-  if (rq.rows == 0 || rq.rows > a.few) return;
-  const int span = rq.end - rq.base, len = decode_split(span, a.pool.kv_heads);
-  const int splits = max(1, (span + len - 1) / len);
+  if (rq.rows == 0 || rq.rows > kFewRows) return;
+  const Cut cut = cut_request<T>(rq.rows, rq.end - rq.base, a.pool.kv_heads);
+  const int splits = cut.splits, len = cut.len;
   if (split >= splits) return;
   const int begin = rq.base + split * len, end = min(rq.end, begin + len);
   Rows<T, 1> rows;
@@ -937,11 +951,10 @@ __device__ __forceinline__ void prompt_part(const Fp4Args& a, PromptShared& shar
   auto& operands = shared.operands;
   auto& flags = shared.flags;
   const Request rq(a, b);
-  if (rq.rows <= a.few) return;
+  if (rq.rows <= kFewRows) return;
   const int blocks = (rq.rows + kBlock - 1) / kBlock;
-  const int groups = (blocks + 3) / 4;
-  const int span = rq.end - rq.base, len = prompt_split(span, groups, a.pool.kv_heads);
-  const int splits = max(1, (span + len - 1) / len);
+  const Cut cut = cut_request<T>(rq.rows, rq.end - rq.base, a.pool.kv_heads);
+  const int groups = cut.groups, splits = cut.splits, len = cut.len;
   if (place >= groups * splits) return;
   const int split = place / groups, group = groups - 1 - (place - split * groups);  // the rows that see most keys first
   const int row0 = (4 * group + w) * kBlock;
@@ -1047,11 +1060,9 @@ __global__ __launch_bounds__(kThreads) void fp4_combine_kernel(Fp4Args a) {  // 
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int heads = a.group * a.pool.kv_heads, b = blockIdx.y;
   const Request rq(a, b);
-  const int span = rq.end - rq.base;
-  const bool few = rq.rows <= a.few;
   const int blocks = (rq.rows + kBlock - 1) / kBlock;
-  const int len = few ? decode_split(span, a.pool.kv_heads) : prompt_split(span, (blocks + 3) / 4, a.pool.kv_heads);
-  const int splits = (span + len - 1) / len, stride = few ? 16 : blocks * kBlock;
+  const Cut cut = cut_request<T>(rq.rows, rq.end - rq.base, a.pool.kv_heads);
+  const int splits = cut.splits, stride = cut.groups == 0 ? 16 : blocks * kBlock;
   if (splits <= 1 || splits > kMostSplits) return;
   const int pairs = rq.rows * a.pool.kv_heads, stride_pairs = kWaveEach ? 4 * gridDim.x : gridDim.x;
   constexpr int kEach = (D + 63) / 64;
@@ -1128,18 +1139,17 @@ __global__ __launch_bounds__(kThreads) void fp4_combine_kernel(Fp4Args a) {  // 
 }
 
 struct Plan {
-  int few, decode_splits, prompt_places, region, most_splits;  // places: row blocks of a workgroup times splits, of a request's head
+  int decode_splits, prompt_places, region, most_splits;  // places: row blocks of a workgroup times splits, of a request's head
 };
 
 // What is launched for requests of at most `most` tokens and `longest` keys: bounds for every shorter one.  (In host code the plain
 // min and max are those of int: what may pass 31 bits takes the standard library's.)
 template <typename T>
 Plan make_plan(int kv_heads, int group, int most, int longest, int window) {
-  constexpr int kGroupRows = 64 * kPromptTiles<T>;
-  Plan p{16, 1, 0, 0, 1};
+  Plan p{1, 0, 0, 1};
   // the keys that a request's rows see, at most: with a window those of its tokens and the window before, in whole tiles
   const auto seen = [&](int n) { return window > 0 ? (int)std::min<long>(longest, (long)n + window - 1 + kSharedKeys) : longest; };
-  const int span = seen(min(max(1, p.few / group), most));
+  const int span = seen(min(max(1, kFewRows / group), most));
   if (span > kOneSplit) {
     const auto most_of = [&](int n) { return (n + shortest_split(n, kv_heads) - 1) / shortest_split(n, kv_heads); };
     p.decode_splits = min(max(most_of(span), most_of(min(span, 4096))), (kDecodeGroups + kv_heads - 1) / kv_heads);
@@ -1147,13 +1157,13 @@ Plan make_plan(int kv_heads, int group, int most, int longest, int window) {
     p.most_splits = p.decode_splits;
   }
   const long rows = (long)most * group;
-  if (rows > p.few) {
+  if (rows > kFewRows) {
     // a request with more than one split has `want` places at most, and no split is shorter than the shortest
     const int want = max(1, kPromptGroups / kv_heads), far = seen(most);
-    p.prompt_places = (int)((rows + kGroupRows - 1) / kGroupRows);
+    p.prompt_places = (int)((rows + kGroupRows<T> - 1) / kGroupRows<T>);
     if (want > 1 && far > kPromptShortest) {
       p.prompt_places = (int)std::max<long>(p.prompt_places, std::min<long>(want, (long)p.prompt_places * ((far + kPromptShortest - 1) / kPromptShortest)));
-      p.region = max(p.region, want * kGroupRows);
+      p.region = max(p.region, want * kGroupRows<T>);
       p.most_splits = max(p.most_splits, min(want, (far + kPromptShortest - 1) / kPromptShortest));
     }
   }
@@ -1178,7 +1188,6 @@ template <typename T>
 int run_fp4(Fp4Args& a, int most, int longest, void* scratch, long scratch_bytes, hipStream_t stream) {
   const Plan p = make_plan<T>(a.pool.kv_heads, a.group, most, longest, a.window);
   const int heads = a.pool.kv_heads;
-  a.few = p.few;
   const long entries = entries_of(p, heads, a.group, a.requests, a.rows);
   a.by_row = entries != (long)a.requests * heads * p.region;
   a.region = a.by_row ? p.most_splits : p.region;
@@ -1212,6 +1221,34 @@ extern "C" long ls_fp4_attention_scratch_bytes(int dtype, int rows, int requests
   const Plan p = dtype == kF32 ? make_plan<float>(kv_heads, group, most, longest, window)
                                : make_plan<bf16_t>(kv_heads, group, most, longest, window);
   return entries_of(p, kv_heads, group, requests, rows) * (D + 2) * (long)sizeof(float);
+}
+
+namespace ls {
+template <typename T>
+void plan_of(int rows, int requests, int kv_heads, int group, int most, int longest, int window, int tokens, int length, long* out) {
+  const Plan p = make_plan<T>(kv_heads, group, most, longest, window);
+  const Cut c = cut_request<T>(tokens * group, length - first_tile(length - tokens, window), kv_heads);
+  const long entries = entries_of(p, kv_heads, group, requests, rows);
+  const bool by_row = entries != (long)requests * kv_heads * p.region;
+  const int block = 16 * kPromptTiles<T>, padded = c.groups == 0 ? 16 : (tokens * group + block - 1) / block * block;
+  out[0] = c.splits;
+  out[1] = c.groups == 0 ? c.splits : (long)c.groups * c.splits;
+  out[2] = c.groups == 0 ? p.decode_splits : p.prompt_places;
+  out[3] = c.splits == 1 ? 0 : (long)c.splits * (by_row ? tokens * group : padded);
+  out[4] = by_row ? (long)tokens * group * p.most_splits : p.region;
+  out[5] = entries;
+}
+}  // namespace ls
+
+extern "C" int ls_fp4_attention_plan(int dtype, int rows, int requests, int kv_heads, int group, int most, int longest, int window,
+                                     int tokens, int length, long* out) {
+  using namespace ls;
+  LS_REQUIRE((dtype == kF32 || dtype == kBF16) && rows >= 1 && requests >= 1 && kv_heads >= 1 && group >= 1 && tokens >= 1 &&
+                 tokens <= most && most <= rows && length >= tokens && length <= longest && window >= 0 && (long)most * group <= 0x7fffff00l,
+             "fp4_attention: no plan for a request of %d tokens and %d keys among %d rows", tokens, length, rows);
+  if (dtype == kF32) plan_of<float>(rows, requests, kv_heads, group, most, longest, window, tokens, length, out);
+  else plan_of<bf16_t>(rows, requests, kv_heads, group, most, longest, window, tokens, length, out);
+  return 0;
 }
 
 extern "C" int ls_fp4_attention(int dtype, const void* q, long ldq, void* out, long ldo, int rows, const void* k_codes,

@@ -4,6 +4,7 @@ plain implementations against one another (no GPU needed)."""
 from __future__ import annotations
 
 import ctypes
+import random
 
 import pytest
 import torch
@@ -102,3 +103,39 @@ def test_memory_of_large_steps_is_counted_in_64_bits(rows, requests, heads, grou
     count.restype = ctypes.c_long
     one = count(1, rows, requests, heads, group, most, longest, 0)
     assert 0 < one < 2 ** 33 and count(1, 1000 * rows, 1000 * requests, heads, group, most, longest, 0) == 1000 * one
+
+
+def plan_entry(head_dim):
+    """(splits, workgroups, launched, entries, room, all entries) of a request in a step, by the library's own host code."""
+    lib = ctypes.CDLL(str(kernel_build.build_fp4_attention(head_dim)))
+    entry, code = lib.ls_fp4_attention_plan, {torch.float32: 0, torch.bfloat16: 1}
+    lib.ls_last_error.restype = ctypes.c_char_p
+
+    def plan(dtype, rows, requests, heads, group, most, longest, window, tokens, length):
+        out = (ctypes.c_long * 6)()
+        assert entry(code[dtype], rows, requests, heads, group, most, longest, window, tokens, length, out) == 0, lib.ls_last_error()
+        return tuple(out)
+    return plan
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("head_dim", [64, 160, 256])
+def test_the_library_launches_enough_for_every_request(head_dim, dtype):
+    """What a launch is sized for (workgroups, room for the splits' sums) covers every request that it may hold."""
+    plan = plan_entry(head_dim)
+    rng = random.Random(head_dim)
+    for _ in range(6000):
+        heads, group = rng.choice((1, 2, 3, 4, 5, 8, 12, 64, 300, 600)), rng.choice((1, 2, 3, 4, 8, 16, 17, 40))
+        requests = rng.choice((1, 2, 7, 64, 300))
+        longest = int(2 ** rng.uniform(0, 20.5))
+        most = min(longest, int(2 ** rng.uniform(0, 13)))
+        rows = most + rng.choice((0, requests - 1, rng.randrange(most * requests)))
+        window = rng.choice((0, 0, 1, int(2 ** rng.uniform(0, 20))))
+        window = 0 if window >= longest else window
+        for tokens in {1, most, max(1, min(most, 16 // group)), min(most, 16 // group + 1), rng.randint(1, most), rng.randint(1, min(most, 40))}:
+            for length in {longest, tokens, rng.randint(tokens, longest), min(longest, tokens + 4096)}:
+                case = (dtype, rows, requests, heads, group, most, longest, window, tokens, length)
+                splits, groups, launched, entries, room, held = plan(*case)
+                assert 1 <= splits <= groups <= launched, case
+                assert splits == 1 or 0 < entries <= room <= held, case
+                assert splits <= 512 and (splits - 1) * 256 < length, case
