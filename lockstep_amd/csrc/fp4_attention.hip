@@ -75,7 +75,7 @@ template <typename T> constexpr int kPromptWaves = D <= 128 ? 2 : 1;
 constexpr int kOneSplit = 768, kDecodeGroups = 512;
 __host__ __device__ inline int shortest_split(int span, int kv_heads) { return kv_heads < 4 ? 256 : span <= 4096 ? 512 : 1024; }
 __host__ __device__ inline int decode_split(int span, int kv_heads) {
-  if (span <= kOneSplit) return kOneSplit;
+  if (span <= kOneSplit || kv_heads >= kDecodeGroups) return max(span, kOneSplit);
   const int even = (int)(((long)span * kv_heads + kDecodeGroups - 1) / kDecodeGroups);
   return max(shortest_split(span, kv_heads), (even + 127) / 128 * 128);
 }

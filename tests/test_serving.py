@@ -139,3 +139,12 @@ def test_the_library_launches_enough_for_every_request(head_dim, dtype):
                 assert 1 <= splits <= groups <= launched, case
                 assert splits == 1 or 0 < entries <= room <= held, case
                 assert splits <= 512 and (splits - 1) * 256 < length, case
+
+
+@pytest.mark.parametrize("heads", [511, 512, 600, 1024])
+def test_the_longest_requests_of_many_heads_have_their_splits(heads):
+    plan = plan_entry(128)
+    for longest in (2 ** 29, 2 ** 30 + 12345, 2 ** 31 - 2 ** 16):
+        for tokens in (1, 3, 40):
+            splits, groups, launched, entries, room, held = plan(torch.bfloat16, 40, 2, heads, 4, 40, longest, 0, tokens, longest)
+            assert 1 <= splits <= groups <= launched and entries <= room <= held, (longest, tokens)
