@@ -56,6 +56,28 @@ T* vector(const Tensor& t, int device, int64_t n, at::ScalarType type = at::kInt
   return static_cast<T*>(t.data_ptr());
 }
 
+// Bytes of memory: `rows` runs of `width` bytes, `stride` apart.
+struct Area {
+  uintptr_t lo;
+  int64_t rows, width, stride;
+  uintptr_t end() const { return lo + (uintptr_t)((rows - 1) * stride + width); }
+};
+Area area(const Tensor& t) { return {reinterpret_cast<uintptr_t>(t.data_ptr()), 1, t.numel() * (int64_t)t.element_size(), 0}; }
+Area area(const Tensor& t, int64_t width) {  // the first `width` elements of every row
+  const int64_t item = (int64_t)t.element_size();
+  return {reinterpret_cast<uintptr_t>(t.data_ptr()), t.size(0), width * item, t.stride(0) * item};
+}
+// Whether two areas share a byte.  Windows of columns of one buffer, side by side, do not; rows of different strides that lie in
+// one another's range count as if they did.
+bool meet(const Area& a, const Area& b) {
+  if (a.rows == 0 || b.rows == 0 || a.width == 0 || b.width == 0 || a.end() <= b.lo || b.end() <= a.lo) return false;
+  if (a.stride == b.stride && a.rows > 1 && b.rows > 1 && a.stride > 0) {
+    const int64_t apart = (int64_t)(b.lo - a.lo) % a.stride, offset = apart < 0 ? apart + a.stride : apart;
+    return offset < a.width || offset + b.width > a.stride;
+  }
+  return true;
+}
+
 struct Bound {
   decltype(&ls_step_tables) step_tables;
   decltype(&ls_fp4_write) fp4_write;
@@ -177,6 +199,7 @@ PyObject* step_tables(PyObject*, PyObject* const* x, Py_ssize_t n) {
 struct Pool {  // a pool of pages in 4 bits, checked
   int64_t pages, heads, page_size, dim;
   void* data[4];
+  Area areas[4];
   Pool(PyObject* o, int device) {
     need(PyTuple_Check(o) && PyTuple_GET_SIZE(o) == 4);
     const Tensor& codes = tensor(PyTuple_GET_ITEM(o, 0));
@@ -195,6 +218,7 @@ struct Pool {  // a pool of pages in 4 bits, checked
       need(t.scalar_type() == at::kByte && on(t, device) && t.dim() == dims[i] && t.is_contiguous());
       for (int k = 0; k < dims[i]; ++k) need(t.size(k) == shapes[i][k]);
       data[i] = t.data_ptr();
+      areas[i] = area(t);
       need((reinterpret_cast<uintptr_t>(data[i]) & 15) == 0);
     }
   }
@@ -258,7 +282,9 @@ PyObject* fp4_attention(PyObject*, PyObject* const* x, Py_ssize_t n) {
     need(requests <= 65535 && columns <= k31 && most >= 0 && longest >= 0 && longest <= columns * pool.page_size && window >= 0 &&
          scale >= -1e30 && scale <= 1e30);
     void *qp = q.data_ptr(), *op = out.data_ptr();
-    need(rows == 0 || qp != op);
+    const Area to = area(out, nq * d);
+    need(!meet(to, area(q, nq * d)) && !meet(to, area(table)) && !meet(to, area(offsets)) && !meet(to, area(lengths)));
+    for (const Area& held : pool.areas) need(!meet(to, held));
     most = std::min(most, rows);
     if (most == 0 || requests == 0) return 0;
     need(longest <= k31);

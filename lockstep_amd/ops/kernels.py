@@ -67,6 +67,36 @@ def _rows_ok(t: torch.Tensor, name: str) -> None:
                           f"strides {t.stride()} on {t.device}")
 
 
+class _Area(NamedTuple):
+    """Bytes of memory: ``rows`` runs of ``width`` bytes, ``stride`` apart."""
+
+    lo: int
+    rows: int
+    width: int
+    stride: int
+
+
+def _area(t: torch.Tensor, width=None) -> _Area:
+    """What a contiguous tensor, or the first ``width`` elements of every row of a matrix, lies in."""
+    item = t.element_size()
+    if width is None:
+        return _Area(t.data_ptr(), 1, t.numel() * item, 0)
+    return _Area(t.data_ptr(), t.shape[0], width * item, t.stride(0) * item)
+
+
+def _meet(a: _Area, b: _Area) -> bool:
+    """Whether two areas share a byte.  Windows of columns of one buffer, side by side, do not; rows of different strides that
+    lie in one another's range count as if they did."""
+    if not (a.rows and b.rows and a.width and b.width):
+        return False
+    if a.lo + (a.rows - 1) * a.stride + a.width <= b.lo or b.lo + (b.rows - 1) * b.stride + b.width <= a.lo:
+        return False
+    if a.stride == b.stride and a.rows > 1 and b.rows > 1 and a.stride > 0:
+        offset = (b.lo - a.lo) % a.stride
+        return offset < a.width or offset + b.width > a.stride
+    return True
+
+
 def _load_calls():
     """The extension module of checked calls, or None where it cannot be built (Python's checks do without it)."""
     from importlib.machinery import ExtensionFileLoader
@@ -2202,7 +2232,8 @@ class Kernels:
 
         ``q [tokens, >= nq * d]`` (float32 or bfloat16; ``out`` likewise): request i has the rows ``offsets[i]`` to
         ``offsets[i + 1] - 1``, the last of them at position ``lengths[i] - 1`` (its key and value are in the pages
-        already); ``table [requests, columns]`` are the block tables (int32, as are offsets and lengths).  With a
+        already); ``table [requests, columns]`` are the block tables (int32, as are offsets and lengths).  ``out`` shares no
+        memory with ``q`` (columns of one wider buffer, side by side, do not) or another operand.  With a
         ``window`` a row sees that many keys, its own among them.  ``max_tokens`` and ``max_length``: the most rows and
         the greatest length of any request; they size the launches, so a request of more rows is left out (its rows stay as
         they are) and a greater length counts as that one.  Rows that belong to no request stay as they are; a row that sees no key (a length of 0, pages that the table does not
@@ -2238,8 +2269,9 @@ class Kernels:
                 and rows <= 0x7FFFFFFF and columns <= 0x7FFFFFFF and count <= 0x7FFFFFFF and -1e30 <= scale <= 1e30):
             raise KernelError(f"fp4_attention: {rows} rows, at most {max_tokens} rows and {max_length} keys a request, window "
                               f"{window}, {requests} requests with {columns} of {count} pages of {page_size}, {nkv} kv heads, scale {scale}")
-        if q.data_ptr() == out.data_ptr() and rows:
-            raise KernelError("fp4_attention: q and out are the same rows")
+        to = _area(out, nq * d)
+        if _meet(to, _area(q, nq * d)) or any(_meet(to, _area(t)) for t in (*pages, table, offsets, lengths)):
+            raise KernelError("fp4_attention: out overlaps q or another operand")
         max_tokens = min(max_tokens, rows)
         if max_tokens == 0 or requests == 0:
             return

@@ -148,3 +148,33 @@ def test_the_longest_requests_of_many_heads_have_their_splits(heads):
         for tokens in (1, 3, 40):
             splits, groups, launched, entries, room, held = plan(torch.bfloat16, 40, 2, heads, 4, 40, longest, 0, tokens, longest)
             assert 1 <= splits <= groups <= launched and entries <= room <= held, (longest, tokens)
+
+
+def test_areas_that_share_memory():
+    from lockstep_amd.ops.kernels import _area, _meet
+
+    buffer = torch.arange(6 * 40).reshape(6, 40)
+    rng = random.Random(2)
+
+    def window(strides):
+        first, last = sorted(rng.sample(range(7), 2))
+        left, right = sorted(rng.sample(range(41), 2))
+        x = buffer[first:last, left:right]
+        return (x, x) if strides is None else (x[::strides], x[::strides])
+
+    exact = met = 0
+    for _ in range(4000):
+        kind = rng.choice((None, None, 2))
+        (a, _), (b, _) = window(None), window(kind)
+        shared = bool(set(a.reshape(-1).tolist()) & set(b.reshape(-1).tolist()))
+        found = _meet(_area(a, a.shape[1]), _area(b, b.shape[1]))
+        assert found == _meet(_area(b, b.shape[1]), _area(a, a.shape[1]))
+        assert found or not shared
+        if kind is None and a.shape[0] > 1 and b.shape[0] > 1:
+            exact, met = exact + 1, met + shared
+            if a.shape == b.shape and a.storage_offset() // 40 == b.storage_offset() // 40:     # the same rows: never refused in vain
+                assert found == shared
+    assert exact > 1000 and met > 300
+    x = torch.zeros(10)
+    assert _meet(_area(x), _area(x[9:])) and not _meet(_area(x[:9]), _area(x[9:])) and not _meet(_area(x), _area(x[:0]))
+    assert _meet(_area(x[2:3].expand(4, 3), 3), _area(x)) and not _meet(_area(x[:0].reshape(0, 3), 3), _area(x))

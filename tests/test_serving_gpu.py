@@ -486,6 +486,51 @@ def test_attention_refusals():
     torch.cuda.synchronize()
 
 
+@pytest.fixture(params=["module", "python"])
+def route(request):
+    """Calls through the extension module, and through Python's checks alone."""
+    k = kernels()
+    k.serving, k.fp4_attention_lib(64)
+    module = k._calls
+    assert module is not None
+    if request.param == "python":
+        k._calls = None
+    yield request.param
+    k._calls = module
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attention_refuses_outputs_in_its_operands(route, dtype):
+    k = kernels()
+    g = torch.Generator().manual_seed(30)
+    pool, table = make_cache(g, [20, 30], 2, 64, 16)
+    rows = torch.randn((6, 600), generator=g).to(dtype).to(DEV)
+    call = lambda q, out, **change: k.fp4_attention(**{**dict(  # noqa: E731
+        q=q, nq=4, nkv=2, d=64, pages=pool, table=torch.tensor(table, dtype=torch.int32, device=DEV), offsets=i32([0, 1, 3]),
+        lengths=i32([20, 30]), max_tokens=2, max_length=30, out=out, scale=0.125), **change})
+    before = rows.clone()
+    for q, out in ((rows[:3], rows[:3]), (rows[:3], rows[1:4]), (rows[1:4], rows[:3]), (rows[:3], rows[2:5]), (rows[:3], rows[:3, 1:]),
+                   (rows[:3], rows[:3, 255:]), (rows[:3, 255:], rows[:3]), (rows[:3], rows[:5:2]), (rows[:3, 300:], rows[1:4, 45:])):
+        with pytest.raises(KernelError, match="overlap"):
+            call(q, out)
+    ints = torch.zeros(3 * 256, dtype=torch.float32, device=DEV)
+    room = ints.view(torch.int32)
+    if dtype is torch.float32:
+        room[:3] = i32([0, 1, 3])
+        for change in (dict(offsets=room[:3]), dict(lengths=room[766:]), dict(table=room[100:104].view(2, 2))):
+            with pytest.raises(KernelError, match="overlap"):
+                call(rows[:3], ints.view(3, 256), **change)
+    torch.cuda.synchronize()
+    assert torch.equal(rows, before)
+    # columns side by side, rows behind one another: taken
+    want = torch.empty((3, 256), dtype=dtype, device=DEV)
+    call(rows[:3], want)
+    for q, out in ((rows[:3], rows[:3, 256:512]), (rows[:3], rows[3:]), (rows[:3], rows[2:5, 256:]), (rows[:3], rows[:3, 344:])):
+        rows.copy_(before)
+        call(q, out)
+        assert torch.equal(out[:, :256], want) and torch.equal(rows[:3, :256], before[:3, :256])
+
+
 def test_no_memory_of_a_call_in_noted_launches():
     """Launches that are noted to be made again would use a call's memory after its end; those without any may be noted."""
     k = kernels()
