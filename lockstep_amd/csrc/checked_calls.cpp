@@ -241,7 +241,11 @@ PyObject* fp4_rows(PyObject* const* x, Py_ssize_t n, bool write) {
     void *kp = k.data_ptr(), *vp = v.data_ptr();
     const int64_t ldk = k.stride(0), ldv = v.stride(0);
     if (tokens == 0) return 0;
-    if (!write) need((tokens <= 1 || (ldk >= width && ldv >= width)) && kp != vp);
+    if (!write) {
+      const Area keys = area(k, width), values = area(v, width), ids = area(slots);
+      need((tokens <= 1 || (ldk >= width && ldv >= width)) && !meet(keys, values) && !meet(keys, ids) && !meet(values, ids));
+      for (const Area& held : pool.areas) need(!meet(keys, held) && !meet(values, held));
+    }
     return without_gil([&] {
       return write ? bound.fp4_write(code, kp, ldk, vp, ldv, slot, (int)tokens, (int)pool.heads, (int)pool.dim, pool.data[0], pool.data[1],
                                      pool.data[2], pool.data[3], (int)pool.pages, (int)pool.page_size, stream)

@@ -2213,13 +2213,17 @@ class Kernels:
 
     def fp4_read(self, pages: Fp4Pages, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
         """The keys and values that the slots hold, as float32 or bfloat16 (both exact) rows ``[tokens, kv heads * d]``;
-        rows whose slot is negative or beyond the pool stay as they are."""
+        rows whose slot is negative or beyond the pool stay as they are.  Keys and values share no memory (columns of one wider
+        buffer, side by side, do not), nor do they with the pages or the slots."""
         calls = self._calls
         if calls is not None and self.tape is None and calls.fp4_read(here := _raw_device(), _raw_stream(here), k, v, slots, pages):
             return
         args = self._fp4_rows("fp4_read", k, v, slots, pages)
-        if not ((args[6] <= 1 or (args[2] >= k.shape[1] and args[4] >= k.shape[1])) and (args[6] == 0 or args[1] != args[3])):
-            raise KernelError("fp4_read: rows overlap")
+        areas = [_area(k, k.shape[1]), _area(v, v.shape[1])]
+        others = [_area(t) for t in (*pages, slots)]
+        if not (args[6] <= 1 or (args[2] >= k.shape[1] and args[4] >= k.shape[1])) or _meet(*areas) or any(
+                _meet(a, b) for a in areas for b in others):
+            raise KernelError("fp4_read: rows overlap one another, the pages or the slots")
         if args[6] == 0:
             return
         lib = self.serving

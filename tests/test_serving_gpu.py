@@ -531,6 +531,39 @@ def test_attention_refuses_outputs_in_its_operands(route, dtype):
         assert torch.equal(out[:, :256], want) and torch.equal(rows[:3, :256], before[:3, :256])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_reading_refuses_rows_in_its_operands(route, dtype):
+    k = kernels()
+    g = torch.Generator().manual_seed(31)
+    pool, table = make_cache(g, [20], 2, 64, 16)
+    slots = i32([table[0][0] * 16 + 1, table[0][0] * 16 + 7, table[0][1] * 16 + 2])
+    rows = torch.full((6, 400), 5.0, dtype=dtype, device=DEV)
+    for keys, values in ((rows[:3, :128], rows[:3, :128]), (rows[:3, :128], rows[1:4, :128]), (rows[:3, :128], rows[:3, 127:255]),
+                         (rows[:3, 100:228], rows[:3, :128]), (rows[:3, :128], rows[:5:2, :128]), (rows[:3, 272:], rows[1:4, :128].as_strided((3, 128), (400, 1), 399))):
+        with pytest.raises(KernelError, match="overlap"):
+            k.fp4_read(pool, slots, keys, values)
+    bytes_of = [t.view(-1)[:3 * 256 * rows.element_size()] for t in (pool.k_codes, pool.v_codes)]
+    for held in bytes_of:
+        inside = held[:3 * 128 * rows.element_size()].view(dtype).view(3, 128)
+        for pair in ((inside, rows[:3, :128]), (rows[:3, :128], inside)):
+            with pytest.raises(KernelError, match="overlap"):
+                k.fp4_read(pool, slots, *pair)
+    if dtype is torch.float32:
+        own = torch.zeros((3, 128), device=DEV)
+        own.view(torch.int32).view(-1)[5:8] = slots
+        with pytest.raises(KernelError, match="overlap"):
+            k.fp4_read(pool, own.view(torch.int32).view(-1)[5:8], own, rows[:3, :128])
+    torch.cuda.synchronize()
+    assert bool((rows == 5).all())
+    want = [torch.empty((3, 128), dtype=dtype, device=DEV) for _ in range(2)]
+    k.fp4_read(pool, slots, *want)
+    for keys, values in ((rows[:3, :128], rows[:3, 128:256]), (rows[:3, 272:], rows[:3, :128]), (rows[:3, :128], rows[3:, :128]),
+                         (rows[:3, :128], rows[2:5, 200:328])):
+        rows.fill_(5.0)
+        k.fp4_read(pool, slots, keys, values)
+        assert torch.equal(keys, want[0]) and torch.equal(values, want[1])
+
+
 def test_no_memory_of_a_call_in_noted_launches():
     """Launches that are noted to be made again would use a call's memory after its end; those without any may be noted."""
     k = kernels()
