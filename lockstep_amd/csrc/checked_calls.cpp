@@ -241,7 +241,13 @@ PyObject* fp4_rows(PyObject* const* x, Py_ssize_t n, bool write) {
     void *kp = k.data_ptr(), *vp = v.data_ptr();
     const int64_t ldk = k.stride(0), ldv = v.stride(0);
     if (tokens == 0) return 0;
-    if (!write) {
+    if (write) {
+      const Area others[3] = {area(k, width), area(v, width), area(slots)};
+      for (int i = 0; i < 4; ++i) {
+        for (int j = 0; j < i; ++j) need(!meet(pool.areas[i], pool.areas[j]));
+        for (const Area& x : others) need(!meet(pool.areas[i], x));
+      }
+    } else {
       const Area keys = area(k, width), values = area(v, width), ids = area(slots);
       need((tokens <= 1 || (ldk >= width && ldv >= width)) && !meet(keys, values) && !meet(keys, ids) && !meet(values, ids));
       for (const Area& held : pool.areas) need(!meet(keys, held) && !meet(values, held));

@@ -2201,13 +2201,18 @@ class Kernels:
         """Keys and values ``[tokens, kv heads * d]`` (float32 or bfloat16, rows may be parts of wider ones) rounded to 4
         bits into the slots (page * page size + place in the page) of ``pages``; a token whose slot is negative or
         beyond the pool is left out.  Every group of 32 elements gets a power of two as its scale; a group with an
-        infinity or a NaN is held as NaN.  The slots of a call are distinct: of two tokens with one slot a mix remains."""
+        infinity or a NaN is held as NaN.  The slots of a call are distinct: of two tokens with one slot a mix remains.  The
+        tensors of ``pages`` share no memory with one another or with the operands."""
         calls = self._calls
         if calls is not None and self.tape is None and calls.fp4_write(here := _raw_device(), _raw_stream(here), k, v, slots, pages):
             return
         args = self._fp4_rows("fp4_write", k, v, slots, pages)
         if args[6] == 0:
             return
+        areas = [_area(t) for t in pages]
+        others = [_area(k, k.shape[1]), _area(v, v.shape[1]), _area(slots)]
+        if any(_meet(a, b) for i, a in enumerate(areas) for b in (*areas[:i], *others)):
+            raise KernelError("fp4_write: the pages overlap one another or what is written into them")
         lib = self.serving
         self._launch_plain(lib, lib.ls_fp4_write, args)
 

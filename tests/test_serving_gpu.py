@@ -564,6 +564,35 @@ def test_reading_refuses_rows_in_its_operands(route, dtype):
         assert torch.equal(keys, want[0]) and torch.equal(values, want[1])
 
 
+def test_writing_refuses_operands_in_the_pages(route):
+    k = kernels()
+    pool = Fp4Pages.empty(4, 2, 16, 64, device=DEV)
+    x, slots = torch.ones((3, 128), device=DEV), i32([0, 1, 2])
+    inside = pool.v_codes.view(-1)[64:64 + 3 * 512].view(torch.float32).view(3, 128)
+    scales = pool.k_scales.view(-1)[16:28].view(torch.int32)
+    shifted = torch.zeros(2 * pool.k_scales.numel(), dtype=torch.uint8, device=DEV)
+    half = pool.k_scales.numel()
+    for args in ((inside, x, slots, pool), (x, inside, slots, pool), (x, x, scales, pool),
+                 (x, x, slots, pool._replace(v_codes=pool.k_codes.view(pool.v_codes.shape))),
+                 (x, x, slots, pool._replace(v_scales=pool.k_scales.view(pool.v_scales.shape))),
+                 (x, x, slots, pool._replace(k_scales=shifted[:half].view(pool.k_scales.shape),
+                                             v_scales=shifted[half - 16:2 * half - 16].view(pool.v_scales.shape)))):
+        with pytest.raises(KernelError, match="overlap"):
+            k.fp4_write(*args)
+    torch.cuda.synchronize()
+    assert not any(bool(t.any()) for t in pool)
+    # pages that lie behind one another in one allocation, and one tensor as keys and values: taken
+    whole = torch.zeros(sum(t.numel() for t in pool), dtype=torch.uint8, device=DEV)
+    parts, at = [], 0
+    for t in pool:
+        parts.append(whole[at:at + t.numel()].view(t.shape))
+        at += t.numel()
+    k.fp4_write(x, x, slots, Fp4Pages(*parts))
+    keys, values = torch.zeros_like(x), torch.zeros_like(x)
+    k.fp4_read(Fp4Pages(*parts), slots, keys, values)
+    assert torch.equal(keys, x) and torch.equal(values, x)
+
+
 def test_no_memory_of_a_call_in_noted_launches():
     """Launches that are noted to be made again would use a call's memory after its end; those without any may be noted."""
     k = kernels()
