@@ -331,6 +331,12 @@ PyObject* token_logprobs(PyObject*, PyObject* const* x, Py_ssize_t n) {
     need(top <= bound.max_top && top <= vocab);
     if (rows == 0) return 0;
     need(vocab >= 1 && vocab <= bound.max_vocab);
+    const Area outs[5] = {area(tensor(x[4])), area(tensor(x[5])), area(tensor(x[6])), area(ids), area(theirs)};
+    const Area ins[2] = {area(logits, vocab), area(tensor(x[3]))};
+    for (int i = 0; i < 5; ++i) {
+      for (int j = 0; j < i; ++j) need(!meet(outs[i], outs[j]));
+      for (const Area& in : ins) need(!meet(outs[i], in));
+    }
     const int64_t bytes = bound.logprobs_scratch((int)rows, (int)vocab);
     const Tensor scratch = call_scratch(bytes, logits);
     void* memory = bytes > 0 ? scratch.data_ptr() : nullptr;

@@ -2300,7 +2300,8 @@ class Kernels:
         """Log probabilities of the given ``tokens [rows]`` (int32) under the softmax of ``logits [rows, vocabulary]``
         (float32 or bfloat16): ``logprob`` and ``entropy`` (natural logarithms, float32 ``[rows]``), ``rank`` (int32: how many
         tokens come before it, larger logits first, then lower ids) and the first ``k`` tokens of that order, ``top_ids``
-        (int32) and ``top_logprobs`` (float32) ``[rows, k]``, k from 0 to 32 and at most the vocabulary.
+        (int32) and ``top_logprobs`` (float32) ``[rows, k]``, k from 0 to 32 and at most the vocabulary.  Outputs share no memory
+        with one another or with an input.
 
         A token outside the vocabulary (-1: none) gets NaN and the rank -1.  A NaN counts as larger than every number; rows
         with a NaN, with an infinity of +, or with nothing but -inf have NaN for what the formula leaves undefined."""
@@ -2331,6 +2332,10 @@ class Kernels:
                               f"on GPU {device}, got {top_ids.dtype} {list(shape)} and {top_logprobs.dtype} {list(top_logprobs.shape)}")
         if rows == 0:
             return
+        outs = [_area(t) for t in (logprob, entropy, rank, top_ids, top_logprobs)]
+        ins = (_area(logits, vocab), _area(tokens))
+        if any(_meet(a, b) for i, a in enumerate(outs) for b in (*outs[:i], *ins)):
+            raise KernelError("token_logprobs: outputs overlap one another or an input")
         if not (1 <= vocab <= widest and rows <= 0x7FFFFFFF):
             raise KernelError(f"token_logprobs takes 1 to {widest} logits a row and 31 bits of rows, got {rows} of {vocab}")
         need = lib.ls_logprobs_scratch_bytes(rows, vocab)

@@ -593,6 +593,28 @@ def test_writing_refuses_operands_in_the_pages(route):
     assert torch.equal(keys, x) and torch.equal(values, x)
 
 
+def test_logprobs_refuse_outputs_in_their_operands(route):
+    k = kernels()
+    f, i = (lambda *s: torch.full(s, 9.0, device=DEV)), (lambda *s: torch.full(s, 9, dtype=torch.int32, device=DEV))
+    logits = torch.randn((6, 50), generator=torch.Generator().manual_seed(32)).to(DEV)
+    before = logits.clone()
+    base = dict(logits=logits, tokens=i32([1, 2, 3, 4, 5, 6]), logprob=f(6), entropy=f(6), rank=i(6), top_ids=i(6, 4), top_logprobs=f(6, 4))
+    both, ints = f(11), i(24 + 6)
+    for change in (dict(entropy=base["logprob"]), dict(logprob=both[:6], entropy=both[5:]), dict(rank=base["tokens"]),
+                   dict(rank=base["logprob"].view(torch.int32)), dict(top_ids=base["top_logprobs"].view(torch.int32)),
+                   dict(rank=ints[:6], top_ids=ints[5:29].view(6, 4)), dict(logprob=logits.view(-1)[100:106]),
+                   dict(top_logprobs=logits.view(-1)[276:].view(6, 4)), dict(tokens=ints[23:29], top_ids=ints[:24].view(6, 4))):
+        with pytest.raises(KernelError, match="overlap"):
+            k.token_logprobs(**{**base, **change})
+    torch.cuda.synchronize()
+    assert torch.equal(logits, before) and bool((both == 9).all()) and bool((ints == 9).all())
+    k.token_logprobs(**base)
+    one = f(12)
+    near = dict(logprob=one[:6], entropy=one[6:], rank=ints[:6], top_ids=ints[6:].view(6, 4))       # behind one another: taken
+    k.token_logprobs(**{**base, **near})
+    assert all(torch.equal(x, base[name]) for name, x in near.items())
+
+
 def test_no_memory_of_a_call_in_noted_launches():
     """Launches that are noted to be made again would use a call's memory after its end; those without any may be noted."""
     k = kernels()
