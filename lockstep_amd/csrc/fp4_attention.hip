@@ -79,11 +79,22 @@ __host__ __device__ inline int decode_split(int span, int kv_heads) {
   const int even = (int)(((long)span * kv_heads + kDecodeGroups - 1) / kDecodeGroups);
   return max(shortest_split(span, kv_heads), (even + 127) / 128 * 128);
 }
-// The same for prompts, by how many workgroups its rows fill.
-constexpr int kPromptGroups = 512, kPromptShortest = 256;
-__host__ __device__ inline int prompt_split(int span, int groups, int kv_heads) {
-  const int want = max(1, kPromptGroups / (max(1, groups) * kv_heads));
-  return max(kPromptShortest, ((span + want - 1) / want + 63) / 64 * 64);  // whole tiles of 64
+// The same for prompts, by how many workgroups its rows fill.  A split leaves 4 (D + 2) bytes a row, written and read again, and
+// reads 17/16 D a key: with bfloat16 operands one is no shorter than four keys a row, so that many portions of a few tokens
+// behind long contexts do not move more sums than keys, up to 1,024 keys, from where on the products take longer.  (32 heads over
+// 8 of 128, all splits down to 256 keys / by rows: 64 requests of 33 tokens behind 8,192 keys 1,260 us and 1.1 GB for sums / 875
+// and 0.6; 16 of 64 behind 4,096 229 / 119, 4 of 128 106 / 67; one of 33 behind 8,192 36 / 33, behind 1,000 21 / 28.)  The float32
+// path has three products for one, so its sums weigh a third: 7 requests of up to 129 tokens of 12 heads over 4 of 64 with a
+// window of 500 34 / 41 to 47.
+constexpr int kPromptGroups = 512, kPromptShortest = 256, kPromptShortMost = 1024;
+template <typename T> __host__ __device__ inline int shortest_prompt_split(int rows) {
+  if (sizeof(T) == 4 || rows <= kPromptShortest / 4) return kPromptShortest;
+  return rows >= kPromptShortMost / 4 ? kPromptShortMost : (4 * rows + 63) / 64 * 64;
+}
+__host__ __device__ inline int prompt_splits_wanted(int groups, int kv_heads) { return max(1, kPromptGroups / (max(1, groups) * kv_heads)); }
+template <typename T> __host__ __device__ inline int prompt_split(int span, int groups, int kv_heads, int rows) {
+  const int want = prompt_splits_wanted(groups, kv_heads);
+  return max(shortest_prompt_split<T>(rows), ((span + want - 1) / want + 63) / 64 * 64);  // whole tiles of 64
 }
 
 // How a request of `rows` rows a head whose rows see `span` keys is cut: the same in the kernels and on the host.
@@ -96,7 +107,7 @@ template <typename T>
 __host__ __device__ inline Cut cut_request(int rows, int span, int kv_heads) {
   Cut c;
   c.groups = rows <= kFewRows ? 0 : (rows + kGroupRows<T> - 1) / kGroupRows<T>;
-  c.len = c.groups == 0 ? decode_split(span, kv_heads) : prompt_split(span, c.groups, kv_heads);
+  c.len = c.groups == 0 ? decode_split(span, kv_heads) : prompt_split<T>(span, c.groups, kv_heads, rows);
   c.splits = max(1, (span + c.len - 1) / c.len);
   return c;
 }
@@ -122,37 +133,31 @@ struct Fp4Args {
   int window;
   float* part_acc;         // [entries][D]: the sums of a row's split (see split_entry)
   float* part_ml;          // [entries][2]: reference, sum of the weights
-  int region;              // entries a request's head, or (by_row) a query head of a row of q
-  bool by_row;
+  long per_row, per_request, head_entries;  // room for entries that a row of q and a request have, and a head in all
 };
 
 // One request as all kernels see it.
 struct Request {
-  int first, rows, start, base, end;  // first packed row, rows a head, first position, keys that are seen: base .. end - 1
+  int first, tokens, rows, start, base, end;  // first packed row, rows, rows a head, first position, keys that are seen: base .. end - 1
   __device__ __forceinline__ Request(const Fp4Args& a, int b) {
     const int from = a.offsets[b], to = a.offsets[b + 1];
     const bool ok = from >= 0 && to >= from && to <= a.rows && to - from <= a.most;
     first = ok ? from : 0;
-    const int n = ok ? to - from : 0;
-    rows = n * a.group;
+    tokens = ok ? to - from : 0;
+    rows = tokens * a.group;
     const int room = (int)min((long)a.columns << a.pool.page_shift, (long)a.longest);  // (a few tiles on stay below 2^31)
     end = min(max(a.lengths[b], 0), room);
-    start = end - n;
+    start = end - tokens;
     base = first_tile(start, a.window);
   }
 };
 
-// Where the sums of a split of row r (of `stride` rows, padding included) of a head lie, -1 where there is no room.  By request
-// or by row of q, whichever takes less: prompts of one length lie close together by request, a prompt beside many decoded
-// tokens does by row.
-__device__ __forceinline__ long split_entry(const Fp4Args& a, const Request& rq, int b, int head, int split, int stride, int r) {
-  if (a.by_row) {
-    const int token = r / a.group;
-    const long row = (long)(rq.first + token) * a.pool.kv_heads * a.group + head * a.group + (r - token * a.group);
-    return split < a.region ? row * a.region + split : -1;
-  }
-  const long entry = (long)split * stride + r;
-  return entry < a.region ? ((long)b * a.pool.kv_heads + head) * a.region + entry : -1;
+// Where the sums of a split of row r of a head lie, -1 where there is no room.  The entries of a request of n tokens lie between
+// those of the requests before it and after it: `per_row` n + `per_request` are its own, which is never less than what it leaves.
+__device__ __forceinline__ long split_entry(const Fp4Args& a, const Request& rq, int b, int head, int split, int r) {
+  const long entry = (long)split * rq.rows + r;
+  if (entry >= a.per_row * rq.tokens + a.per_request) return -1;
+  return head * a.head_entries + a.per_row * rq.first + a.per_request * b + entry;
 }
 
 struct KeyTile {  // what a lane has of 32 keys and values, as they lie in the pages
@@ -652,7 +657,7 @@ __device__ __forceinline__ void decode_part(const Fp4Args& a, FoldShared& fold, 
       const int token = r / a.group, sub = r - token * a.group;
       store_run<T>(static_cast<T*>(a.out) + (long)(rq.first + token) * a.ldo + (long)(head * a.group + sub) * D + d, x, 4);
     } else {
-      const long at = split_entry(a, rq, b, head, split, 16, r);
+      const long at = split_entry(a, rq, b, head, split, r);
       if (at >= 0) {
         store_run<float>(a.part_acc + at * D + d, x, 4);
         if (d == 0) {
@@ -952,7 +957,6 @@ __device__ __forceinline__ void prompt_part(const Fp4Args& a, PromptShared& shar
   auto& flags = shared.flags;
   const Request rq(a, b);
   if (rq.rows <= kFewRows) return;
-  const int blocks = (rq.rows + kBlock - 1) / kBlock;
   const Cut cut = cut_request<T>(rq.rows, rq.end - rq.base, a.pool.kv_heads);
   const int groups = cut.groups, splits = cut.splits, len = cut.len;
   if (place >= groups * splits) return;
@@ -1007,7 +1011,7 @@ __device__ __forceinline__ void prompt_part(const Fp4Args& a, PromptShared& shar
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int token = there ? r / a.group : 0, sub = there ? r - token * a.group : 0;
     T* out = static_cast<T*>(a.out) + (long)(rq.first + token) * a.ldo + (long)(head * a.group + sub) * D;
-    const long at = there ? split_entry(a, rq, b, head, split, blocks * kBlock, r) : -1;
+    const long at = there ? split_entry(a, rq, b, head, split, r) : -1;
     const bool keep = at >= 0;
     if (splits > 1 && keep && j == 0) {
       a.part_ml[2 * at] = rows.m[t];
@@ -1056,13 +1060,10 @@ template <typename T, bool kWaveEach>
 __global__ __launch_bounds__(kThreads) void fp4_combine_kernel(Fp4Args a) {  // grid ((row, head) pairs of a request, requests)
   __shared__ float factor[kWaveEach ? 1 : kMostSplits];
   __shared__ float part[kWaveEach ? 1 : 4][D];
-  constexpr int kBlock = 16 * kPromptTiles<T>;
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int heads = a.group * a.pool.kv_heads, b = blockIdx.y;
   const Request rq(a, b);
-  const int blocks = (rq.rows + kBlock - 1) / kBlock;
-  const Cut cut = cut_request<T>(rq.rows, rq.end - rq.base, a.pool.kv_heads);
-  const int splits = cut.splits, stride = cut.groups == 0 ? 16 : blocks * kBlock;
+  const int splits = cut_request<T>(rq.rows, rq.end - rq.base, a.pool.kv_heads).splits;
   if (splits <= 1 || splits > kMostSplits) return;
   const int pairs = rq.rows * a.pool.kv_heads, stride_pairs = kWaveEach ? 4 * gridDim.x : gridDim.x;
   constexpr int kEach = (D + 63) / 64;
@@ -1070,8 +1071,8 @@ __global__ __launch_bounds__(kThreads) void fp4_combine_kernel(Fp4Args a) {  // 
   for (int place = kWaveEach ? 4 * blockIdx.x + w : blockIdx.x; place < pairs; place += stride_pairs) {
     const int token = place / heads, query_head = place - token * heads, row = rq.first + token;
     const int head = query_head / a.group, r = token * a.group + (query_head - head * a.group);
-    const long base = split_entry(a, rq, b, head, 0, stride, r), apart = a.by_row ? 1 : stride;
-    if (split_entry(a, rq, b, head, splits - 1, stride, r) < 0) return;
+    const long base = split_entry(a, rq, b, head, 0, r), apart = rq.rows;
+    if (split_entry(a, rq, b, head, splits - 1, r) < 0) return;
     T* out = static_cast<T*>(a.out) + (long)row * a.ldo + (long)query_head * D;
     const auto sum_at = [&](int s, int y) LS_INLINED -> float { return a.part_acc[(base + s * apart) * D + min(d0 + y, D - 1)]; };
     // (asked for before the factors are known)
@@ -1139,41 +1140,70 @@ __global__ __launch_bounds__(kThreads) void fp4_combine_kernel(Fp4Args a) {  // 
 }
 
 struct Plan {
-  int decode_splits, prompt_places, region, most_splits;  // places: row blocks of a workgroup times splits, of a request's head
+  int decode_splits = 1, prompt_places = 0;  // places: row blocks of a workgroup times splits, of a request's head
+  bool fold = false;                         // a request may have more than one split
+  long per_row = 0, per_request = 0, head_entries = 0;
 };
 
-// What is launched for requests of at most `most` tokens and `longest` keys: bounds for every shorter one.  (In host code the plain
-// min and max are those of int: what may pass 31 bits takes the standard library's.)
+// What is launched for `requests` requests with `rows` rows, of at most `most` tokens and `longest` keys: bounds for every such step.
+// (In host code the plain min and max are those of int: what may pass 31 bits takes the standard library's.)
 template <typename T>
-Plan make_plan(int kv_heads, int group, int most, int longest, int window) {
-  Plan p{1, 0, 0, 1};
+Plan make_plan(int kv_heads, int group, int rows, int requests, int most, int longest, int window) {
+  Plan p;
+  // What requests of so many tokens leave a head at most, at both ends of every run of lengths (behind its first a sixth more: 17 to
+  // 32,768 tokens are 49 runs): between them it is no more than on the straight line, and where it reaches `most_entries`, which
+  // no prompt passes, it stays there.
+  struct End {
+    long tokens, entries;
+  } ends[128];
+  int used = 0;
+  const auto run_of = [&](long first, long last, int splits, long most_entries) {
+    ends[used++] = {first, std::min<long>(first * group * splits, most_entries)};
+    ends[used++] = {std::min<long>(last, std::max<long>(first, most_entries / ((long)group * splits))), std::min<long>(last * group * splits, most_entries)};
+  };
   // the keys that a request's rows see, at most: with a window those of its tokens and the window before, in whole tiles
   const auto seen = [&](int n) { return window > 0 ? (int)std::min<long>(longest, (long)n + window - 1 + kSharedKeys) : longest; };
-  const int span = seen(min(max(1, kFewRows / group), most));
+  const int few = kFewRows / group, span = seen(min(max(1, few), most));
   if (span > kOneSplit) {
     const auto most_of = [&](int n) { return (n + shortest_split(n, kv_heads) - 1) / shortest_split(n, kv_heads); };
     p.decode_splits = min(max(most_of(span), most_of(min(span, 4096))), (kDecodeGroups + kv_heads - 1) / kv_heads);
-    p.region = 16 * p.decode_splits;
-    p.most_splits = p.decode_splits;
+    if (p.decode_splits > 1 && few > 0) run_of(1, min(few, most), p.decode_splits, kFewRows * (long)p.decode_splits);
   }
-  const long rows = (long)most * group;
-  if (rows > kFewRows) {
-    // a request with more than one split has `want` places at most, and no split is shorter than the shortest
-    const int want = max(1, kPromptGroups / kv_heads), far = seen(most);
-    p.prompt_places = (int)((rows + kGroupRows<T> - 1) / kGroupRows<T>);
-    if (want > 1 && far > kPromptShortest) {
-      p.prompt_places = (int)std::max<long>(p.prompt_places, std::min<long>(want, (long)p.prompt_places * ((far + kPromptShortest - 1) / kPromptShortest)));
-      p.region = max(p.region, want * kGroupRows<T>);
-      p.most_splits = max(p.most_splits, min(want, (far + kPromptShortest - 1) / kPromptShortest));
+  if (most > few) {
+    const auto groups_of = [&](int n) { return (int)(((long)n * group + kGroupRows<T> - 1) / kGroupRows<T>); };
+    p.prompt_places = groups_of(most);
+    // (a run's first length has most splits)
+    for (int n = few + 1, last; n <= most; n = last + 1) {
+      const int groups = groups_of(n), want = prompt_splits_wanted(groups, kv_heads);
+      if (want == 1) break;  // nor has any longer one more than one split
+      last = min(most, n + n / 6);
+      const int shortest = shortest_prompt_split<T>((int)std::min<long>((long)n * group, kPromptShortMost));
+      const int splits = min(want, (seen(last) + shortest - 1) / shortest);
+      if (splits > 1) {
+        const int places = prompt_splits_wanted(1, kv_heads);  // of a request with more than one split, at most
+        run_of(n, last, splits, (long)places * kGroupRows<T>);
+        p.prompt_places = max(p.prompt_places, min(places, groups_of(last) * splits));
+      }
     }
   }
+  p.fold = used > 0;
+  // Room by rows, by requests or some of each, whichever takes least: with so much a row, a request has what it may still lack.
+  for (long splits = 0; p.fold && splits <= kDecodeGroups; splits = splits ? 2 * splits : 1)
+    for (const long per_row : {splits * group, (long)p.decode_splits * group}) {
+      long lacks = 0;
+      for (int i = 0; i < used; ++i) lacks = std::max<long>(lacks, ends[i].entries - per_row * ends[i].tokens);
+      const long all = per_row * rows + lacks * requests;
+      if (p.head_entries == 0 || all < p.head_entries) {
+        p.per_row = per_row;
+        p.per_request = lacks;
+        p.head_entries = all;
+      }
+    }
   return p;
 }
 
-// Splits' sums that a step may leave.
-inline long entries_of(const Plan& p, int kv_heads, int group, int requests, int rows) {
-  return p.region == 0 ? 0 : std::min<long>((long)requests * kv_heads * p.region, (long)rows * kv_heads * group * p.most_splits);
-}
+// Bytes of the splits' sums that a step may leave.
+inline long bytes_of(const Plan& p, int kv_heads) { return p.head_entries * kv_heads * (D + 2) * (long)sizeof(float); }
 
 template <typename T, bool kWholePages>
 void launch_parts(const Fp4Args& a, const Plan& p, hipStream_t stream) {
@@ -1186,19 +1216,16 @@ void launch_parts(const Fp4Args& a, const Plan& p, hipStream_t stream) {
 
 template <typename T>
 int run_fp4(Fp4Args& a, int most, int longest, void* scratch, long scratch_bytes, hipStream_t stream) {
-  const Plan p = make_plan<T>(a.pool.kv_heads, a.group, most, longest, a.window);
   const int heads = a.pool.kv_heads;
-  const long entries = entries_of(p, heads, a.group, a.requests, a.rows);
-  a.by_row = entries != (long)a.requests * heads * p.region;
-  a.region = a.by_row ? p.most_splits : p.region;
+  const Plan p = make_plan<T>(heads, a.group, a.rows, a.requests, most, longest, a.window);
+  a.per_row = p.per_row; a.per_request = p.per_request; a.head_entries = p.head_entries;
   LS_REQUIRE((long)p.prompt_places + p.decode_splits <= 65535, "fp4_attention: %d rows a request", most);
-  LS_REQUIRE(scratch_bytes >= entries * (D + 2) * (long)sizeof(float), "fp4_attention: %ld bytes of scratch, %ld needed",
-             scratch_bytes, entries * (D + 2) * (long)sizeof(float));
+  LS_REQUIRE(scratch_bytes >= bytes_of(p, heads), "fp4_attention: %ld bytes of scratch, %ld needed", scratch_bytes, bytes_of(p, heads));
   a.part_acc = static_cast<float*>(scratch);
-  a.part_ml = a.part_acc + entries * D;
+  a.part_ml = a.part_acc + p.head_entries * heads * D;
   if (a.pool.page_shift >= 4) launch_parts<T, true>(a, p, stream);
   else launch_parts<T, false>(a, p, stream);
-  if (p.region > 0) {
+  if (p.fold) {
     const long pairs = (long)most * a.group * heads;  // of the request with most
     LS_REQUIRE(pairs <= 0x7ffffff0l, "fp4_attention: %d rows of %d heads", most, a.group * heads);
     if (pairs * a.requests >= 2048)
@@ -1218,25 +1245,21 @@ extern "C" int ls_fp4_attention_head_dim() { return ls::D; }
 extern "C" long ls_fp4_attention_scratch_bytes(int dtype, int rows, int requests, int kv_heads, int group, int most, int longest, int window) {
   using namespace ls;
   if (rows <= 0 || requests <= 0 || kv_heads <= 0 || group <= 0 || most <= 0) return 0;
-  const Plan p = dtype == kF32 ? make_plan<float>(kv_heads, group, most, longest, window)
-                               : make_plan<bf16_t>(kv_heads, group, most, longest, window);
-  return entries_of(p, kv_heads, group, requests, rows) * (D + 2) * (long)sizeof(float);
+  return bytes_of(dtype == kF32 ? make_plan<float>(kv_heads, group, rows, requests, most, longest, window)
+                                : make_plan<bf16_t>(kv_heads, group, rows, requests, most, longest, window), kv_heads);
 }
 
 namespace ls {
 template <typename T>
 void plan_of(int rows, int requests, int kv_heads, int group, int most, int longest, int window, int tokens, int length, long* out) {
-  const Plan p = make_plan<T>(kv_heads, group, most, longest, window);
+  const Plan p = make_plan<T>(kv_heads, group, rows, requests, most, longest, window);
   const Cut c = cut_request<T>(tokens * group, length - first_tile(length - tokens, window), kv_heads);
-  const long entries = entries_of(p, kv_heads, group, requests, rows);
-  const bool by_row = entries != (long)requests * kv_heads * p.region;
-  const int block = 16 * kPromptTiles<T>, padded = c.groups == 0 ? 16 : (tokens * group + block - 1) / block * block;
   out[0] = c.splits;
   out[1] = c.groups == 0 ? c.splits : (long)c.groups * c.splits;
   out[2] = c.groups == 0 ? p.decode_splits : p.prompt_places;
-  out[3] = c.splits == 1 ? 0 : (long)c.splits * (by_row ? tokens * group : padded);
-  out[4] = by_row ? (long)tokens * group * p.most_splits : p.region;
-  out[5] = entries;
+  out[3] = c.splits == 1 ? 0 : (long)c.splits * tokens * group;
+  out[4] = p.per_row * tokens + p.per_request;
+  out[5] = p.head_entries;
 }
 }  // namespace ls
 

@@ -14,7 +14,7 @@ int ls_fp4_attention_head_dim();
 long ls_fp4_attention_scratch_bytes(int dtype, int rows, int requests, int kv_heads, int group, int most, int longest, int window);
 // How a request of `tokens` rows and `length` keys is cut in such a step, and what the launch has for it (host code, nothing is
 // launched): out[0] its splits; its workgroups a head [1] and how many there are at most [2]; splits' sums a head that it
-// leaves [3], how many have room [4], and how many the scratch holds in all [5].
+// leaves [3], how many have room [4], and how many the scratch holds a head [5].
 int ls_fp4_attention_plan(int dtype, int rows, int requests, int kv_heads, int group, int most, int longest, int window, int tokens,
                           int length, long* out);
 int ls_fp4_attention(int dtype, const void* q, long ldq, void* out, long ldo, int rows, const void* k_codes,

@@ -178,3 +178,28 @@ def test_areas_that_share_memory():
     x = torch.zeros(10)
     assert _meet(_area(x), _area(x[9:])) and not _meet(_area(x[:9]), _area(x[9:])) and not _meet(_area(x), _area(x[:0]))
     assert _meet(_area(x[2:3].expand(4, 3), 3), _area(x)) and not _meet(_area(x[:0].reshape(0, 3), 3), _area(x))
+
+
+def test_splits_leave_no_more_sums_than_they_read_keys():
+    """With bfloat16 operands a request of up to 256 rows a head leaves at most what its keys and values take in their pages, but
+    for one split's sums (the last split is shorter than the others)."""
+    plan = plan_entry(128)
+    for group in (1, 2, 4, 8, 16):
+        for tokens in {t for t in (1, 3, 5, 9, 17, 20, 33, 64, 100, 256) if t * group <= 256}:
+            for length in (300, 800, 1000, 2100, 4096, 8192, 32768, 131072):
+                for heads in (1, 2, 8):
+                    splits, _, _, entries, _, _ = plan(torch.bfloat16, 256, 4, heads, group, 256, length, 0, tokens, length)
+                    rows = tokens * group
+                    assert splits == 1 or (entries - rows) * (128 + 2) * 4 <= length * 128 * 17 // 16, (group, tokens, length, heads)
+
+
+@pytest.mark.parametrize("rows,requests,most,longest", [(64 * 33, 64, 33, 8192), (63 + 2048, 64, 2048, 8192), (255 + 2048, 256, 2048, 32768),
+                                                        (255 + 8192, 256, 8192, 131072), (64, 64, 1, 8192)])
+def test_memory_of_a_step_is_less_than_its_pages(rows, requests, most, longest):
+    """The splits' sums of many short portions, and of a prompt beside decoded tokens, against the pages of such requests (32 heads
+    over 8 of 128): a third more at most, where many requests may be of a few tokens behind 8,192 keys."""
+    lib = ctypes.CDLL(str(kernel_build.build_fp4_attention(128)))
+    count = lib.ls_fp4_attention_scratch_bytes
+    count.restype = ctypes.c_long
+    pages = requests * longest * 8 * 128 * 17 // 16
+    assert 0 < count(1, rows, requests, 8, 4, most, longest, 0) <= pages * 4 // 3
