@@ -2060,15 +2060,16 @@ class Kernels:
             lib.ls_fp4_write.argtypes = [i, p, n, p, n, p, i, i, i, p, p, p, p, i, i, p]
             lib.ls_fp4_read.argtypes = lib.ls_fp4_write.argtypes
             lib.ls_token_logprobs.argtypes = [i, p, n, p, i, i, i, p, p, p, p, p, p, n, p]
-            self._serving = lib
-            self.serving_path = str(path)
             self._serving_limits = (int(lib.ls_step_tables_max_requests()), int(lib.ls_logprobs_max_top()),
                                     int(lib.ls_logprobs_max_vocab()))
             if _raw_stream is not None and _raw_device is not None and torch.cuda.is_available():
-                self._calls = _load_calls()
-                if self._calls is not None:
+                calls = _load_calls()
+                if calls is not None:
                     entries = (lib.ls_step_tables, lib.ls_fp4_write, lib.ls_fp4_read, lib.ls_token_logprobs, lib.ls_logprobs_scratch_bytes)
-                    self._calls.bind_serving(*map(_address, entries), *self._serving_limits)
+                    calls.bind_serving(*map(_address, entries), *self._serving_limits)
+                self._calls = calls
+            self.serving_path = str(path)
+            self._serving = lib                 # last: another thread that finds it finds the rest
         return self._serving
 
     def fp4_attention_lib(self, head_dim: int):
@@ -2083,11 +2084,11 @@ class Kernels:
             lib.ls_fp4_attention.argtypes = [i, p, n, p, n, i, p, p, p, p, i, i, i, i, p, i, p, p, i, i, i, c_float, i, p, n, p]
             if not (lib.ls_fp4_attention_head_dim() == head_dim):
                 raise KernelError(f"{path} was built for another head size")
-            self._fp4_attention[head_dim] = lib
-            self.fp4_attention_paths[head_dim] = str(path)
             self.serving                        # (loads the extension module)
             if self._calls is not None:
                 self._calls.bind_attention(head_dim, _address(lib.ls_fp4_attention), _address(lib.ls_fp4_attention_scratch_bytes))
+            self.fp4_attention_paths[head_dim] = str(path)
+            self._fp4_attention[head_dim] = lib
         return lib
 
     def _launch_plain(self, lib, entry, args: tuple) -> None:

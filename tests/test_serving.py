@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes
 import random
+import threading
 
 import pytest
 import torch
@@ -203,3 +204,37 @@ def test_memory_of_a_step_is_less_than_its_pages(rows, requests, most, longest):
     count.restype = ctypes.c_long
     pages = requests * longest * 8 * 128 * 17 // 16
     assert 0 < count(1, rows, requests, 8, 4, most, longest, 0) <= pages * 4 // 3
+
+
+def test_a_library_is_whole_for_the_thread_that_finds_it(monkeypatch):
+    """While one thread loads the library, another one that asks for it gets its limits too."""
+    from lockstep_amd.ops.kernels import Kernels
+
+    k = Kernels.__new__(Kernels)
+    k._serving = k._calls = None
+    failed, asked = [], []
+
+    def other():
+        try:
+            assert k.serving is not None and len(k._serving_limits) == 3
+        except Exception as exc:  # noqa: BLE001 - reported below
+            failed.append(exc)
+
+    real = ctypes.CDLL
+
+    class Library:
+        """The library, whose first call lets another thread in (as every call does that releases the interpreter's lock)."""
+
+        def __init__(self, path):
+            self.__dict__["lib"] = real(path)
+
+        def __getattr__(self, name):
+            if name == "ls_step_tables_max_requests" and not asked:
+                asked.append(threading.Thread(target=other))
+                asked[0].start()
+                asked[0].join()
+            return getattr(self.lib, name)
+
+    monkeypatch.setattr(ctypes, "CDLL", Library)
+    assert k.serving is not None
+    assert len(asked) == 1 and not failed, failed
