@@ -85,6 +85,7 @@ struct Bound {
   decltype(&ls_token_logprobs) token_logprobs;
   decltype(&ls_logprobs_scratch_bytes) logprobs_scratch;
   int64_t max_requests, max_top, max_vocab;
+  PyTypeObject* pages;  // the type of a pool of pages in 4 bits
   struct {
     decltype(&ls_fp4_attention) run;
     decltype(&ls_fp4_attention_scratch_bytes) scratch;
@@ -120,7 +121,8 @@ int without_gil(F call) {
 }
 
 PyObject* bind_serving(PyObject*, PyObject* const* x, Py_ssize_t n) {
-  return accepted(n, 8, [&] {
+  return accepted(n, 9, [&] {
+    need(PyType_Check(x[8]));
     bind(bound.step_tables, x[0]);
     bind(bound.fp4_write, x[1]);
     bind(bound.fp4_read, x[2]);
@@ -129,6 +131,8 @@ PyObject* bind_serving(PyObject*, PyObject* const* x, Py_ssize_t n) {
     bound.max_requests = integer(x[5]);
     bound.max_top = integer(x[6]);
     bound.max_vocab = integer(x[7]);
+    Py_INCREF(x[8]);
+    bound.pages = reinterpret_cast<PyTypeObject*>(x[8]);
     return 0;
   });
 }
@@ -201,7 +205,7 @@ struct Pool {  // a pool of pages in 4 bits, checked
   void* data[4];
   Area areas[4];
   Pool(PyObject* o, int device) {
-    need(PyTuple_Check(o) && PyTuple_GET_SIZE(o) == 4);
+    need(bound.pages != nullptr && PyObject_TypeCheck(o, bound.pages) && PyTuple_Check(o) && PyTuple_GET_SIZE(o) == 4);
     const Tensor& codes = tensor(PyTuple_GET_ITEM(o, 0));
     need(codes.dim() == 4);
     pages = codes.size(0);

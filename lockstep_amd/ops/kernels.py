@@ -2066,7 +2066,7 @@ class Kernels:
                 calls = _load_calls()
                 if calls is not None:
                     entries = (lib.ls_step_tables, lib.ls_fp4_write, lib.ls_fp4_read, lib.ls_token_logprobs, lib.ls_logprobs_scratch_bytes)
-                    calls.bind_serving(*map(_address, entries), *self._serving_limits)
+                    calls.bind_serving(*map(_address, entries), *self._serving_limits, Fp4Pages)
                 self._calls = calls
             self.serving_path = str(path)
             self._serving = lib                 # last: another thread that finds it finds the rest
@@ -2181,8 +2181,14 @@ class Kernels:
             ins[0][0], ins[1][0], requests, outs[6][0], columns, page_size, ins[2][0], free_pages.numel(), ins[3][0],
             outs[0][0], outs[1][0], outs[2][0], tokens, outs[3][0], outs[4][0], outs[5][0], stream))
 
+    @staticmethod
+    def _fp4_geometry(what: str, pages) -> tuple[int, int, int, int]:
+        if not isinstance(pages, Fp4Pages):
+            raise KernelError(f"{what}: pages in 4 bits are an Fp4Pages, got {type(pages).__name__}")
+        return pages.geometry()
+
     def _fp4_rows(self, what: str, k, v, slots, pages: Fp4Pages):
-        count, kv_heads, page_size, d = pages.geometry()
+        count, kv_heads, page_size, d = self._fp4_geometry(what, pages)
         device = pages.k_codes.get_device()
         stream = self._current(device, what)
         shape = (slots.numel(), kv_heads * d)
@@ -2255,7 +2261,7 @@ class Kernels:
                 here := _raw_device(), _raw_stream(here), q, nq, nkv, d, pages, table, offsets, lengths, max_tokens, max_length, out,
                 scale, window):
             return
-        count, kv_heads, page_size, dim = pages.geometry()
+        count, kv_heads, page_size, dim = self._fp4_geometry("fp4_attention", pages)
         device = q.get_device()
         stream = self._current(device, "fp4_attention")
         _rows_ok(q, "fp4_attention q"); _rows_ok(out, "fp4_attention out")

@@ -238,3 +238,14 @@ def test_a_library_is_whole_for_the_thread_that_finds_it(monkeypatch):
     monkeypatch.setattr(ctypes, "CDLL", Library)
     assert k.serving is not None
     assert len(asked) == 1 and not failed, failed
+
+
+def test_pages_are_fp4_pages():
+    k = kernels()
+    i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    for pages in (tuple(Fp4Pages.empty(2, 1, 16, 32, device="cpu")), list(Fp4Pages.empty(2, 1, 16, 32, device="cpu")), None):
+        for call in (lambda: k.fp4_write(torch.zeros(2, 32), torch.zeros(2, 32), i(2), pages),
+                     lambda: k.fp4_read(pages, i(2), torch.zeros(2, 32), torch.zeros(2, 32)),
+                     lambda: k.fp4_attention(torch.zeros(2, 32), 1, 1, 32, pages, i(1, 2), i(2), i(1), 2, 8, torch.zeros(2, 32), 1.0)):
+            with pytest.raises(KernelError, match="Fp4Pages"):
+                call()

@@ -808,6 +808,27 @@ def test_calls_by_the_module_and_by_python():
         assert torch.equal(a.view(torch.uint8) if a.is_floating_point() else a, b.view(torch.uint8) if b.is_floating_point() else b), i
 
 
+def test_the_module_takes_the_pages_that_python_takes(route):
+    """Four tensors that are not an Fp4Pages are refused by both, before the library is loaded and afterwards."""
+    k = kernels()
+    pool = Fp4Pages.empty(2, 2, 16, 64, device=DEV)
+    x, slots = torch.ones((3, 128), device=DEV), i32([0, 1, 2])
+    q, out = torch.zeros((1, 256), device=DEV), torch.zeros((1, 256), device=DEV)
+    table = torch.zeros((1, 2), dtype=torch.int32, device=DEV)
+    k.fp4_write(x, x, slots, pool)
+    for pages in (tuple(pool), list(pool)):
+        for call in (lambda: k.fp4_write(x, x, slots, pages), lambda: k.fp4_read(pages, slots, x, x.clone()),
+                     lambda: k.fp4_attention(q, 4, 2, 64, pages, table, i32([0, 1]), i32([3]), 1, 3, out, 0.1)):
+            with pytest.raises(KernelError, match="Fp4Pages"):
+                call()
+
+    class Mine(Fp4Pages):
+        pass
+
+    k.fp4_read(Mine(*pool), slots, x, x.clone())
+    torch.cuda.synchronize()
+
+
 # -- together ---------------------------------------------------------------------------------------------------------------
 class Serving:
     """A small decoder's serving state: a linear model of keys, values, queries and logits from token ids."""
