@@ -265,6 +265,30 @@ def build_fp4_attention(head_dim: int, force: bool = False) -> Path:
 CALLS_SOURCE = "checked_calls.cpp"
 
 
+def _find_cxx() -> str:
+    """A compiler of host code: the system's, or the one that comes with hipcc."""
+    candidates = [os.environ.get("CXX"), shutil.which("g++"), shutil.which("c++")]
+    try:
+        hipcc = Path(find_hipcc())
+        candidates += [str(folder / "amdclang++") for folder in (hipcc.parent, hipcc.resolve().parent)]
+    except BuildError:
+        pass
+    for candidate in candidates:
+        if candidate and Path(candidate).is_file():
+            return candidate
+    raise BuildError("no C++ compiler was found (looked at $CXX, g++, c++ and beside hipcc); the checked calls cannot be built")
+
+
+def build_calls_if_possible(force: bool = False) -> Path | None:
+    """``build_calls``, or None where the module cannot be built: without it calls go through Python's checks, so that a build
+    does not fail for it."""
+    try:
+        return build_calls(force)
+    except BuildError as exc:
+        print(f"[lockstep_amd] without the checked calls: {exc}", file=sys.stderr, flush=True)
+        return None
+
+
 def build_calls(force: bool = False) -> Path:
     """The extension module ``lockstep_calls`` (host code), for the torch and the Python that run."""
     import torch
@@ -281,9 +305,7 @@ def build_calls(force: bool = False) -> Path:
         for folder in lib_dirs():
             if (folder / name).is_file():
                 return folder / name
-    compiler = next((c for c in (os.environ.get("CXX"), shutil.which("g++"), shutil.which("c++")) if c and Path(c).is_file()), None)
-    if compiler is None:
-        raise BuildError("no C++ compiler was found (looked at $CXX, g++ and c++); the checked calls cannot be built")
+    compiler = _find_cxx()
     for folder in lib_dirs():
         if not _writable(folder):
             continue
@@ -337,9 +359,9 @@ def build_all(head_dims=DEFAULT_HEAD_DIMS, force: bool = True, mutants: bool = T
     talking-heads attention library of each shape, the sink attention
     library of each key and value size, the experts and the serving library, the checked calls and attention over pages in 4 bits for each
     of its head sizes, a few at a time; with ``mutants`` also the control
-    libraries of the tests."""
+    libraries of the tests.  The checked calls are left out where the machine cannot build them."""
     jobs = [lambda: build_core(force), lambda: build_mixers(force), lambda: build_experts(force)]
-    jobs += [lambda: build_serving(force), lambda: build_calls(force)] + [lambda d=d: build_fp4_attention(d, force) for d in fp4_head_dims]
+    jobs += [lambda: build_serving(force), lambda: build_calls_if_possible(force)] + [lambda d=d: build_fp4_attention(d, force) for d in fp4_head_dims]
     jobs += [lambda shape=shape: build_sink(*shape, force) for shape in sink_shapes]
     jobs += [lambda d=d: build_attention(d, force) for d in head_dims]
     jobs += [lambda shape=shape: build_talking(*shape, force) for shape in talking_shapes]
@@ -364,4 +386,4 @@ def build_all(head_dims=DEFAULT_HEAD_DIMS, force: bool = True, mutants: bool = T
             t.join()
     if errors:
         raise errors[0]
-    return results
+    return [path for path in results if path is not None]

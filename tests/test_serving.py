@@ -6,6 +6,7 @@ from __future__ import annotations
 import ctypes
 import random
 import threading
+from pathlib import Path
 
 import pytest
 import torch
@@ -249,3 +250,45 @@ def test_pages_are_fp4_pages():
                      lambda: k.fp4_attention(torch.zeros(2, 32), 1, 1, 32, pages, i(1, 2), i(2), i(1), 2, 8, torch.zeros(2, 32), 1.0)):
             with pytest.raises(KernelError, match="Fp4Pages"):
                 call()
+
+
+def test_checked_calls_without_a_compiler_of_the_system(monkeypatch, tmp_path):
+    """With hipcc alone the module is built by the compiler that comes with it."""
+    from importlib.machinery import ExtensionFileLoader
+    from importlib.util import module_from_spec, spec_from_loader
+
+    hipcc = kernel_build.find_hipcc()
+    monkeypatch.delenv("CXX", raising=False)
+    monkeypatch.setenv("HIPCC", hipcc)
+    monkeypatch.setattr(kernel_build.shutil, "which", lambda name: None)
+    monkeypatch.setattr(kernel_build, "lib_dirs", lambda: [tmp_path])
+    path = kernel_build.build_calls(force=True)
+    loader = ExtensionFileLoader("lockstep_calls", str(path))
+    module = module_from_spec(spec_from_loader("lockstep_calls", loader))
+    loader.exec_module(module)
+    assert module.fp4_write(0, 0, torch.zeros(1), torch.zeros(1), torch.zeros(1), None) is False
+
+
+def test_a_build_goes_on_without_the_checked_calls(monkeypatch, capsys):
+    made = []
+
+    def stub(name):
+        def build(*args, **kwargs):
+            made.append(name)
+            return Path(name)
+        return build
+
+    for name in dir(kernel_build):
+        if name.startswith("build_") and name not in ("build_all", "build_calls_if_possible"):
+            monkeypatch.setattr(kernel_build, name, stub(name))
+
+    def fails(force=False):
+        raise kernel_build.BuildError("no Python.h")
+
+    monkeypatch.setattr(kernel_build, "build_calls", fails)
+    paths = kernel_build.build_all()
+    assert len(paths) == len(made) > 20 and all(isinstance(p, Path) for p in paths)
+    assert "no Python.h" in capsys.readouterr().err
+    monkeypatch.setattr(kernel_build, "build_serving", fails)
+    with pytest.raises(kernel_build.BuildError):
+        kernel_build.build_all()
