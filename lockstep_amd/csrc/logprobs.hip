@@ -335,7 +335,8 @@ __device__ __forceinline__ void first_equal(FinishShared& sh, const T* __restric
   __syncthreads();
 }
 
-// What is left when every stream's lanes have their sums: a workgroup of kRowThreads, wave w with stream w.
+// What is left when every stream's lanes have their sums: a workgroup of kRowThreads, wave w with stream w.  Rows have three pieces
+// at least (shorter ones are a wave's), of which two are whole: 32 parts have logits, as many as may be wanted.
 template <typename T>
 __device__ __forceinline__ void finish_row(FinishShared& sh, const float* __restrict__ set_max, LaneSums mine, int before,
                                            const T* __restrict__ row, int vocab, int pieces, int given, float given_logit,
@@ -389,12 +390,7 @@ __device__ __forceinline__ void finish_row(FinishShared& sh, const float* __rest
       const auto y = __builtin_amdgcn_permlane32_swap(part, part, false, false);
       part = max((unsigned int)y[0], (unsigned int)y[1]);
     }
-    // (rows of one or two pieces: the lanes of their two waves are the parts)
-    if (pieces <= 2) {
-      if (w < 2) sh.part[w * 64 + lane] = lane_key;
-    } else if (lane < 16) {
-      sh.part[w * 16 + lane] = part;
-    }
+    if (lane < 16) sh.part[w * 16 + lane] = part;
     __syncthreads();
     {  // how many parts are larger: a quarter of the comparisons a thread
       const int mine = t & (kParts - 1), from = (t / kParts) * (kParts / 4);
@@ -761,6 +757,7 @@ inline bool logprobs_short(int rows, int vocab) {
 }
 // With fewer rows than compute units a workgroup a row leaves units idle; a wave a piece pays for its second launch once the
 // streams have more than two pieces (8 rows of 15,000 logits: 6.5 us by rows, 7.8 by pieces; of 60,000: 9.9 and 8.4).
+// (Fewer rows than that fit a grid's y.)
 inline bool logprobs_by_pieces(int rows, int vocab) { return rows < compute_units() && logprob_pieces(vocab) > 2 * kStreams; }
 
 template <typename T>
@@ -786,7 +783,6 @@ int run_logprobs(const void* logits, long ld, const int* tokens, int rows, int v
                                                                        top_logprobs);
     });
   } else if (logprobs_by_pieces(rows, vocab)) {
-    LS_REQUIRE(rows <= 65535, "token_logprobs: %d rows", rows);
     if (lds > 48 * 1024) {
       const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(logprobs_fold_kernel<T>),
                                                hipFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024 + 1024);
