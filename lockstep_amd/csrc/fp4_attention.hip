@@ -525,15 +525,12 @@ __device__ __forceinline__ void walk_keys_by_pages(Rows<T, NT>& rows, const Fp4A
   int base = first >> shift;  // the entry that lane 0 has
   int now = table_row[min(base + lane, a.columns - 1)], later = table_row[min(base + 64 + lane, a.columns - 1)];
   const auto load = [&](KeyTile& tile, int t0) LS_INLINED {
-    if (((t0 + 16) >> shift) - base >= 64) {  // (uniform; two neighbouring entries: never more than one run behind)
+    // (uniform.  Tiles begin at multiples of 32, and so does the first run: both halves of a tile lie in one run.  A step is eight
+    // entries at most: never more than one run ahead.)
+    if (__builtin_expect(((t0 + 16) >> shift) - base >= 64, 0)) {  // (said to be rare: without it heads of 128 spill two registers)
       base += 64;
       now = later;
       later = table_row[min(base + 64 + lane, a.columns - 1)];
-      if ((t0 >> shift) - base >= 64 || (t0 >> shift) < base) {  // the tile lies across two runs, or far behind: begin there
-        base = t0 >> shift;
-        now = table_row[min(base + lane, a.columns - 1)];
-        later = table_row[min(base + 64 + lane, a.columns - 1)];
-      }
     }
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
