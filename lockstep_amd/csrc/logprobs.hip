@@ -192,6 +192,13 @@ struct FinishShared {
   int wave_count[kStreams];
 };
 
+// What the wave's lanes have written to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_handover() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Exclusive sum over the workgroup's threads; `total` gets the whole sum.
 __device__ __forceinline__ int row_scan(int v, int* __restrict__ wave_sums, int& total) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -293,8 +300,9 @@ __device__ __forceinline__ void list_tokens(FinishShared& sh, const float* __res
     }
   if (listed <= kMaxSets) {
     constexpr int VEC = Row<T>::VEC;
+    wave_handover();
 #pragma unroll 4
-    for (int i = 0; i < listed * kLaneElems; i += 64) {  // (a wave reads what it has written itself)
+    for (int i = 0; i < listed * kLaneElems; i += 64) {
       const int j = i + lane, set = sh.set_list[w][min(j / kLaneElems, listed - 1)], e = j % kLaneElems;
       const int id = (set >> 6) * kPiece + ((e / VEC) * 64 + (set & 63)) * VEC + e % VEC;
       const unsigned int key = logit_key(to_f32(row[min(id, vocab - 1)]));
@@ -682,9 +690,7 @@ __global__ __launch_bounds__(kShortThreads) void logprobs_short_kernel(const T* 
         sets += __popcll(hit);
       }
     if (sets <= kShortList) {
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      wave_handover();
       listed = 0;
       // two sets of 32 at a time (or more of fewer); vectors behind the row's end do not count
       for (int i = 0; i < sets * kElems; i += 64) {
@@ -726,9 +732,7 @@ __global__ __launch_bounds__(kShortThreads) void logprobs_short_kernel(const T* 
     if (listed < top)
       listed = list_in_order<T>(sh, w, lane, row, vocab, listed, top - listed, [&](unsigned int key) LS_INLINED { return key == bound; });
   }
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  wave_handover();
   // their order: a token's place is how many of the others come before it
   for (int c0 = 0; c0 < listed; c0 += 64) {  // (uniform)
     const int c = min(c0 + lane, listed - 1);
