@@ -22,12 +22,14 @@
 // row's result does not depend on what else is in the step.
 //
 // What bounds it: decoding, the bytes (17/32 a key element): 4 requests of 131,071 keys (32 heads over 8, 570 MB) are read in
-// 107 us, 5.3 TB/s, and their splits folded in 5; 64 of 1 to 8,192 (367 MB) take 84 and 5, 64 of 4,608 each (321 MB) 75 in all.
+// 105 us, 5.4 TB/s, and their splits folded in 7; 64 of 1 to 8,192 (367 MB) take 79 and 4.5, 64 of 4,608 each (321 MB) 64 to 67 in all.
 // Some 6 vector instructions a key and lane column are two thirds of what that leaves room for.  Prompts, the vector unit next
 // to the matrix units: a tile of 16 rows by 32 keys has 16 products of 16 cycles and some 60 vector instructions of 4, of them
 // 8 exponentials of 16, and two waves a SIMD overlap them in part (6,660 rows of 32 heads behind up to 8,192 keys in pages of 16:
-// 770 us, 880 TFLOP/s, where a large product of the library reaches 1,190).  Two groups of waves a barrier apart, one at the matrix and
-// one at the vector units, were slower (885 us for 770: alone on its SIMD, a wave waits for its own results).
+// 780 us, 870 TFLOP/s, where a large product of the library reaches 1,190).  Two groups of waves a barrier apart, one at the matrix and
+// one at the vector units, were slower (885 us for 770: alone on its SIMD, a wave waits for its own results).  The float32 path
+// is at the matrix units' rate there (4 times 2,048 rows behind 8,192 keys 2,450 us, 393 TFLOP/s of three products each); decoding,
+// its three products and two waves a SIMD take 95 us for 64 requests of 4,608 keys and 152 for 4 of 131,071.
 
 #include "fp4.h"
 #include "fp4_attention_api.h"
@@ -69,9 +71,11 @@ template <typename T> constexpr int kPromptTiles = std::is_same_v<T, float> ? 1 
 template <typename T> constexpr int kPromptWaves = D <= 128 ? 2 : 1;
 
 // Keys a split of a request of few rows covers, by how many keys its rows see and how many heads do so: some 512 workgroups
-// a request at most, and no split too short to be worth its launch.  One split leaves out the second launch.  (8 requests of
-// 532 keys, 8 heads: one split 8.1 us, two 9.4; 64 of up to 8,192: splits of 512 keys 113 us, of 512 and 1,024 96, of 2,048
-// 94; 4 of 131,071: 1,024 keys 134 us, 2,048 122.)
+// a request at most, and no split too short to be worth its launch.  One split leaves out the second launch.  (32 heads over 8,
+// shortest splits of 512 keys / of 512 up to 4,096 keys and 1,024 behind / of 512 and 2,048, us: 64 requests of 1 to 8,192 keys
+// 65.6 / 62.8 / 62.1, 64 of 8,192 122 / 116 / 111, 128 of 1 to 16,384 264 / 238 / 226, 8 of 8,192 21.2 / 19.4 / 20.1, one of 8,192
+// 10.6 / 12.6 / 18.3, one of 32,768 16.2 / 16.1 / 20.0: longer ones would gain 5 % where requests fill the card and lose a quarter
+// to a half where they do not.  8 of 532, 16 heads: one split 7.4, two 9.7.)
 constexpr int kOneSplit = 768, kDecodeGroups = 512;
 __host__ __device__ inline int shortest_split(int span, int kv_heads) { return kv_heads < 4 ? 256 : span <= 4096 ? 512 : 1024; }
 __host__ __device__ inline int decode_split(int span, int kv_heads) {
