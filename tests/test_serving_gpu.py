@@ -433,6 +433,33 @@ def test_more_rows_or_keys_than_stated(heads, dtype):
     check_attention(out, q, heads, 2, 64, pool, table, offsets, [min(n, 950) for n in lengths], 16, 0)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("window", [0, 1000])
+def test_many_portions_behind_long_contexts(dtype, window):
+    """Splits' sums of requests of every size lie beside one another: portions of a few tokens, decoded tokens, requests that bring
+    nothing or more than stated, each with the bits that it has alone."""
+    heads, kv_heads, d, page = 8, 2, 64, 16
+    lengths = [2500, 1900, 1300, 2900, 3000, 700, 1100, 2600, 1700, 2200]
+    news = [33, 1, 5, 0, 9, 90, 1, 33, 2, 17]
+    g = torch.Generator().manual_seed(40)
+    pool, table = make_cache(g, lengths, kv_heads, d, page)
+    offsets = [0]
+    for n in news:
+        offsets.append(offsets[-1] + n)
+    q = torch.randn((offsets[-1] + 3, heads * d), generator=g).to(dtype).to(DEV)
+    out = run_attention(q, heads, kv_heads, d, pool, table, offsets, lengths, window, most=33)
+    left = news.index(90)                   # more rows than stated: left out
+    assert bool((out[offsets[left]:offsets[left + 1]] == 9).all()) and bool((out[offsets[-1]:] == 9).all())
+    whole = run_attention(q, heads, kv_heads, d, pool, table, offsets, lengths, window)
+    check_attention(whole, q, heads, kv_heads, d, pool, table, offsets, lengths, page, window)
+    whole[offsets[left]:offsets[left + 1]] = 9
+    assert torch.equal(out, whole)
+    for i, n in enumerate(news):
+        if n and i != left:
+            rows = slice(offsets[i], offsets[i + 1])
+            assert torch.equal(run_attention(q[rows], heads, kv_heads, d, pool, [table[i]], [0, n], [lengths[i]], window), out[rows]), i
+
+
 @pytest.mark.parametrize("news", [1, 30])
 def test_windows_as_wide_as_the_context(news):
     g = torch.Generator().manual_seed(10)
